@@ -29,7 +29,14 @@ SOURCES = [
     "comm.cu",
     "moe.cu",
     "fp8.cu",
+    "rotary.cu",
+    "sandwich_norm.cu",
+    "adamw_tensors.cu",
 ]
+
+# Sources compiled with IEEE divisions, square roots and denormals: angles of far positions, and moments whose
+# bits the CPU restatement of the optimizer has to give again.
+IEEE_SOURCES = {"rotary.cu", "sandwich_norm.cu", "adamw_tensors.cu"}
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -38,6 +45,10 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC",
     "-shared",
 ]
+
+
+def nvcc_flags(name: str) -> list[str]:
+    return [f for f in NVCC_FLAGS if not (f == "--use_fast_math" and name in IEEE_SOURCES)]
 
 
 def nvcc_path() -> str:
@@ -52,7 +63,7 @@ def _digest(src: Path) -> str:
     h.update(src.read_bytes())
     for hdr in sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")):
         h.update(hdr.read_bytes())
-    h.update(" ".join(NVCC_FLAGS).encode())
+    h.update(" ".join(nvcc_flags(src.name)).encode())
     return h.hexdigest()
 
 
@@ -96,7 +107,7 @@ def build_one(name: str, verbose: bool = False, force: bool = False) -> Path:
     digest = _digest(src)
     if not force and out.exists() and stamp.exists() and stamp.read_text() == digest:
         return out
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", str(CSRC), "-o", "@OUT@", str(src)]
+    cmd = [nvcc_path(), *nvcc_flags(name), "-I", str(CSRC), "-o", "@OUT@", str(src)]
     if verbose:
         cmd[1:1] = ["-Xptxas", "-v"]
     return _locked_build(out, digest, cmd, name, verbose, force)

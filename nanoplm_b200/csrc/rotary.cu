@@ -1,0 +1,221 @@
+// Rotary positions of queries and keys in one launch: half (i, i + R/2) or interleaved (2i, 2i + 1) pairs, the first R of a
+// head's D channels, any number of query and key heads, any token, head and batch strides.
+//
+// For pair i of a token at position p, with a = p w_i, and the factor f of the frequency scaling:
+//   y1 = f (x1 cos a - x2 sin a),  y2 = f (x2 cos a + x1 sin a);  the gradient is the transpose, sin negated.
+//
+// Bound by memory: a pair costs 4 multiplications, and its cos and sin serve all heads of the token. So a block takes a few
+// tokens, forms their cos and sin once in shared memory and then streams the heads. No table: a table in fp32 ends at a
+// largest position, and fp32 angles are off by p 2^-24 radians. Here p w_i is formed in fp64 as a number of turns, whose
+// whole part is dropped before the rest becomes a fp32 argument in [-1, 1] half turns of sincospi, good to fp32's last
+// bits for every position that a 32-bit integer holds.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace nplm {
+
+constexpr int ROT_THREADS = 256;
+constexpr int ROT_PAIRS = 2048;     // cos and sin of a block's tokens: 16 KB
+constexpr int ROT_UNROLL = 4;       // heads that a thread has in flight
+
+struct RotaryArgs {
+  const void* x[2];                 // queries, keys (keys may have no heads)
+  void* y[2];
+  long long xb[2], xt[2], xh[2], yb[2], yt[2], yh[2];   // strides in elements: batch, token, head
+  int heads[2];
+  const void* pos;
+  long long pb, pt;                 // strides of the positions
+  int pos64;
+  const double* freq;               // [R / 2] radians a position
+  float factor, sign;
+  long long tokens;                 // batch * seq
+  long long seq;
+  int D, R, tile;                   // tile: tokens a block
+  int in_place;                     // the channels from R on are there already
+};
+
+template <typename T, int VE>
+struct alignas(sizeof(T) * VE) RotVec {
+  T v[VE];
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// VE: elements an access, a divisor of R / 2, of D - R and of all strides, with the addresses on its multiples. A thread's
+// item is VE pairs of a head (two accesses) or up to 2 VE channels behind the rotated ones. Its place in the head stays the
+// same, so that only token and head advance from item to item.
+template <typename T, int VE, bool INTER>
+__global__ void __launch_bounds__(ROT_THREADS)
+rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  using Vec = RotVec<T, VE>;
+  __shared__ __align__(16) float sm_cos[ROT_PAIRS], sm_sin[ROT_PAIRS];
+  grid_chain();
+  const int half = a.R >> 1;
+  const long long t0 = static_cast<long long>(blockIdx.x) * a.tile;
+  const int tokens = static_cast<int>(min(static_cast<long long>(a.tile), a.tokens - t0));
+  for (int j = threadIdx.x; j < tokens * half; j += ROT_THREADS) {
+    const int tok = j / half, i = j - tok * half;
+    const long long t = t0 + tok, b = t / a.seq, s = t - b * a.seq;
+    const long long at = b * a.pb + s * a.pt;
+    const double p = a.pos64 ? static_cast<double>(static_cast<const long long*>(a.pos)[at])
+                             : static_cast<double>(static_cast<const int*>(a.pos)[at]);
+    const double turns = p * (a.freq[i] * 0.15915494309189535);   // 1 / (2 pi)
+    const float rest = static_cast<float>(turns - rint(turns));
+    float sn, cs;
+    sincospif(2.f * rest, &sn, &cs);
+    sm_cos[j] = a.factor * cs;
+    sm_sin[j] = a.factor * a.sign * sn;
+  }
+  __syncthreads();
+
+  const int rot = half / VE;                                          // items a head: pairs,
+  const int behind = a.in_place ? 0 : (a.D - a.R + 2 * VE - 1) / (2 * VE);   // and what is copied
+  const int per_head = rot + behind;
+  const int stride = ROT_THREADS / per_head;                          // heads that the block takes at a time
+  const int first = threadIdx.x / per_head, c = threadIdx.x - first * per_head;
+  if (first >= stride) return;
+  const int heads = a.heads[0] + a.heads[1], rows = tokens * heads;
+  const int step_t = stride / heads, step_h = stride - step_t * heads;
+  int tok = first / heads, h = first - tok * heads;
+  const bool pairs = c < rot;
+  // offsets of the two accesses in a head
+  const int i = c * VE;
+  const int o0 = pairs ? (INTER ? 2 * i : i) : a.R + (c - rot) * 2 * VE;
+  const int o1 = pairs ? (INTER ? 2 * i + VE : i + half) : o0 + VE;
+  const bool second = o1 < a.D;
+
+  for (int row = first; row < rows; row += ROT_UNROLL * stride) {
+    Vec v0[ROT_UNROLL], v1[ROT_UNROLL];
+    T* to[ROT_UNROLL];
+    int at[ROT_UNROLL];
+#pragma unroll
+    for (int u = 0; u < ROT_UNROLL; ++u) {
+      to[u] = nullptr;
+      if (row + u * stride < rows) {
+        const int k = h >= a.heads[0];
+        const int hh = h - (k ? a.heads[0] : 0);
+        const long long t = t0 + tok;
+        long long b = 0, s = t;
+        if (a.seq != a.tokens) {
+          b = t / a.seq;
+          s = t - b * a.seq;
+        }
+        const T* from = static_cast<const T*>(a.x[k]) + b * a.xb[k] + s * a.xt[k] + hh * a.xh[k];
+        to[u] = static_cast<T*>(a.y[k]) + b * a.yb[k] + s * a.yt[k] + hh * a.yh[k];
+        at[u] = tok * half + i;
+        v0[u] = *reinterpret_cast<const Vec*>(from + o0);
+        if (second) v1[u] = *reinterpret_cast<const Vec*>(from + o1);
+        tok += step_t;
+        h += step_h;
+        if (h >= heads) {
+          h -= heads;
+          ++tok;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < ROT_UNROLL; ++u) {
+      if (to[u] != nullptr) {
+        if (pairs) {
+          Vec w0, w1;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float cs = sm_cos[at[u] + e], sn = sm_sin[at[u] + e];
+            // the two members of pair e of this item
+            const int j0 = INTER ? 2 * e : e, j1 = INTER ? 2 * e + 1 : VE + e;
+            const float x1 = to_f32(j0 < VE ? v0[u].v[j0 % VE] : v1[u].v[j0 % VE]);
+            const float x2 = to_f32(j1 < VE ? v0[u].v[j1 % VE] : v1[u].v[j1 % VE]);
+            const T y1 = from_f32<T>(x1 * cs - x2 * sn), y2 = from_f32<T>(x2 * cs + x1 * sn);
+            if (j0 < VE) w0.v[j0 % VE] = y1; else w1.v[j0 % VE] = y1;
+            if (j1 < VE) w0.v[j1 % VE] = y2; else w1.v[j1 % VE] = y2;
+          }
+          v0[u] = w0;
+          v1[u] = w1;
+        }
+        *reinterpret_cast<Vec*>(to[u] + o0) = v0[u];
+        if (second) *reinterpret_cast<Vec*>(to[u] + o1) = v1[u];
+      }
+    }
+  }
+}
+
+template <typename T, int VE>
+static cudaError_t launch_rotary(const RotaryArgs& a, int interleaved, unsigned blocks, cudaStream_t st) {
+  const long long n = a.tokens * (a.heads[0] + a.heads[1]) * a.D;
+  return interleaved ? launch_when(n <= CHAIN_ELEMENTS, rotary_kernel<T, VE, true>, blocks, ROT_THREADS, 0, st, a)
+                     : launch_when(n <= CHAIN_ELEMENTS, rotary_kernel<T, VE, false>, blocks, ROT_THREADS, 0, st, a);
+}
+
+template <typename T>
+static cudaError_t launch_rotary(const RotaryArgs& a, int ve, int interleaved, unsigned blocks, cudaStream_t st) {
+  if (ve * sizeof(T) >= 16) return launch_rotary<T, 16 / sizeof(T)>(a, interleaved, blocks, st);
+  if (ve >= 4) return launch_rotary<T, 4>(a, interleaved, blocks, st);
+  if (ve >= 2) return launch_rotary<T, 2>(a, interleaved, blocks, st);
+  return launch_rotary<T, 1>(a, interleaved, blocks, st);
+}
+
+}  // namespace nplm
+
+using namespace nplm;
+
+// dtype: 0 bf16, 1 fp16, 2 fp32. strides: batch, token and head of q, then of its output, then the same of k. k may be null
+// (k_heads 0). pos: int32 or int64 (pos64), strides pb, pt. D at most 512.
+extern "C" int nplm_rotary_qk(const void* q, void* q_out, const void* k, void* k_out, const long long* strides, int q_heads,
+                              int k_heads, const void* pos, int pos64, long long pb, long long pt, const double* freq,
+                              float factor, int transposed, long long batch, long long seq, int D, int R, int dtype,
+                              int interleaved, cudaStream_t st) {
+  if (batch < 0 || seq < 0 || q_heads < 1 || k_heads < 0 || D < 2 || D > 512 || R < 2 || R > D || R % 2 || dtype < 0 ||
+      dtype > 2)
+    return -1;
+  if (batch == 0 || seq == 0) return 0;
+  RotaryArgs a;
+  a.x[0] = q; a.x[1] = k; a.y[0] = q_out; a.y[1] = k_out;
+  a.heads[0] = q_heads; a.heads[1] = k_heads;
+  for (int j = 0; j < 2; ++j) {
+    a.xb[j] = strides[6 * j]; a.xt[j] = strides[6 * j + 1]; a.xh[j] = strides[6 * j + 2];
+    a.yb[j] = strides[6 * j + 3]; a.yt[j] = strides[6 * j + 4]; a.yh[j] = strides[6 * j + 5];
+  }
+  a.pos = pos; a.pos64 = pos64; a.pb = pb; a.pt = pt; a.freq = freq; a.factor = factor;
+  a.sign = transposed ? -1.f : 1.f;
+  a.tokens = batch * seq; a.seq = seq; a.D = D; a.R = R;
+  a.in_place = q == q_out && (k_heads == 0 || k == k_out);
+  // the widest access, up to 16 bytes, that sizes, strides and addresses allow
+  const int size = dtype == 2 ? 4 : 2;
+  int ve = 16 / size;
+  auto fits = [&](int v) {
+    if ((R / 2) % v || (D - R) % v) return false;
+    for (int j = 0; j < (k_heads ? 2 : 1); ++j) {
+      const long long all = a.xb[j] | a.xt[j] | a.xh[j] | a.yb[j] | a.yt[j] | a.yh[j];
+      if (all % v || reinterpret_cast<uintptr_t>(a.x[j]) % (v * size) || reinterpret_cast<uintptr_t>(a.y[j]) % (v * size))
+        return false;
+    }
+    return true;
+  };
+  while (ve > 1 && !fits(ve)) ve /= 2;
+  const int half = R / 2;
+  const int per_token = (q_heads + k_heads) * (half / ve + (a.in_place ? 0 : (D - R + 2 * ve - 1) / (2 * ve)));
+  // enough tokens that every thread has its unrolled items, as long as their cos and sin fit
+  int tile = (ROT_THREADS * ROT_UNROLL + per_token - 1) / per_token;
+  if (tile > ROT_PAIRS / half) tile = ROT_PAIRS / half;
+  a.tile = tile;
+  const long long blocks = (a.tokens + tile - 1) / tile;
+  if (blocks > 0x7fffffffLL) return -2;
+  const unsigned n = static_cast<unsigned>(blocks);
+  cudaError_t e;
+  if (dtype == 0) e = launch_rotary<__nv_bfloat16>(a, ve, interleaved, n, st);
+  else if (dtype == 1) e = launch_rotary<__half>(a, ve, interleaved, n, st);
+  else e = launch_rotary<float>(a, ve, interleaved, n, st);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return static_cast<int>(cudaGetLastError());
+}

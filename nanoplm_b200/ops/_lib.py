@@ -60,7 +60,7 @@ def loaded_libraries() -> list[str]:
 
 
 def typed(lib_name: str, function: str, spec: str):
-    """The C function with its argument types declared ("p" pointer, "i" int, "f" float), so that calls pass plain
+    """The C function with its argument types declared ("p" pointer, "i" int, "l" 64-bit int, "f" float), so that calls pass plain
     Python numbers: half the cost of wrapping 20 - 26 arguments one by one."""
     f = getattr(lib(lib_name), function)
     if f.argtypes is None:
@@ -68,7 +68,7 @@ def typed(lib_name: str, function: str, spec: str):
     return f
 
 
-_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}
+_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
 
 def raw_stream() -> int:

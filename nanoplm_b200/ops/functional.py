@@ -90,6 +90,9 @@ class _NoGradCtx:
     def mark_non_differentiable(self, *tensors):
         pass
 
+    def set_materialize_grads(self, value):
+        pass
+
 
 def functions_observed() -> bool:
     """Somebody has to see the autograd Functions themselves: a forward-mode level, a function transform, or a tracer
@@ -388,6 +391,62 @@ def norm(x, w, eps: float = 1e-5, rms: bool = False):
     return y.to(x.dtype)
 
 
+class _SandwichFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, post, nxt, gate, scale, eps, rms, sigmoid, with_next):
+        ctx.set_materialize_grads(False)
+        rows = lambda t: t if t is None or t.dim() < 2 or t.stride(1) == 1 else t.contiguous()
+        x, f, gate = rows(x), rows(f), rows(gate)
+        y, h, stats = K.sandwich_fwd(x, f, post, nxt, gate, scale, eps, rms, sigmoid, with_next,
+                                     stats=any(ctx.needs_input_grad))
+        ctx.save_for_backward(x, f, post, nxt, gate, scale, stats)
+        ctx.how = (rms, sigmoid)
+        ctx.refs = (nxt, post, scale, gate)     # (saved-tensor hooks may give back copies, without the running gradients)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        if dy is None and dh is None:
+            return (None,) * 10
+        x, f, post, nxt, gate, scale, stats = ctx.saved_tensors
+        rms, sigmoid = ctx.how
+        rows = lambda t: t if t is None or t.stride(1) == 1 else t.contiguous()
+        need = ctx.needs_input_grad
+        wanted = (need[3] and dh is not None, need[2], need[5], need[4] and gate is not None and gate.dim() == 1)
+        sums, add = [], []
+        for p, want in zip(ctx.refs, wanted):
+            running = want and _has_main_grad(p) and p.main_grad.dtype == torch.float32 and p.main_grad.is_contiguous()
+            add.append(running)
+            sums.append(None if not want else p.main_grad if running else torch.empty_like(p, memory_format=torch.contiguous_format))
+        dx, df, dg = K.sandwich_bwd(rows(dy), rows(dh), x, f, stats, post, nxt, gate, scale, rms, sigmoid, sums, add)
+        dnext, dpost, dscale, dgate = (None if a else s for s, a in zip(sums, add))
+        if dg is not None:
+            dgate = dg
+        if need[3] and dh is None and not _has_main_grad(ctx.refs[0]):
+            dnext = torch.zeros_like(nxt)
+        return dx, df, dpost, dnext, dgate, dscale, None, None, None, None
+
+
+def sandwich_norm(x, f, post=None, next=None, *, gate=None, sigmoid: bool = False, scale=None, eps: float = 1e-5,
+                  rms: bool = False, with_next: bool = True):
+    """The end of a residual block with norms before and after it: y = scale x + g norm(f) post and h = norm(y) next, for the
+    block's input x and output f, both [T, C]; returns (y, h), h None without `with_next`.
+
+    post, next, scale: weights [C], or None for ones. gate: None for g = 1, weights [C], or values [T, C], of which the
+    sigmoid is taken with `sigmoid`. Norms are LayerNorm without bias, or RMSNorm."""
+    if sigmoid and (gate is None or gate.dim() != 2):
+        raise ValueError("sigmoid is for gates of tokens [T, C]")
+    K.check_sandwich(x, f, gate, post, next, scale, sigmoid)
+    if x.is_cuda and x.dtype in K.ROW_TYPES and x.shape[1] <= K.SANDWICH_MAX_C:
+        return _call(_SandwichFn, x, f, post, next, gate, scale, eps, rms, sigmoid, with_next)
+    n = norm(f.float(), post, eps, rms)
+    if gate is not None:
+        n = n * (torch.sigmoid(gate.float()) if sigmoid else gate.float())
+    y = n + (x.float() if scale is None else scale.float() * x.float())
+    return y.to(x.dtype), (norm(y, next, eps, rms).to(x.dtype) if with_next else None)
+
+
 class _EmbedNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, table, w, eps, rms):
@@ -456,6 +515,84 @@ def rope_qkv(qkv, pos, cos, sin, H: int, D: int):
         return (tf * c + torch.cat((-t2, t1), -1) * s).to(t.dtype)
 
     return torch.stack((rot(x[:, 0]), rot(x[:, 1]), x[:, 2]), dim=1).reshape(T, 3 * H * D)
+
+
+def rotary_frequencies(rotated: int, theta: float, scaling: dict | None = None, device=None) -> tuple[torch.Tensor, float]:
+    """(frequencies fp64 [rotated / 2] in radians a position, factor on cos and sin) for `rotary`.
+
+    scaling {"type": ..., "factor": s > 1} stretches the positions that a model was trained on (`original_max_position`)
+    s-fold: "linear" divides every frequency by s; "ntk" raises theta so that the slowest pair turns s times slower and
+    the fastest as before; "yarn" (Peng et al., 2023) divides the frequencies of pairs that turn at most `beta_slow` (1) times in
+    the original context, keeps those above `beta_fast` (32) turns, blends between, and multiplies cos and sin by
+    0.1 ln s + 1 (or `attention_factor`)."""
+    if rotated < 2 or rotated % 2:
+        raise ValueError(f"an even number of channels rotates, got {rotated}")
+    at = torch.arange(0, rotated, 2, dtype=torch.float64, device=device) / rotated
+    if not scaling or scaling.get("type", "none") == "none":
+        return float(theta) ** -at, 1.0
+    kind, s = scaling["type"], float(scaling["factor"])
+    if s < 1.0:
+        raise ValueError(f"a scaling factor below 1: {s}")
+    if kind == "linear":
+        return float(theta) ** -at / s, 1.0
+    if kind == "ntk":
+        return (float(theta) * (s ** (rotated / (rotated - 2)) if rotated > 2 else 1.0)) ** -at, 1.0
+    if kind == "yarn":
+        w = float(theta) ** -at
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        if not 0 < slow < fast:
+            raise ValueError(f"beta_slow and beta_fast must be positive and in this order: {slow}, {fast}")
+        turns = float(scaling["original_max_position"]) * w / (2 * math.pi)
+        keep = ((turns.log() - math.log(slow)) / (math.log(fast) - math.log(slow))).clamp(0, 1)
+        factor = scaling.get("attention_factor")
+        return w / s * (1 - keep) + w * keep, float(0.1 * math.log(s) + 1.0 if factor is None else factor)
+    raise ValueError(f"unknown rotary scaling {kind!r}: none, linear, ntk or yarn")
+
+
+def _rotate_plain(x, positions, frequencies, factor, interleaved):
+    R = 2 * frequencies.numel()
+    a = positions.double()[..., None] * frequencies
+    c, s = (factor * a.cos()).to(torch.float32)[..., None, :], (factor * a.sin()).to(torch.float32)[..., None, :]
+    r, rest = x[..., :R].float(), x[..., R:]
+    x1, x2 = (r[..., 0::2], r[..., 1::2]) if interleaved else r.chunk(2, dim=-1)
+    y1, y2 = x1 * c - x2 * s, x2 * c + x1 * s
+    y = torch.stack((y1, y2), -1).flatten(-2) if interleaved else torch.cat((y1, y2), -1)
+    return torch.cat((y.to(x.dtype), rest), -1)
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, frequencies, factor, interleaved, transposed):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = (factor, interleaved, transposed)
+        unit = lambda t: t if t is None or t.stride(-1) == 1 else t.contiguous()
+        return K.rotary(unit(q), unit(k), positions, frequencies, factor, interleaved, transposed)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, frequencies = ctx.saved_tensors
+        factor, interleaved, transposed = ctx.how
+        if dq is None and dk is None:
+            return (None,) * 7
+        if dq is None:
+            dk, _ = _call(_RotaryFn, dk, None, positions, frequencies, factor, interleaved, not transposed)
+        else:
+            dq, dk = _call(_RotaryFn, dq, dk, positions, frequencies, factor, interleaved, not transposed)
+        return dq, dk, None, None, None, None, None
+
+
+def rotary(q, k=None, *, positions, frequencies, factor: float = 1.0, interleaved: bool = False):
+    """Rotary positions of queries and keys [T, heads, width] or [B, S, heads, width] (widths alike, any head counts, any strides):
+    (q', k'), or q' alone without k. positions: integers [T], [B, S] or [S]; frequencies (fp64) and factor from
+    `rotary_frequencies`: their 2 n first channels rotate, as pairs (i, i + n) or, interleaved, (2 i, 2 i + 1). Angles are
+    exact to fp32 for every 32-bit position: there is no table that ends."""
+    K.check_rotary(q, k, positions, frequencies)
+    if q.is_cuda and q.dtype in K.ROW_TYPES and q.shape[-1] <= K.ROTARY_MAX_WIDTH:
+        out = _call(_RotaryFn, q, k, positions, frequencies, factor, interleaved, False)
+        return out[0] if k is None else out
+    out = _rotate_plain(q, positions, frequencies, factor, interleaved)
+    return out if k is None else (out, _rotate_plain(k, positions, frequencies, factor, interleaved))
 
 
 # ------------------------------------------------------------------------------------- attention

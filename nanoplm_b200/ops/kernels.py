@@ -5,7 +5,8 @@ stream and returns output tensors. ``nanoplm_b200.ops.functional`` builds differ
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong
+from contextlib import nullcontext
+from ctypes import c_float, c_int, c_longlong, c_ubyte, c_void_p
 from functools import lru_cache
 
 import torch
@@ -35,6 +36,20 @@ def _dp(t: torch.Tensor | None):
 
 def _is_tracing() -> bool:
     return torch._C._is_tracing()
+
+
+ROW_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_NULL = nullcontext()
+
+
+def _device_of(first: torch.Tensor, *rest):
+    """A context in which the first tensor's device is the current one; ValueError where another tensor is elsewhere."""
+    if not first.is_cuda:
+        raise ValueError("the tensors must be on a CUDA device")
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    return _NULL if first.device.index == torch._C._cuda_getDevice() else torch.cuda.device(first.device)
 
 
 def _rowmajor(t: torch.Tensor, name: str) -> int:
@@ -328,6 +343,111 @@ def norm_bwd(dy, x, w, mean, rstd, *, rms=False, dres=None, dw=None, ids=None, d
     return dx
 
 
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_SIGMOID = 0, 1, 2, 3
+SANDWICH_MAX_C = 4096
+
+
+def check_sandwich(x, f, gate, post, nxt, scale, sigmoid) -> tuple[int, bool]:
+    """Checks the arguments of a sandwich norm; (gate mode, whether the [C] weights are fp32 beside other rows)."""
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be [T, C], got {tuple(x.shape)}")
+    C = x.shape[1]
+    if f.shape != x.shape or f.dtype != x.dtype:
+        raise ValueError(f"f must be {tuple(x.shape)} {x.dtype}, got {tuple(f.shape)} {f.dtype}")
+    mode = GATE_NONE
+    vectors = [("post", post), ("next", nxt), ("scale", scale)]
+    if gate is not None and gate.dim() == 1:
+        if sigmoid:
+            raise ValueError("a gate per channel is a weight: sigmoid is for gates of tokens")
+        mode = GATE_CHANNEL
+        vectors.append(("gate", gate))
+    elif gate is not None:
+        if gate.shape != x.shape or gate.dtype != x.dtype:
+            raise ValueError(f"gate must be [{C}] or {tuple(x.shape)} {x.dtype}, got {tuple(gate.shape)} {gate.dtype}")
+        mode = GATE_SIGMOID if sigmoid else GATE_TOKEN
+    kinds = set()
+    for name, v in vectors:
+        if v is not None:
+            if tuple(v.shape) != (C,) or not v.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous [{C}], got {tuple(v.shape)}")
+            kinds.add(v.dtype)
+    if len(kinds) > 1 or not kinds <= {x.dtype, torch.float32}:
+        raise ValueError(f"the [C] weights must all be {x.dtype} or all fp32, got {sorted(map(str, kinds))}")
+    return mode, bool(kinds) and kinds != {x.dtype}
+
+
+def _sandwich_rows(x, *rows):
+    if x.dtype not in ROW_TYPES or x.shape[1] > SANDWICH_MAX_C:
+        raise ValueError(f"x must be bf16, fp16 or fp32 with up to {SANDWICH_MAX_C} channels, got {x.dtype} {tuple(x.shape)}")
+    for t in (x, *rows):
+        if t is not None and t.dim() == 2 and t.stride(1) != 1 and t.shape[1] > 1 and t.numel():
+            raise ValueError("rows must have a contiguous last dim")
+
+
+def sandwich_fwd(x, f, post, nxt, gate=None, scale=None, eps: float = 1e-5, rms: bool = False, sigmoid: bool = False,
+                 with_next: bool = True, stats: bool = True):
+    """y = scale x + g norm(f) post, h = norm(y) nxt for rows of up to 4 096 channels: (y, h, stats), h None without
+    `with_next`. gate: None, [C], or like x (with `sigmoid` through one). post, nxt, scale: [C] or None, all of x's type
+    or all fp32. stats: fp32 [4, T] for `sandwich_bwd`."""
+    mode, param32 = check_sandwich(x, f, gate, post, nxt, scale, sigmoid)
+    _sandwich_rows(x, f, gate)
+    (T, C), kind = x.shape, ROW_TYPES[x.dtype]
+    with _device_of(x, f, gate, post, nxt, scale):
+        y = torch.empty((T, C), dtype=x.dtype, device=x.device)
+        h = torch.empty_like(y) if with_next else None
+        st = torch.empty((4, T), dtype=torch.float32, device=x.device) if stats else None
+        if T:
+            strides = (c_longlong * 3)(x.stride(0), f.stride(0), gate.stride(0) if mode >= GATE_TOKEN else 0)
+            rc = typed("sandwich_norm", "nplm_sandwich_fwd", "pppppppppplifiiiip")(
+                x.data_ptr(), f.data_ptr(), _dp(gate), _dp(post), _dp(nxt), _dp(scale), strides, y.data_ptr(), _dp(h), _dp(st),
+                T, C, eps, rms, mode, kind, param32, raw_stream())
+            check_rc(rc, "sandwich_fwd")
+            count_launch()
+    return y, h, st
+
+
+_SUM_KINDS = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
+
+
+def sandwich_bwd(dy, dh, x, f, stats, post, nxt, gate=None, scale=None, rms: bool = False, sigmoid: bool = False,
+                 sums=(None, None, None, None), add=(False, False, False, False)):
+    """Gradients of `sandwich_fwd` from dy and dh (one of them may be None): (dx, df, dgate of a gate of tokens or None).
+    sums: [C] tensors for the gradients of nxt, post, scale and a gate per channel, None where unwanted; written, or
+    with `add` (fp32 only) added to."""
+    mode, param32 = check_sandwich(x, f, gate, post, nxt, scale, sigmoid)
+    _sandwich_rows(x, f, gate, dy, dh)
+    (T, C), kind = x.shape, ROW_TYPES[x.dtype]
+    if dy is None and dh is None:
+        raise ValueError("dy or dh is needed")
+    for name, d in (("dy", dy), ("dh", dh)):
+        if d is not None and (d.shape != x.shape or d.dtype != x.dtype):
+            raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}, got {tuple(d.shape)} {d.dtype}")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (4, T) or not stats.is_contiguous():
+        raise ValueError(f"stats must be the fp32 [4, {T}] of the forward pass")
+    with _device_of(x, f, gate, post, nxt, scale, dy, dh, stats, *sums):
+        dx, df = torch.empty((T, C), dtype=x.dtype, device=x.device), torch.empty((T, C), dtype=x.dtype, device=x.device)
+        dg = torch.empty((T, C), dtype=x.dtype, device=x.device) if mode >= GATE_TOKEN else None
+        kinds = []
+        for s, a in zip(sums, add):
+            if s is not None and (s.numel() != C or not s.is_contiguous() or s.dtype not in _SUM_KINDS
+                                  or (a and s.dtype != torch.float32)):
+                raise ValueError(f"sums must be contiguous [{C}] tensors, fp32 where added to")
+            kinds.append(0 if s is None else 4 if a else _SUM_KINDS[s.dtype])
+        partial = None
+        if any(kinds):
+            blocks = typed("sandwich_norm", "nplm_sandwich_bwd_blocks", "li")(T, C) if T else 0
+            partial = torch.empty((4, blocks, C), dtype=torch.float32, device=x.device)
+        rs = lambda t: 0 if t is None else t.stride(0)
+        strides = (c_longlong * 5)(x.stride(0), f.stride(0), gate.stride(0) if mode >= GATE_TOKEN else 0, rs(dy), rs(dh))
+        rc = typed("sandwich_norm", "nplm_sandwich_bwd", "pppppppppp" + "pppppp" + "liiiiip")(
+            _dp(dy), _dp(dh), x.data_ptr(), f.data_ptr(), _dp(gate), _dp(post), _dp(nxt), _dp(scale), _dp(stats), strides,
+            dx.data_ptr(), df.data_ptr(), _dp(dg), _dp(partial), (c_void_p * 4)(*[_dp(s) for s in sums]),
+            (c_int * 4)(*kinds), T, C, rms, mode, kind, param32, raw_stream())
+        check_rc(rc, "sandwich_bwd")
+        count_launch((T > 0) + any(kinds))
+    return dx, df, dg
+
+
 # --------------------------------------------------------------------------- rope / swiglu / act
 def rope_(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, H: int,
           D: int, backward: bool = False) -> torch.Tensor:
@@ -340,6 +460,81 @@ def rope_(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Te
     check_rc(rc, "rope")
     count_launch()
     return qkv
+
+
+ROTARY_MAX_WIDTH = 512
+
+
+def _heads_last(t: torch.Tensor, name: str):
+    """(batch, tokens, heads, width) and the strides of the first three of a [T, H, D] or [B, S, H, D] tensor."""
+    if t.dim() == 3:
+        return (1, *t.shape), (0, t.stride(0), t.stride(1))
+    if t.dim() == 4:
+        return tuple(t.shape), t.stride()[:3]
+    raise ValueError(f"{name} must be [tokens, heads, width] or [batch, tokens, heads, width], got {tuple(t.shape)}")
+
+
+def check_rotary(q, k, positions, frequencies):
+    """Checks the arguments of a rotation: (sizes of q, its strides, heads of k, its strides, strides of the positions, number
+    of channels that rotate)."""
+    (B, S, H, D), qs = _heads_last(q, "q")
+    Hk, ks = 0, (0, 0, 0)
+    if k is not None:
+        (Bk, Sk, Hk, Dk), ks = _heads_last(k, "k")
+        if k.dim() != q.dim() or (Bk, Sk, Dk) != (B, S, D):
+            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in tokens or width")
+        if k.dtype != q.dtype:
+            raise ValueError(f"k must be {q.dtype}, got {k.dtype}")
+    if H < 1 or (k is not None and Hk < 1):
+        raise ValueError(f"at least one head is needed: got {H} and {Hk}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    if positions.dim() == 1 and positions.shape[0] == S:
+        ps = (0, positions.stride(0))
+    elif q.dim() == 4 and tuple(positions.shape) == (B, S):
+        ps = positions.stride()
+    else:
+        raise ValueError(f"positions {tuple(positions.shape)} do not fit q {tuple(q.shape)}")
+    R = 2 * frequencies.numel()
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not 2 <= R <= D or not frequencies.is_contiguous():
+        raise ValueError(f"frequencies must be a contiguous fp64 vector of 1 to {D // 2} pairs, got "
+                         f"{tuple(frequencies.shape)} {frequencies.dtype}")
+    return (B, S, H, D), qs, Hk, ks, ps, R
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, factor: float = 1.0,
+           interleaved: bool = False, transposed: bool = False, inplace: bool = False):
+    """Rotary positions on q [T, H, D] or [B, S, H, D] and, in the same launch, k with as many tokens, any number of heads and
+    the same width: (q', k'), contiguous, or with `inplace` q and k themselves.
+
+    bf16, fp16 or fp32; the last dimension contiguous, the others of any stride. positions: int32 or int64, [T], [B, S], or [S]
+    for all of a batch. frequencies: fp64 [R / 2], radians a position for each pair of the first R channels of a head; the
+    others pass. Pairs are (i, i + R / 2), or (2 i, 2 i + 1) with `interleaved`. factor multiplies cos and sin. transposed:
+    the gradient's rotation, backwards and with the same factor."""
+    (B, S, H, D), qs, Hk, ks, ps, R = check_rotary(q, k, positions, frequencies)
+    if q.dtype not in ROW_TYPES or D > ROTARY_MAX_WIDTH:
+        raise ValueError(f"q must be bf16, fp16 or fp32 with heads of up to {ROTARY_MAX_WIDTH} channels, got {q.dtype}, {D}")
+    for t, name in ((q, "q"), (k, "k")):
+        if t is not None and t.stride(-1) != 1 and t.numel():
+            raise ValueError(f"{name} must have a contiguous last dim")
+        if inplace and t is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{name} is written in place but has elements that share memory")
+    with _device_of(q, k, positions, frequencies):
+        if inplace:
+            qo, ko = q, k
+        else:
+            qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        qos = _heads_last(qo, "q")[1]
+        kos = (0, 0, 0) if ko is None else _heads_last(ko, "k")[1]
+        if B * S:
+            rc = typed("rotary", "nplm_rotary_qk", "pppppiipillpfilliiiip")(
+                q.data_ptr(), qo.data_ptr(), _dp(k), _dp(ko), (c_longlong * 12)(*qs, *qos, *ks, *kos), H, Hk,
+                positions.data_ptr(), positions.dtype == torch.int64, *ps, frequencies.data_ptr(), factor, transposed, B, S,
+                D, R, ROW_TYPES[q.dtype], interleaved, raw_stream())
+            check_rc(rc, "rotary")
+            count_launch()
+    return qo, ko
 
 
 def swiglu_fwd(pre: torch.Tensor) -> torch.Tensor:
@@ -553,6 +748,132 @@ def adamw_slots_(p, m, v, g, p_bf16, offsets, numels, decay, max_numel: int, sum
         stream_ptr())
     check_rc(rc, "adamw_slots")
     count_launch()
+
+
+MOMENT_BLOCK = 256      # elements of a tensor that share the offset of their 8-bit moments
+
+
+def moment_blocks(numels) -> int:
+    """Blocks that the moments of tensors of these sizes take: every tensor starts one."""
+    return sum(-(-n // MOMENT_BLOCK) for n in numels)
+
+
+def check_moments(m: torch.Tensor, v: torch.Tensor, scales: torch.Tensor | None) -> tuple[int, int]:
+    """(bits, blocks) of moments: fp32 without scales, or uint8 with scales uint8 [2, blocks]."""
+    bits = {torch.float32: 32, torch.uint8: 8}.get(m.dtype)
+    if bits is None or v.dtype != m.dtype or (bits == 8) != (scales is not None):
+        raise ValueError(f"moments must be fp32, or uint8 with scales: got {m.dtype}, {v.dtype}"
+                         f"{'' if scales is None else ' and scales'}")
+    blocks = m.numel() // MOMENT_BLOCK
+    if m.numel() != blocks * MOMENT_BLOCK or v.numel() != m.numel() or not (m.is_contiguous() and v.is_contiguous()):
+        raise ValueError(f"moments must be contiguous, equally large and whole blocks of {MOMENT_BLOCK}")
+    if scales is not None and (tuple(scales.shape) != (2, blocks) or scales.dtype != torch.uint8
+                               or not scales.is_contiguous()):
+        raise ValueError(f"scales must be a contiguous uint8 [2, {blocks}], got {tuple(scales.shape)} {scales.dtype}")
+    return bits, blocks
+
+
+def check_step(params, grads, copies, decay, m, v, scales, hyper, rng, sumsq) -> tuple[int, int, list[int]]:
+    """Checks the arguments of an AdamW step over tensors; (bits, blocks, sizes)."""
+    bits, blocks = check_moments(m, v, scales)
+    n = len(params)
+    if len(grads) != n or (copies is not None and len(copies) != n) or (decay is not None and len(decay) != n):
+        raise ValueError("params, grads, copies and decay must be equally long")
+    sizes = [p.numel() for p in params]
+    if sizes != [g.numel() for g in grads] or (copies is not None and sizes != [c.numel() for c in copies]):
+        raise ValueError("params, grads and copies must have the same sizes")
+    if moment_blocks(sizes) > blocks:
+        raise ValueError(f"the moments hold {blocks} blocks of {MOMENT_BLOCK}, the tensors take {moment_blocks(sizes)}")
+    for name, ts, allowed in (("params", params, (torch.float32, _BF16)), ("grads", grads, (torch.float32, _BF16)),
+                              ("copies", copies, (_BF16,))):
+        if ts:
+            kinds = {t.dtype for t in ts}
+            if len(kinds) != 1 or not kinds <= set(allowed):
+                raise ValueError(f"{name} must all be one of {allowed}, got {sorted(map(str, kinds))}")
+            if not all([t.is_contiguous() for t in ts]):
+                raise ValueError(f"{name} must be contiguous")
+    if copies is not None and n and params[0].dtype != torch.float32:
+        raise ValueError("bf16 copies are of fp32 params")
+    starts = [p.data_ptr() for p, k in zip(params, sizes) if k]
+    if len(set(starts)) != len(starts):
+        raise ValueError("a tensor is listed twice")
+    if hyper.dtype != torch.float32 or hyper.numel() != 9 or not hyper.is_contiguous():
+        raise ValueError("hyper must be 9 contiguous fp32 numbers")
+    if sumsq is not None and (sumsq.dtype != torch.float32 or sumsq.numel() != 1):
+        raise ValueError("sumsq must be one fp32 number")
+    if bits == 8 and (rng is None or rng.dtype != torch.int64 or rng.numel() != 1):
+        raise ValueError("8-bit moments need rng, one int64 number")
+    devices = {t.device for ts in (params, grads, copies or ()) for t in ts}
+    devices |= {t.device for t in (m, v, scales, hyper, rng, sumsq) if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"tensors on different devices: {sorted(map(str, devices))}")
+    return bits, blocks, sizes
+
+
+def adamw_tensors_(params, grads, exp_avg, exp_avg_sq, hyper, *, scales=None, rng=None, copies=None, decay=None,
+                   sumsq=None) -> None:
+    """One AdamW step (the update of `adamw_`) over a list of tensors, 128 to a launch.
+
+    params, grads: lists of contiguous tensors, fp32 or bf16 each. copies: bf16 copies of fp32 params, written too.
+    decay: which tensors the weight decay acts on (None: all). exp_avg, exp_avg_sq: fp32 [blocks * 256] in the order of the
+    tensors, each starting a block; or their 8-bit codes, uint8, with scales uint8 [2, blocks] (see `moment_values`) and rng,
+    an int64 number that must be another one each step: codes are rounded stochastically.
+    hyper: fp32 [9] lr, beta1, beta2, eps, weight decay, bias corrections 1 and 2, gradient scale, largest norm; with sumsq, the
+    sum of the gradients' squares, gradients are clipped to the largest norm. hyper, rng and sumsq are read on the
+    device, by a captured step at each replay."""
+    bits, blocks, sizes = check_step(params, grads, copies, decay, exp_avg, exp_avg_sq, scales, hyper, rng, sumsq)
+    n = len(params)
+    if not n:
+        return
+    if exp_avg.data_ptr() % 16 or exp_avg_sq.data_ptr() % 16:
+        raise ValueError("moments must start on 16 bytes")
+    first, at = [], 0
+    for k in sizes:
+        first.append(at)
+        at += -(-k // MOMENT_BLOCK)
+    ptrs = c_void_p * n
+    kind = lambda t: 2 if t.dtype == torch.float32 else 0
+    with _device_of(exp_avg):
+        rc = typed("adamw_tensors", "nplm_adamw_tensors", "ppppppiiiippplpppp")(
+            ptrs(*[p.data_ptr() for p in params]), ptrs(*[g.data_ptr() for g in grads]),
+            None if copies is None else ptrs(*[c.data_ptr() for c in copies]), (c_longlong * n)(*sizes),
+            (c_longlong * n)(*first), (c_ubyte * n)(*([1] * n if decay is None else map(bool, decay))), n, kind(params[0]),
+            kind(grads[0]), bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), _dp(scales), blocks, hyper.data_ptr(), _dp(sumsq),
+            _dp(rng), raw_stream())
+        check_rc(rc, "adamw_tensors")
+    count_launch(-(-sum(k > 0 for k in sizes) // 128))
+
+
+def moment_values(exp_avg, exp_avg_sq, scales, dtype=torch.float32):
+    """What the codes of 8-bit moments stand for: (first, second) moments [blocks * 256], fp32 or bf16, both exact."""
+    _, blocks = check_moments(exp_avg, exp_avg_sq, scales)
+    if exp_avg.dtype != torch.uint8 or dtype not in (torch.float32, _BF16):
+        raise ValueError("8-bit moments as fp32 or bf16")
+    with _device_of(exp_avg, exp_avg_sq, scales):
+        m = torch.empty(blocks * MOMENT_BLOCK, dtype=dtype, device=exp_avg.device)
+        v = torch.empty_like(m)
+        rc = typed("adamw_tensors", "nplm_moment_values", "ppplppip")(
+            exp_avg.data_ptr(), exp_avg_sq.data_ptr(), scales.data_ptr(), blocks, m.data_ptr(), v.data_ptr(),
+            2 if dtype == torch.float32 else 0, raw_stream())
+        check_rc(rc, "moment_values")
+        count_launch(blocks > 0)
+    return m, v
+
+
+def moment_codes(m: torch.Tensor, v: torch.Tensor):
+    """(codes of the first moments, of the second, scales) of fp32 [blocks * 256] moments, rounded to the nearest code: what
+    `moment_values` gave comes back as it was."""
+    _, blocks = check_moments(m, v, None)
+    with _device_of(m, v):
+        mc, vc = (torch.empty(m.numel(), dtype=torch.uint8, device=m.device) for _ in range(2))
+        scales = torch.empty((2, blocks), dtype=torch.uint8, device=m.device)
+        if m.data_ptr() % 16 or v.data_ptr() % 16:
+            raise ValueError("moments must start on 16 bytes")
+        rc = typed("adamw_tensors", "nplm_moment_codes", "ppppplp")(
+            m.data_ptr(), v.data_ptr(), mc.data_ptr(), vc.data_ptr(), scales.data_ptr(), blocks, raw_stream())
+        check_rc(rc, "moment_codes")
+        count_launch(blocks > 0)
+    return mc, vc, scales
 
 
 def cast_f32_bf16_(src: torch.Tensor, dst: torch.Tensor) -> None:

@@ -1,0 +1,240 @@
+"""One AdamW step over a list of tensors with moments in fp32 or 8 bits: the restatement on the CPU, and the kernel against it."""
+import math
+
+import pytest
+import torch
+
+from nanoplm_b200.ops import kernels as K
+from nanoplm_b200.ops import moments as M
+
+BF, F32 = torch.bfloat16, torch.float32
+SIZES = [(3,), (256,), (257,), (40, 64), (1,), (0,), (33, 33), (8192 + 256 + 5,), (64, 256)]
+
+
+def _hyper(t, lr=1e-2, b1=0.9, b2=0.999, wd=0.1, gs=0.5, most=1.0, device="cpu"):
+    return torch.tensor([lr, b1, b2, 1e-8, wd, 1 - b1 ** t, 1 - b2 ** t, gs, most], device=device)
+
+
+def _set(shapes, p_type, g_type, shift=0, seed=0):
+    """(params, grads, copies or None) on the CPU; with shift inside larger buffers at odd addresses."""
+    gen = torch.Generator().manual_seed(seed)
+
+    def make(dtype, scale):
+        out = []
+        for s in shapes:
+            n = math.prod(s)
+            buf = torch.zeros(n + shift, dtype=dtype)
+            buf[shift:] = (scale * torch.randn(n, generator=gen) * torch.exp(2 * torch.randn(n, generator=gen))).to(dtype)
+            out.append(buf[shift:].view(s))
+        return out
+    params = make(p_type, 0.1)
+    return params, make(g_type, 0.01), [torch.zeros_like(p, dtype=BF) for p in params] if p_type == F32 else None
+
+
+# ------------------------------------------------------------------------------------------- CPU
+def test_fp32_moments_follow_torch():
+    params, grads, copies = _set([(5, 7), (300,)], F32, F32)
+    ref = [p.clone().requires_grad_(True) for p in params]
+    opt = torch.optim.AdamW([{"params": ref[:1], "weight_decay": 0.1}, {"params": ref[1:], "weight_decay": 0.0}], lr=1e-2)
+    st = M.TensorMoments([p.numel() for p in params], "cpu")
+    for t in range(1, 8):
+        for r, g in zip(ref, grads):
+            r.grad = g * 0.5
+        opt.step()
+        st.step(params, grads, _hyper(t, most=0.0), copies=copies, decay=[True, False])
+    for p, r, c in zip(params, ref, copies):
+        assert torch.allclose(p, r, rtol=1e-5, atol=1e-6) and torch.equal(c, p.to(BF))
+
+
+def test_codes_are_neighbours_and_come_back():
+    x = torch.randn(4 * M.BLOCK) * torch.exp(4 * torch.randn(4 * M.BLOCK))
+    x[5] = 0.0
+    for values, signed, octaves in ((x, True, 15), (x.square(), False, 31)):
+        for r in (0, 0x80000, 0xfffff):
+            codes, e = M.encode(values, r, signed)
+            back = M.decode(codes, e, signed)
+            assert back[5] == 0
+            big = values.abs() > values.abs().view(-1, M.BLOCK).amax(1).repeat_interleave(M.BLOCK) * 2.0 ** -(octaves - 1)
+            # 3 bits of mantissa: neighbours are an eighth of the octave apart, the nearest half of that
+            step = torch.exp2(torch.floor(torch.log2(values.abs().clamp(min=1e-30)))) / 8
+            assert ((back - values).abs()[big] <= (step * (0.5 if r == 0x80000 else 1) * (1 + 1e-6))[big]).all()
+            again, e2 = M.encode(back, 0x80000, signed)
+            assert torch.equal(M.decode(again, e2, signed), back)
+            assert signed or (back[values > 0] > 0).all()
+
+
+def test_rounding_keeps_the_mean():
+    """The mean of n independent roundings of x is off x by at most 5 of its deviations: a value that is kept as a or b, d apart,
+    has a deviation of at most d / 2."""
+    n = 4096
+    for signed, value in ((True, 1.03), (True, -0.9999), (False, 0.7), (True, 2.0 ** -17 * 1.3), (True, -(2.0 ** -16))):
+        x = torch.full((n * M.BLOCK // 256, 256), value)
+        x[:, 0] = 1.5 if abs(value) < 1 else value          # the largest of every block
+        r = M.random_bits(x.numel(), torch.tensor([12345])) & 0xfffff
+        codes, e = M.encode(x.view(-1), r, signed)
+        back = M.decode(codes, e, signed).view(-1, 256)[:, 1:].double()
+        d = float(back.max() - back.min())
+        assert abs(float(back.mean()) - value) <= 5 * max(d, 1e-12) / 2 / back.numel() ** 0.5 + abs(value) * 2e-6
+        assert len(back.unique()) <= 2
+
+
+def test_slow_average_is_followed():
+    """A second moment that moves by 0.1 % a step reaches its gradient's square, which rounding to the nearest code would not let
+    it do: after 4 000 steps the fp32 average is at 98 % of it."""
+    st = M.TensorMoments([512], "cpu", 8)
+    p, g = torch.zeros(512), torch.full((512,), 0.1)
+    for t in range(1, 4001):
+        st.step([p], [g], _hyper(t, most=0.0, gs=1.0), rng=torch.tensor([t * 7919]))
+    v = st.values()[1][0]
+    assert float(v.mean()) == pytest.approx(0.01 * (1 - 0.999 ** 4000), rel=0.05)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_load_what_they_gave(bits):
+    shapes = [(300,), (5, 5), (700,)]
+    params, grads, _ = _set(shapes, F32, F32)
+    st = M.TensorMoments([p.numel() for p in params], "cpu", bits)
+    for t in (1, 2, 3):
+        st.step(params, grads, _hyper(t), rng=torch.tensor([t]))
+    m, v = st.values()
+    other = M.TensorMoments([p.numel() for p in params], "cpu", bits)
+    other.load([t.clone() for t in m], [t.clone() for t in v])
+    assert all(torch.equal(a, b) for a, b in zip(m + v, sum(other.values(), [])))
+    assert st.nbytes() == (6 if bits == 8 else 6) * 256 * (2 if bits == 8 else 8) + (12 if bits == 8 else 0)
+
+
+def test_refusals():
+    params, grads, copies = _set([(300,), (8,)], F32, F32)
+    st = M.TensorMoments([300, 8], "cpu", 8)
+    rng, hyper = torch.tensor([1]), _hyper(1)
+    ok = dict(params=params, grads=grads, hyper=hyper, rng=rng, copies=copies, decay=None, sumsq=None)
+    step = lambda **k: (lambda a: st.step(a.pop("params"), a.pop("grads"), a.pop("hyper"), **a))(ok | k)
+    step()
+    for bad in (dict(params=params[:1], grads=grads[:1], copies=copies[:1]), dict(grads=grads[:1]), dict(copies=copies[:1]),
+                dict(decay=[True]), dict(rng=None), dict(rng=torch.tensor([1.0])), dict(hyper=hyper[:8]), dict(hyper=hyper.double()),
+                dict(grads=[grads[0], grads[1].to(BF)]), dict(grads=[g.double() for g in grads]), dict(copies=grads),
+                dict(grads=[grads[0][:299], grads[1]]), dict(sumsq=torch.zeros(2)), dict(params=[p.half() for p in params])):
+        with pytest.raises(ValueError):
+            step(**bad)
+    with pytest.raises(ValueError):     # bf16 copies of bf16 params
+        step(params=[p.to(BF) for p in params])
+    with pytest.raises(ValueError):     # the same tensor twice
+        M.TensorMoments([8, 8], "cpu").step([params[1]] * 2, [grads[1]] * 2, hyper)
+    with pytest.raises(ValueError):     # not contiguous
+        M.TensorMoments([16], "cpu").step([torch.zeros(4, 4).t()[:, :]], [torch.zeros(4, 4)], hyper)
+    with pytest.raises(ValueError):
+        M.TensorMoments([8], "cpu", 16)
+    with pytest.raises(ValueError):
+        st.load([torch.zeros(300)], [torch.zeros(300)])
+    with pytest.raises(ValueError):     # too few blocks
+        K.check_step(params, grads, None, None, torch.zeros(512), torch.zeros(512), None, hyper, None, None)
+    with pytest.raises(ValueError):     # codes without their scales
+        K.check_step(params, grads, None, None, torch.zeros(768, dtype=torch.uint8), torch.zeros(768, dtype=torch.uint8), None, hyper, rng, None)
+
+
+# ------------------------------------------------------------------------------------------- GPU
+def _both(shapes, p_type, g_type, bits, shift=0, steps=3, clip=True, decay=None):
+    """The same steps on the CPU and on the GPU: ([params, copies, m, v, scales] of each)."""
+    params, grads, copies = _set(shapes, p_type, g_type, shift)
+    dev = lambda ts: None if ts is None else [torch.cat((torch.zeros(shift, dtype=t.dtype), t.reshape(-1))).cuda()[shift:].view(t.shape) for t in ts]
+    gp, gg, gc = dev(params), dev(grads), dev(copies)
+    sizes = [p.numel() for p in params]
+    a, b = M.TensorMoments(sizes, "cpu", bits), M.TensorMoments(sizes, "cuda", bits)
+    sumsq = torch.stack([g.float().square().sum() for g in grads]).sum().reshape(1) if clip else None
+    for t in range(1, steps + 1):
+        rng = torch.tensor([t * 2 ** 33 + 17 * t])
+        a.step(params, grads, _hyper(t), rng=rng, copies=copies, decay=decay, sumsq=sumsq)
+        b.step(gp, gg, _hyper(t, device="cuda"), rng=rng.cuda(), copies=gc, decay=decay, sumsq=None if sumsq is None else sumsq.cuda())
+    return (params, copies, a), (gp, gc, b)
+
+
+def _same(cpu, gpu, p_type):
+    (p, c, a), (gp, gc, b) = cpu, gpu
+    assert torch.equal(a.m, b.m.cpu()) and torch.equal(a.v, b.v.cpu())
+    assert a.scales is None or torch.equal(a.scales, b.scales.cpu())
+    for x, y in zip(p, gp):
+        x, y = x.double(), y.cpu().double()
+        # each of three steps: the quotient is good to 2^-20 of at most 10 lr (m / sqrt v is at most 1 / sqrt(1 - b2)), the
+        # sum to a step of the weight's type, which may be rounded the other way
+        tol = 3 * (0.01 * 32 * 2.0 ** -20 + 2 * torch.finfo(p_type).eps / 2 * x.abs())
+        assert ((x - y).abs() <= tol).all()
+    for x, y in zip(gp, gc or ()):
+        assert torch.equal(x.to(BF), y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("p_type,g_type", [(F32, F32), (F32, BF), (BF, BF), (BF, F32)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_kernel_has_the_bits_of_the_restatement(bits, p_type, g_type, shift, cuda_status):
+    if p_type == BF:        # a weight that is rounded the other way changes no moment: gradients are given
+        cpu, gpu = _both(SIZES, p_type, g_type, bits, shift, decay=[i % 2 == 0 for i in range(len(SIZES))])
+    else:
+        cpu, gpu = _both(SIZES, p_type, g_type, bits, shift, clip=shift == 0)
+    _same(cpu, gpu, p_type)
+
+
+@pytest.mark.gpu
+def test_more_tensors_than_a_launch_takes(cuda_status):
+    shapes = [(1 + 37 * i % 900,) for i in range(301)]
+    _same(*_both(shapes, F32, F32, 8, steps=1), F32)
+
+
+@pytest.mark.gpu
+def test_nothing_behind_a_tensor_is_written(cuda_status):
+    """Views of one buffer with a gap behind each keep their gaps."""
+    buf = torch.randn(4, 700, device="cuda")
+    before = buf.clone()
+    params = [buf[i, :n] for i, n in enumerate((1, 255, 513, 690))]
+    grads = [torch.randn_like(p) for p in params]
+    st = M.TensorMoments([p.numel() for p in params], "cuda", 8)
+    st.step(params, grads, _hyper(1, device="cuda"), rng=torch.tensor([3], device="cuda"))
+    for i, p in enumerate(params):
+        assert torch.equal(buf[i, p.numel():], before[i, p.numel():]) and not torch.equal(p, before[i, :p.numel()])
+        assert not M.decode(st.m.cpu(), st.scales[0].cpu(), True).view(-1)[sum(-(-q.numel() // 256) for q in params[:i]) * 256 + p.numel():][:-p.numel() % 256].any()
+
+
+@pytest.mark.gpu
+def test_captured_step_reads_its_numbers_at_replay(cuda_status):
+    shapes = [(700,), (64, 64)]
+    params, grads, copies = ([t.cuda() for t in ts] for ts in _set(shapes, F32, F32))
+    eager = [[t.clone() for t in ts] for ts in (params, grads, copies)]
+    sizes = [p.numel() for p in params]
+    a, b = M.TensorMoments(sizes, "cuda", 8), M.TensorMoments(sizes, "cuda", 8)
+    hyper, rng = _hyper(1, device="cuda"), torch.tensor([1], device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    a.step(params, grads, hyper, rng=rng, copies=copies)       # (loads the library)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        a.step(params, grads, hyper, rng=rng, copies=copies)
+    b.step(*eager[:2], _hyper(1, device="cuda"), rng=torch.tensor([1], device="cuda"), copies=eager[2])
+    for t in (2, 3, 4):
+        hyper.copy_(_hyper(t, lr=1e-2 * t))
+        rng.fill_(t * 99)
+        graph.replay()
+        b.step(*eager[:2], _hyper(t, lr=1e-2 * t, device="cuda"), rng=torch.tensor([t * 99], device="cuda"), copies=eager[2])
+    assert all(torch.equal(x, y) for x, y in zip(params + copies + [a.m, a.v, a.scales], eager[0] + eager[2] + [b.m, b.v, b.scales]))
+
+
+@pytest.mark.gpu
+def test_values_and_codes(cuda_status):
+    (_, _, a), (_, _, b) = _both([(5000,), (77,)], F32, F32, 8)
+    for dtype in (F32, BF):
+        m, v = K.moment_values(b.m, b.v, b.scales, dtype)
+        assert torch.equal(m.cpu().float(), M.decode(a.m, a.scales[0], True))
+        assert torch.equal(v.cpu().float(), M.decode(a.v, a.scales[1], False))
+    m, v = K.moment_values(b.m, b.v, b.scales)
+    again = K.moment_values(*K.moment_codes(m, v))
+    assert torch.equal(again[0], m) and torch.equal(again[1], v)
+    x, y = torch.randn(1024), torch.rand(1024) * torch.exp(9 * torch.randn(1024))
+    codes = K.moment_codes(x.cuda(), y.cuda())
+    for got, values, row, signed in ((codes[0], x, 0, True), (codes[1], y, 1, False)):
+        c, e = M.encode(values, 0x80000, signed)
+        assert torch.equal(got.cpu(), c) and torch.equal(codes[2][row].cpu(), e)
+
+
+@pytest.mark.gpu
+def test_no_tensors(cuda_status):
+    M.TensorMoments([], "cuda", 8).step([], [], _hyper(1, device="cuda"), rng=torch.tensor([1], device="cuda"))
+    m, v = K.moment_values(*(torch.zeros(0, dtype=torch.uint8, device="cuda") for _ in range(2)), torch.zeros(2, 0, dtype=torch.uint8, device="cuda"))
+    assert m.numel() == v.numel() == 0

@@ -1,0 +1,261 @@
+"""Norm of a block's output, gate, residual scale, sum and the next norm in one operator, forward and backward, against the
+formulas in 64 bits."""
+import pytest
+import torch
+
+from nanoplm_b200.ops import functional as ops
+from nanoplm_b200.ops import kernels as K
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+EPS = 1e-5
+
+
+def _unit(v, rms):
+    if not rms:
+        v = v - v.mean(-1, keepdim=True)
+    return v / (v.square().mean(-1, keepdim=True) + EPS).sqrt()
+
+
+def _formula(x, f, post, nxt, gate, sigmoid, scale, rms):
+    n = _unit(f, rms)
+    n = n if post is None else n * post
+    if gate is not None:
+        n = n * (torch.sigmoid(gate) if sigmoid else gate)
+    y = n + (x if scale is None else scale * x)
+    h = _unit(y, rms)
+    return y, h if nxt is None else h * nxt
+
+
+def _inputs(T, C, dtype, gate, scaled, weighted, device, w_type=None):
+    rnd = lambda *s: torch.randn(*s, device=device)
+    w_type = w_type or dtype
+    p = {"x": (2 * rnd(T, C)).to(dtype), "f": (0.5 * rnd(T, C) + 0.1).to(dtype), "post": None, "nxt": None, "gate": None, "scale": None}
+    if weighted:
+        p["post"], p["nxt"] = (1 + 0.2 * rnd(C)).to(w_type), (1 + 0.2 * rnd(C)).to(w_type)
+    if gate == "channel":
+        p["gate"] = (0.4 + 0.2 * rnd(C)).to(w_type)
+    elif gate != "none":
+        p["gate"] = rnd(T, C).to(dtype)
+    if scaled:
+        p["scale"] = (1 + 0.2 * rnd(C)).to(w_type)
+    return {k: v if v is None else v.requires_grad_(True) for k, v in p.items()}
+
+
+def _call(p, sigmoid, rms, **more):
+    return ops.sandwich_norm(p["x"], p["f"], p["post"], p["nxt"], gate=p["gate"], sigmoid=sigmoid, scale=p["scale"], eps=EPS,
+                             rms=rms, **more)
+
+
+def _check(p, sigmoid, rms, use=("y", "h")):
+    """Outputs and gradients. fp32 errors: every value of a row is a chain of some 40 operations on numbers no larger than the
+    row's largest times 1 / std, and its two means are sums of depth log C + C / (8 threads): 256 units of 2^-24 of the
+    row's largest. A sum over T rows adds those of its terms and T units more of the sum of their magnitudes."""
+    names = [k for k in p if p[k] is not None]
+    y, h = _call(p, sigmoid, rms, with_next="h" in use)
+    ref = {k: (None if v is None else v.detach().double().requires_grad_(True)) for k, v in p.items()}
+    ye, he = _formula(ref["x"], ref["f"], ref["post"], ref["nxt"], ref["gate"], sigmoid, ref["scale"], rms)
+    out = {"y": (y, ye), "h": (h, he)}
+    ds = {k: torch.randn_like(ye).to(p["x"].dtype) for k in use}
+    u = 2.0 ** -24
+    for k in use:
+        got, want = out[k]
+        assert got.dtype == p["x"].dtype and got.is_contiguous()
+        if want.numel():
+            std = (ye.var(-1, unbiased=False, keepdim=True) + EPS).sqrt() if k == "h" else 1.0
+            tol = torch.finfo(got.dtype).eps / 2 * want.abs() + 256 * u * (ye.abs().amax(-1, keepdim=True) / std + 1)
+            assert ((got.double() - want).abs() <= tol).all(), k
+    back = torch.autograd.grad([out[k][0] for k in use], [p[k] for k in names], [ds[k] for k in use], allow_unused=True)
+    want = torch.autograd.grad([out[k][1] for k in use], [ref[k] for k in names], [ds[k].double() for k in use], allow_unused=True)
+    T, C = p["x"].shape
+    for k, a, b in zip(names, back, want):
+        if b is None:       # the next norm is not used
+            assert k == "nxt" and (a is None or not a.any())
+            continue
+        assert a.dtype == p[k].dtype and a.shape == p[k].shape, k
+        if not a.numel():
+            continue
+        step = torch.finfo(a.dtype).eps / 2
+        if p[k].dim() == 2:
+            tol = step * b.abs() + 1024 * u * (b.abs().amax(-1, keepdim=True) + 1)
+        else:               # magnitudes of the terms: at most those of dy, dh times those of unit rows and x, some tens
+            tol = step * b.abs() + (1024 + T) * u * T ** 0.5 * 16 + (1024 + T) * u * b.abs()
+        assert ((a.double() - b).abs() <= tol).all(), (k, float(((a.double() - b).abs() - tol).max()))
+    return back
+
+
+# ------------------------------------------------------------------------------------------- CPU
+@pytest.mark.parametrize("gate,sigmoid", [("none", False), ("channel", False), ("token", False), ("token", True)])
+@pytest.mark.parametrize("rms", [False, True])
+def test_restatement(gate, sigmoid, rms):
+    _check(_inputs(5, 24, F32, gate, True, True, "cpu"), sigmoid, rms)
+
+
+def test_refusals():
+    p = _inputs(4, 8, F32, "token", True, True, "cpu")
+    x = p["x"]
+    for bad in (dict(x=x[0]), dict(f=x[:3]), dict(f=x.to(BF)), dict(gate=x[:, :1]), dict(gate=x.to(BF)), dict(post=x[0, :7]),
+                dict(post=p["post"].to(F16)), dict(nxt=p["nxt"].to(BF), post=p["post"].to(BF)), dict(scale=torch.ones(16)[::2]),
+                dict(gate=p["post"], sigmoid=True), dict(gate=None, sigmoid=True)):
+        a = p | {"sigmoid": False} | bad
+        with pytest.raises(ValueError):
+            ops.sandwich_norm(a["x"], a["f"], a["post"], a["nxt"], gate=a["gate"], scale=a["scale"], sigmoid=a["sigmoid"])
+    with pytest.raises(ValueError):
+        K.sandwich_fwd(x, p["f"], None, None)       # no CPU tensors
+    with pytest.raises(ValueError):
+        K.sandwich_fwd(x.double(), p["f"].double(), None, None)
+    with pytest.raises(ValueError):
+        K.sandwich_bwd(None, None, x, x, torch.empty(4, 4), None, None)
+    with pytest.raises(ValueError):
+        K.sandwich_bwd(x, None, x, x, torch.empty(3, 4), None, None)
+
+
+# ------------------------------------------------------------------------------------------- GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,C", [(1, 1), (1, 8), (3, 250), (37, 256), (5, 264), (700, 512), (130, 768), (9, 1111), (1300, 1024),
+                                 (33, 2048), (3, 3001), (5, 4096)])
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("gate,sigmoid,scaled", [("none", False, False), ("channel", False, True), ("token", False, False),
+                                                 ("token", True, True)])
+def test_outputs_and_gradients(T, C, dtype, gate, sigmoid, scaled, cuda_status):
+    _check(_inputs(T, C, dtype, gate, scaled, True, "cuda"), sigmoid, rms=(T + C) % 2 == 0 or C == 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("use", [("y",), ("h",), ("y", "h")])
+def test_outputs_that_are_not_used(rms, use, cuda_status):
+    _check(_inputs(50, 320, BF, "channel", True, True, "cuda"), False, rms, use)
+
+
+@pytest.mark.gpu
+def test_no_weights_and_fp32_weights(cuda_status):
+    _check(_inputs(50, 320, BF, "none", False, False, "cuda"), False, False)
+    _check(_inputs(50, 320, BF, "channel", True, True, "cuda", F32), False, False)
+    _check(_inputs(50, 321, F16, "token", True, True, "cuda", F32), True, True)
+
+
+@pytest.mark.gpu
+def test_no_rows(cuda_status):
+    back = _check(_inputs(0, 64, BF, "channel", True, True, "cuda"), False, False)
+    assert all(not b.any() for b in back)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,shift", [(256, 0), (256, 1), (100, 0)])
+def test_strides_and_addresses(C, shift, cuda_status):
+    """Rows inside wider rows, at odd addresses, transposed, and gradients that share one row or are transposed."""
+    T = 40
+    p = _inputs(T, C, BF, "token", True, True, "cuda")
+    wide = torch.randn(T, 2 * C + 24, device="cuda").to(BF)
+    p["x"] = wide[:, shift:C + shift].detach().requires_grad_(True)
+    p["f"] = torch.randn(C, T, device="cuda").to(BF).t().detach().requires_grad_(True)
+    p["gate"] = wide[:, C + 16 + shift:2 * C + 16 + shift].detach().requires_grad_(True)
+    _check(p, True, False)
+    y, h = _call(p, True, False)
+    dy, dh = torch.randn(C, device="cuda").to(BF).expand(T, C), torch.randn(C, T, device="cuda").to(BF).t()
+    a = torch.autograd.grad((y, h), (p["x"], p["f"], p["gate"], p["post"]), (dy, dh), retain_graph=True)
+    b = torch.autograd.grad((y, h), (p["x"], p["f"], p["gate"], p["post"]), (dy.contiguous(), dh.contiguous()))
+    for s, t in zip(a, b):
+        if shift == 0 and C % 8 == 0:
+            assert torch.equal(s, t)
+        else:
+            assert torch.allclose(s.float(), t.float(), rtol=2 ** -7, atol=1e-5)
+
+
+@pytest.mark.gpu
+def test_the_same_bits_every_run_and_on_another_stream(cuda_status):
+    p = _inputs(3000, 512, BF, "channel", True, True, "cuda")
+    names = list(p)
+    dy, dh = (torch.randn(3000, 512, device="cuda").to(BF) for _ in range(2))
+
+    def run():
+        y, h = _call(p, False, False)
+        return (y, h) + torch.autograd.grad((y, h), [p[k] for k in names], (dy, dh))
+    first = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        second = run()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(cuda_status):
+    """Directional derivatives of the 64-bit formula by central differences (step 1e-5: errors below 1e-8 here) against the
+    kernel's fp32 gradients, whose sum over 4 000 products is good to some 2^-24 of the sum of their magnitudes a row."""
+    p = _inputs(20, 200, F32, "token", True, True, "cuda")
+    names = [k for k in p if p[k] is not None]
+    y, h = _call(p, True, False)
+    dy, dh = torch.randn_like(y), torch.randn_like(h)
+    back = torch.autograd.grad((y, h), [p[k] for k in names], (dy, dh))
+    for k, g in zip(names, back):
+        d = torch.randn_like(p[k]).double()
+
+        def value(t):
+            q = {n: (v.detach().double() + (t * d if n == k else 0)) for n, v in p.items()}
+            a, b = _formula(q["x"], q["f"], q["post"], q["nxt"], q["gate"], True, q["scale"], False)
+            return ((a * dy).sum() + (b * dh).sum()).item()
+        want = (value(1e-5) - value(-1e-5)) / 2e-5
+        got = (g.double() * d).sum().item()
+        assert abs(got - want) <= 1e-6 * (g.double() * d).abs().sum().item() + 1e-5, k
+
+
+@pytest.mark.gpu
+def test_running_gradients_are_added_to(cuda_status):
+    p = _inputs(300, 256, BF, "channel", True, True, "cuda")
+    names = ("post", "nxt", "gate", "scale")
+    dy, dh = (torch.randn(300, 256, device="cuda").to(BF) for _ in range(2))
+    plain = {}
+    y, h = _call(p, False, False)
+    for k, g in zip(names, torch.autograd.grad((y, h), [p[k] for k in names], (dy, dh))):
+        plain[k] = g
+    for k in names:
+        p[k].main_grad = torch.full((256,), 3.0, device="cuda")
+    torch.autograd.backward(_call(p, False, False), (dy, dh))
+    for k in names:
+        assert p[k].grad is None
+        assert torch.allclose(p[k].main_grad - 3.0, plain[k].float(), rtol=2 ** -7, atol=1e-4), k
+
+
+@pytest.mark.gpu
+def test_captured_passes_do_not_share_their_scratch(cuda_status):
+    T, C = 900, 256
+    sets = [[torch.randn(T, C, device="cuda").to(BF) for _ in range(4)] for _ in range(2)]
+    w = torch.ones(C, device="cuda").to(BF)
+    out, graphs = [], []
+
+    def one(x, f, dy, dh):
+        y, h, st = K.sandwich_fwd(x, f, w, w)
+        s = [torch.empty(C, device="cuda") for _ in range(2)]
+        return [y, h, *K.sandwich_bwd(dy, dh, x, f, st, w, w, sums=(*s, None, None))[:2], *s]
+    want = [one(*s) for s in sets]
+    torch.cuda.synchronize()
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out.append(one(*s))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out, want):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_rows_without_variance_and_large_means(cuda_status):
+    """Constant rows are zeros behind a LayerNorm, and a mean a thousand times the deviation costs no more than the cast did."""
+    T, C = 6, 384
+    x, f = torch.randn(T, C, device="cuda"), torch.randn(T, C, device="cuda")
+    f[0] = 3.0
+    f[1] = 0.0
+    f[2] += 1000.0
+    y, h = ops.sandwich_norm(x, f)
+    assert torch.equal(y[:2], x[:2])
+    ye, he = _formula(x.double(), f.double(), None, None, None, False, None, False)
+    # the mean of the third row is known to 2^-24 of 1000, in units of its deviation 1
+    assert (y.double() - ye).abs().max() <= 16 * 1000 * 2.0 ** -24 and (h.double() - he).abs().max() <= 16 * 1000 * 2.0 ** -24
