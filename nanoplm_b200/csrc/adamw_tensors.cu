@@ -25,8 +25,11 @@ namespace nplm {
 
 constexpr int AT_BLOCK = 256;        // elements that share an offset
 constexpr int AT_TENSORS = 128;      // tensors a launch
-constexpr int AT_CHUNK = 32;         // blocks of one tensor that a thread block takes
 constexpr int AT_WARPS = 8;
+constexpr int AT_CHUNK = 4 * AT_WARPS;    // most blocks of one tensor that a thread block takes, its warps side by side
+constexpr int AT_STAGES = 2;         // blocks of a warp in shared memory: the one it works on and the next
+
+static_assert(AT_CHUNK <= 32, "a lane an exponent");
 
 struct AdamTensors {
   void* p[AT_TENSORS];
@@ -36,7 +39,7 @@ struct AdamTensors {
   long long block[AT_TENSORS];         // first block of the tensor in the moments
   int chunk[AT_TENSORS + 1];           // first chunk of the tensor in this launch
   unsigned char flags[AT_TENSORS];     // 1: weight decay, 2: all addresses on 16 bytes
-  int n;
+  int n, per_chunk;
 };
 
 // A 32-bit mix with two multiplications and three shifts (Wellons, "Prospecting for hash functions", 2018).
@@ -51,25 +54,74 @@ __device__ __forceinline__ uint32_t at_base(uint32_t e) {      // offset of the 
   constexpr uint32_t below = SIGNED ? 15 : 31;
   return (e > below ? e - below : 0u) << 3;
 }
-template <bool SIGNED>
-__device__ __forceinline__ float at_decode(uint32_t code, uint32_t base) {
-  const uint32_t low = SIGNED ? code & 127u : code;
-  const uint32_t bits = low ? (low + base) << 20 : 0u;
-  return __uint_as_float(SIGNED ? bits | (code & 128u) << 24 : bits);
+__device__ __forceinline__ uint32_t at_exponent(uint32_t largest) { return (min(largest, 0x7f800000u) + 0xfffffu) >> 23; }
+
+// Bytes of a (0 - 3) and b (4 - 7). In assembly: around __byte_perm nvcc 12.9 drops bits of the sums below whose top bytes it takes.
+template <uint32_t SELECT>
+__device__ __forceinline__ uint32_t at_bytes(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "n"(SELECT));
+  return d;
 }
+
+// Four codes as values. bottom: the block's offset << 20. A code's byte moves to bits 20 - 27 (with one byte selection and one
+// multiplication, which leaves the integer pipe, the busiest one here, to the rest) and the offset is added; zeros are few and set apart.
 template <bool SIGNED>
-__device__ __forceinline__ uint32_t at_encode(float x, uint32_t base, uint32_t r) {
-  const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
-  if (bits == 0u) return 0u;
-  const uint32_t least = (base + 1u) << 20;       // the pattern of code 1
-  uint32_t code = ((bits + r) >> 20) - base;
-  if (bits < least) {
-    if (!SIGNED) return 1u;
-    code = __fmul_rn(static_cast<float>(r), __fmul_rn(__uint_as_float(least), 9.5367431640625e-7f)) < fabsf(x) ? 1u : 0u;
+__device__ __forceinline__ void at_decode(uint32_t four, uint32_t bottom, float* x) {
+  const uint32_t low = SIGNED ? four & 0x7f7f7f7fu : four;
+  uint32_t bits[4] = {at_bytes<0x4044>(low, 0u) * 16u + bottom, at_bytes<0x4144>(low, 0u) * 16u + bottom,
+                      at_bytes<0x4244>(low, 0u) * 16u + bottom, at_bytes<0x4344>(low, 0u) * 16u + bottom};
+  if (SIGNED) {
+    bits[0] |= four << 24 & 0x80000000u;
+    bits[1] |= four << 16 & 0x80000000u;
+    bits[2] |= four << 8 & 0x80000000u;
+    bits[3] |= four & 0x80000000u;
   }
-  return SIGNED && code ? code | (__float_as_uint(x) >> 24 & 128u) : code;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(bits[e]);
+  const bool zeros = SIGNED ? ((low + 0x7f7f7f7fu) & 0x80808080u) != 0x80808080u : ((low - 0x01010101u) & ~low & 0x80808080u) != 0u;
+  if (zeros) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((low >> 8 * e & 255u) == 0u) x[e] = 0.f;
+  }
 }
-__device__ __forceinline__ uint32_t at_exponent(uint32_t largest) { return (largest + 0xfffffu) >> 23; }
+
+// The codes of four values, whatever they are: zero is 0, a second moment below code 1 is 1, a first moment there 1 or 0 with its
+// mean kept. r: random numbers of 20 bits.
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t at_codes(const float* x, const uint32_t* r, uint32_t bottom) {
+  const uint32_t least = bottom + 0x100000u;      // the pattern of code 1
+  const float step = __fmul_rn(__uint_as_float(least), 9.5367431640625e-7f);    // 2^-20 of it
+  uint32_t four = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t bits = __float_as_uint(x[e]) & 0x7fffffffu;
+    uint32_t code = (bits + r[e] - bottom) >> 20;
+    if (bits < least) code = bits == 0u ? 0u : !SIGNED ? 1u : __fmul_rn(static_cast<float>(r[e]), step) < __uint_as_float(bits);
+    if (SIGNED && code) code |= __float_as_uint(x[e]) >> 24 & 128u;
+    four |= code << 8 * e;
+  }
+  return four;
+}
+
+// The same for values of at least code 1 in a block with an exponent E that AT_PLAIN admits. Times 2^(96 - the block's lowest
+// exponent), an exact product, a value's pattern is 96 x 8 + code on bits 20 and up, and 96 x 8 = 0 modulo 256: no offset is
+// left to subtract, nor a sign to cut off, where the pattern is moved up by 4 bits and its top byte taken.
+constexpr int AT_OCTAVE = 96;
+template <bool SIGNED>
+__device__ __forceinline__ bool at_plain(uint32_t e) {        // E from which 2^(96 - lowest) is a number
+  constexpr uint32_t below = SIGNED ? 15 : 31;
+  return e - below < AT_OCTAVE + 126u;
+}
+template <bool SIGNED>
+__device__ __forceinline__ float at_lift(uint32_t e) {
+  return __uint_as_float((AT_OCTAVE + 127u + (SIGNED ? 15 : 31) - e) << 23);
+}
+constexpr float AT_LEAST = 5.2386894822120667e-10f;           // 1.125 x 2^-31: code 1, lifted
+__device__ __forceinline__ uint32_t at_top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return at_bytes<0x5410>(at_bytes<0x0073>(a, b), at_bytes<0x0073>(c, d));
+}
 
 template <typename T>
 __device__ __forceinline__ float at_get(T v);
@@ -89,13 +141,12 @@ struct alignas(sizeof(T) * N) AtVec {
   T v[N];
 };
 
-// The eight elements of a lane in a block. VEC: two runs of four, the block whole and every address on its multiples;
-// else every 32nd, as far as the tensor goes.
-template <bool VEC>
-__device__ __forceinline__ int at_place(int lane, int e) { return VEC ? (e >> 2) * 128 + lane * 4 + (e & 3) : e * 32 + lane; }
-template <bool VEC, typename T>
-__device__ __forceinline__ void at_load(const T* p, int lane, int n, T (&v)[8]) {
-  if (VEC) {
+// A lane has two runs of four elements of a block, 128 apart. vec: the block is whole and every address on its multiples; else
+// element by element, as far as the tensor goes.
+__device__ __forceinline__ int at_place(int lane, int e) { return (e >> 2) * 128 + lane * 4 + (e & 3); }
+template <typename T>
+__device__ __forceinline__ void at_load(const T* p, int lane, int n, bool vec, T (&v)[8]) {
+  if (vec) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const AtVec<T, 4> t = *reinterpret_cast<const AtVec<T, 4>*>(p + j * 128 + lane * 4);
@@ -104,12 +155,12 @@ __device__ __forceinline__ void at_load(const T* p, int lane, int n, T (&v)[8]) 
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e * 32 + lane < n ? p[e * 32 + lane] : T(0.f);
+    for (int e = 0; e < 8; ++e) v[e] = at_place(lane, e) < n ? p[at_place(lane, e)] : T(0.f);
   }
 }
-template <bool VEC, typename T>
-__device__ __forceinline__ void at_store(T* p, int lane, int n, const T (&v)[8]) {
-  if (VEC) {
+template <typename T>
+__device__ __forceinline__ void at_store(T* p, int lane, int n, bool vec, const T (&v)[8]) {
+  if (vec) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       AtVec<T, 4> t;
@@ -120,7 +171,7 @@ __device__ __forceinline__ void at_store(T* p, int lane, int n, const T (&v)[8])
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e * 32 + lane < n) p[e * 32 + lane] = v[e];
+      if (at_place(lane, e) < n) p[at_place(lane, e)] = v[e];
   }
 }
 
@@ -129,120 +180,219 @@ struct AdamScalars {
   uint32_t key;
 };
 
-// One block of a tensor: elements [0, n), their place `at` in the moments' buffers.
-template <typename P, typename G, int BITS, bool VEC>
-__device__ __forceinline__ void at_block(P* p, const G* g, __nv_bfloat16* copy, int n, void* m_all, void* v_all,
-                                         uint8_t* scales, long long blocks, long long block, const AdamScalars& s, bool decays,
-                                         int lane) {
-  const long long at = block * AT_BLOCK;
-  P pv[8];
-  G gv[8];
-  float m[8], v[8];
-  at_load<VEC>(p, lane, n, pv);
-  at_load<VEC>(g, lane, n, gv);
-  if (BITS == 8) {
-    uint8_t *mc = static_cast<uint8_t*>(m_all) + at, *vc = static_cast<uint8_t*>(v_all) + at;
-    const uint32_t bm = at_base<true>(scales[block]), bv = at_base<false>(scales[blocks + block]);
-    uint8_t cm[8], cv[8];   // (the codes' own buffers are whole blocks on multiples of 16)
-    if (VEC) {
+__device__ __forceinline__ float2 at_both(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ void at_copy_16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void at_fetch(T* to, const T* from, int lane) {      // a whole block, on 16 bytes
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t a = *reinterpret_cast<const uint32_t*>(mc + j * 128 + lane * 4);
-        const uint32_t b = *reinterpret_cast<const uint32_t*>(vc + j * 128 + lane * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          cm[j * 4 + e] = a >> 8 * e & 255u;
-          cv[j * 4 + e] = b >> 8 * e & 255u;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        cm[e] = mc[e * 32 + lane];
-        cv[e] = vc[e * 32 + lane];
-      }
+  for (int j = 0; j < static_cast<int>(sizeof(T) * AT_BLOCK); j += 512)
+    if (j + lane * 16 < static_cast<int>(sizeof(T) * AT_BLOCK))
+      at_copy_16(reinterpret_cast<char*>(to) + j + lane * 16, reinterpret_cast<const char*>(from) + j + lane * 16);
+}
+
+// A block of a tensor with 8-bit moments in shared memory.
+template <typename P, typename G>
+struct alignas(16) AtStage {
+  P p[AT_BLOCK];
+  G g[AT_BLOCK];
+  uint8_t m[AT_BLOCK], v[AT_BLOCK];
+};
+
+// A block of a tensor.
+template <typename P, typename G>
+struct AtPlace {
+  P* p;
+  const G* g;
+  __nv_bfloat16* copy;        // or null
+  int rest;                   // elements from here to the end of the thread block's chunk, or of the tensor where that comes first
+  int block;                  // in the moments
+  bool aligned, decays;
+  __device__ __forceinline__ int n() const { return rest < AT_BLOCK ? rest : AT_BLOCK; }
+  __device__ __forceinline__ bool vec() const { return aligned && rest >= AT_BLOCK; }
+  __device__ __forceinline__ void find(const AdamTensors& t, int chunk, int warp) {
+    int lo = 0, hi = t.n;     // the last tensor that starts at or before this chunk
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (t.chunk[mid] <= chunk) lo = mid;
+      else hi = mid;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      m[e] = at_decode<true>(cm[e], bm);
-      v[e] = at_decode<false>(cv[e], bv);
-    }
-  } else {
-    at_load<VEC>(static_cast<const float*>(m_all) + at, lane, n, m);
-    at_load<VEC>(static_cast<const float*>(v_all) + at, lane, n, v);
+    const int off = (chunk - t.chunk[lo]) * t.per_chunk + warp;
+    const long long at = static_cast<long long>(off) * AT_BLOCK, left = t.numel[lo] - at;
+    const int most = (t.per_chunk - warp) * AT_BLOCK;
+    rest = left < most ? static_cast<int>(left) : most;
+    block = static_cast<int>(t.block[lo]) + off;
+    p = static_cast<P*>(t.p[lo]) + at;
+    g = static_cast<const G*>(t.g[lo]) + at;
+    copy = static_cast<__nv_bfloat16*>(t.copy[lo]);
+    if (copy != nullptr) copy += at;
+    decays = t.flags[lo] & 1;
+    aligned = t.flags[lo] & 2;
   }
+  // The warp's next block of the chunk; false behind the last.
+  __device__ __forceinline__ bool next() {
+    constexpr int step = AT_WARPS * AT_BLOCK;
+    rest -= step;
+    p += step;
+    g += step;
+    if (copy != nullptr) copy += step;
+    block += AT_WARPS;
+    return rest > 0;
+  }
+};
+
+// The moments and the weights of a lane's eight elements.
+__device__ __forceinline__ void at_moments(const float (&g)[8], float (&m)[8], float (&v)[8], const AdamScalars& s) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {      // products in pairs; a packed sum of them would become one rounding
+    const float2 gr = mul2(make_float2(g[e], g[e + 1]), at_both(s.scale));
+    const float2 m0 = mul2(make_float2(m[e], m[e + 1]), at_both(s.b1)), m1 = mul2(gr, at_both(s.c1));
+    const float2 v0 = mul2(make_float2(v[e], v[e + 1]), at_both(s.b2)), v1 = mul2(mul2(gr, gr), at_both(s.c2));
+    m[e] = __fadd_rn(m0.x, m1.x);
+    m[e + 1] = __fadd_rn(m0.y, m1.y);
+    v[e] = __fadd_rn(v0.x, v1.x);
+    v[e + 1] = __fadd_rn(v0.y, v1.y);
+  }
+}
+template <typename P, typename G>
+__device__ __forceinline__ void at_weights(const P (&old)[8], const float (&m)[8], const float (&v)[8], const AtPlace<P, G>& at,
+                                           const AdamScalars& s, int lane) {
+  P pv[8];
   __nv_bfloat16 half[8];
-  uint32_t top_m = 0, top_v = 0;
+  float root[8];
+  if (s.eps >= 1e-15f) {      // (a second moment below fp32's normal range does not matter beside eps)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root[e]) : "f"(v[e]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) asm("sqrt.approx.f32 %0, %1;" : "=f"(root[e]) : "f"(v[e]));
+  }
+  const float decay = at.decays ? s.decay : 1.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float gr = __fmul_rn(at_get<G>(gv[e]), s.scale);
-    m[e] = __fadd_rn(__fmul_rn(m[e], s.b1), __fmul_rn(gr, s.c1));
-    v[e] = __fadd_rn(__fmul_rn(v[e], s.b2), __fmul_rn(__fmul_rn(gr, gr), s.c2));
-    if (!VEC && at_place<VEC>(lane, e) >= n) m[e] = v[e] = 0.f;     // behind the tensor: stays zero
-    float root;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v[e]));
-    const float step = __fdividef(m[e], fmaf(root, s.inv_bc2, s.eps));
-    const float pn = fmaf(-s.step, step, __fmul_rn(at_get<P>(pv[e]), decays ? s.decay : 1.f));
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root[e], s.inv_bc2, s.eps)));
+    const float pn = fmaf(-s.step, m[e] * inv, __fmul_rn(at_get<P>(old[e]), decay));
     pv[e] = at_put<P>(pn);
     half[e] = at_put<__nv_bfloat16>(pn);
-    if (BITS == 8) {
-      top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
-      top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
-    }
   }
-  at_store<VEC>(p, lane, n, pv);
-  if (copy != nullptr) at_store<VEC>(copy, lane, n, half);
-  if (BITS == 8) {
-    uint8_t *mc = static_cast<uint8_t*>(m_all) + at, *vc = static_cast<uint8_t*>(v_all) + at;
-    const uint32_t em = at_exponent(__reduce_max_sync(0xffffffffu, top_m)), ev = at_exponent(__reduce_max_sync(0xffffffffu, top_v));
-    const uint32_t bm = at_base<true>(em), bv = at_base<false>(ev);
-    const uint32_t key = at_mix(s.key + static_cast<uint32_t>(at >> 32)), low = static_cast<uint32_t>(at);
-    uint32_t cm[8], cv[8];
+  at_store(at.p, lane, at.n(), at.vec(), pv);
+  if (at.copy != nullptr) at_store(at.copy, lane, at.n(), at.vec(), half);
+}
+
+// A block with fp32 moments.
+template <typename P, typename G>
+__device__ __forceinline__ void at_block(const AtPlace<P, G>& at, float* m_all, float* v_all, const AdamScalars& s, int lane) {
+  float *mp = m_all + static_cast<long long>(at.block) * AT_BLOCK, *vp = v_all + static_cast<long long>(at.block) * AT_BLOCK;
+  P pv[8];
+  G gv[8];
+  float g[8], m[8], v[8];
+  at_load(at.p, lane, at.n(), at.vec(), pv);
+  at_load(at.g, lane, at.n(), at.vec(), gv);
+  at_load(mp, lane, AT_BLOCK, true, m);
+  at_load(vp, lane, AT_BLOCK, true, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t r = at_mix((low + at_place<VEC>(lane, e)) ^ key);
-      cm[e] = at_encode<true>(m[e], bm, r & 0xfffffu);
-      cv[e] = at_encode<false>(v[e], bv, r >> 12);
-    }
-    if (VEC) {
+  for (int e = 0; e < 8; ++e) g[e] = at_get<G>(gv[e]);
+  at_moments(g, m, v, s);       // (behind the tensor m, v and g are zero, and stay so)
+  at_weights(pv, m, v, at, s, lane);
+  at_store(mp, lane, AT_BLOCK, true, m);
+  at_store(vp, lane, AT_BLOCK, true, v);
+}
+
+// A block with 8-bit moments, its inputs in shared memory; em, ev: its exponents, and then the new ones.
+template <typename P, typename G>
+__device__ __forceinline__ void at_block(const AtStage<P, G>& in, const AtPlace<P, G>& at, uint8_t* m_all, uint8_t* v_all,
+                                         uint32_t& em, uint32_t& ev, const AdamScalars& s, int lane) {
+  float m[8], v[8];
+  {
+    G gv[8];
+    float g[8];
+    at_load(in.g, lane, AT_BLOCK, true, gv);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        *reinterpret_cast<uint32_t*>(mc + j * 128 + lane * 4) =
-            cm[j * 4] | cm[j * 4 + 1] << 8 | cm[j * 4 + 2] << 16 | cm[j * 4 + 3] << 24;
-        *reinterpret_cast<uint32_t*>(vc + j * 128 + lane * 4) =
-            cv[j * 4] | cv[j * 4 + 1] << 8 | cv[j * 4 + 2] << 16 | cv[j * 4 + 3] << 24;
-      }
-    } else {
+    for (int e = 0; e < 8; ++e) g[e] = at_get<G>(gv[e]);
+    const uint32_t *sm = reinterpret_cast<const uint32_t*>(in.m) + lane, *sv = reinterpret_cast<const uint32_t*>(in.v) + lane;
+    const uint32_t bm = at_base<true>(em) << 20, bv = at_base<false>(ev) << 20;
+    at_decode<true>(sm[0], bm, m);
+    at_decode<true>(sm[32], bm, m + 4);
+    at_decode<false>(sv[0], bv, v);
+    at_decode<false>(sv[32], bv, v + 4);
+    at_moments(g, m, v, s);
+  }
+  {
+    P pv[8];
+    at_load(in.p, lane, AT_BLOCK, true, pv);
+    at_weights(pv, m, v, at, s, lane);
+  }
+  float top_m = fabsf(m[0]), top_v = v[0], low_m = fabsf(m[0]), low_v = v[0];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        mc[e * 32 + lane] = static_cast<uint8_t>(cm[e]);
-        vc[e * 32 + lane] = static_cast<uint8_t>(cv[e]);
-      }
-    }
-    if (lane == 0) {
-      scales[block] = static_cast<uint8_t>(em);
-      scales[blocks + block] = static_cast<uint8_t>(ev);
+  for (int e = 1; e < 8; ++e) {
+    top_m = fmaxf(top_m, fabsf(m[e]));
+    low_m = fminf(low_m, fabsf(m[e]));
+    top_v = fmaxf(top_v, v[e]);
+    low_v = fminf(low_v, v[e]);
+  }
+  em = at_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)));
+  ev = at_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
+  // The random bits are at_mix(place ^ key) of the element's place. Places of a block differ in their lowest 8 bits, so the
+  // mix's first shift gives all of them the same.
+  const long long first = static_cast<long long>(at.block) * AT_BLOCK;
+  const uint32_t key = at_mix(s.key + static_cast<uint32_t>(first >> 32));
+  uint32_t mine = (static_cast<uint32_t>(first) + lane * 4) ^ key;
+  mine ^= mine >> 16;
+  uint32_t x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    uint32_t h = (mine ^ ((e >> 2) * 128 + (e & 3))) * 0x7feb352du;
+    h = (h ^ (h >> 15)) * 0x846ca68bu;
+    x[e] = h ^ (h >> 16);
+  }
+  uint32_t *mc = reinterpret_cast<uint32_t*>(m_all + first) + lane, *vc = reinterpret_cast<uint32_t*>(v_all + first) + lane;
+  const float lift_m = at_lift<true>(em), lift_v = at_lift<false>(ev);
+  uint32_t cm[2], cv[2];
+  if (at_plain<true>(em) && low_m * lift_m >= AT_LEAST) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      uint32_t t[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = (__float_as_uint(m[j + e] * lift_m) + (x[j + e] & 0xfffffu)) << 4;
+      const uint32_t signs = at_top_bytes(__float_as_uint(m[j]), __float_as_uint(m[j + 1]), __float_as_uint(m[j + 2]), __float_as_uint(m[j + 3]));
+      cm[j / 4] = at_top_bytes(t[0], t[1], t[2], t[3]) | (signs & 0x80808080u);
     }
   } else {
-    at_store<VEC>(static_cast<float*>(m_all) + at, lane, n, m);
-    at_store<VEC>(static_cast<float*>(v_all) + at, lane, n, v);
+    uint32_t r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = x[e] & 0xfffffu;
+    const uint32_t bm = at_base<true>(em) << 20;
+    cm[0] = at_codes<true>(m, r, bm);
+    cm[1] = at_codes<true>(m + 4, r + 4, bm);
   }
+  if (at_plain<false>(ev) && low_v * lift_v >= AT_LEAST) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+      uint32_t t[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = (__float_as_uint(v[j + e] * lift_v) + (x[j + e] >> 12)) << 4;
+      cv[j / 4] = at_top_bytes(t[0], t[1], t[2], t[3]);
+    }
+  } else {
+    uint32_t r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = x[e] >> 12;
+    const uint32_t bv = at_base<false>(ev) << 20;
+    cv[0] = at_codes<false>(v, r, bv);
+    cv[1] = at_codes<false>(v + 4, r + 4, bv);
+  }
+  mc[0] = cm[0];
+  mc[32] = cm[1];
+  vc[0] = cv[0];
+  vc[32] = cv[1];
 }
 
 // hyper: [lr, beta1, beta2, eps, weight_decay, bias_corr1, bias_corr2, grad_scale, max_norm]; rng: one 64-bit number, another one
 // each step. Both in device memory, so that a captured step sees their values at its replay.
-template <typename P, typename G, int BITS>
-__global__ void __launch_bounds__(AT_WARPS * 32)
-adamw_tensors_kernel(const __grid_constant__ AdamTensors t, void* m_all, void* v_all, uint8_t* scales, long long blocks,
-                     const float* __restrict__ hyper, const float* __restrict__ sumsq, const long long* __restrict__ rng) {
-  grid_chain();
-  const int chunk = blockIdx.x, lane = threadIdx.x & 31;
-  int lo = 0, hi = t.n;                 // the last tensor that starts at or before this chunk
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (t.chunk[mid] <= chunk) lo = mid;
-    else hi = mid;
-  }
+__device__ __forceinline__ AdamScalars at_scalars(const float* hyper, const float* sumsq, const long long* rng) {
   AdamScalars s;
   const float lr = hyper[0], gs = hyper[7], most = hyper[8];
   s.b1 = hyper[1];
@@ -259,47 +409,118 @@ adamw_tensors_kernel(const __grid_constant__ AdamTensors t, void* m_all, void* v
     s.scale = __fmul_rn(gs, fminf(most / __fadd_rn(norm, 1e-6f), 1.f));
   }
   s.key = 0;
-  if (BITS == 8) {
+  if (rng != nullptr) {
     const unsigned long long seed = static_cast<unsigned long long>(*rng);
     s.key = at_mix(static_cast<uint32_t>(seed) ^ at_mix(static_cast<uint32_t>(seed >> 32)));
   }
-  const long long numel = t.numel[lo];
-  const bool decays = t.flags[lo] & 1, aligned = t.flags[lo] & 2;
-  const long long first = static_cast<long long>(chunk - t.chunk[lo]) * AT_CHUNK;
-  P* p = static_cast<P*>(t.p[lo]);
-  const G* g = static_cast<const G*>(t.g[lo]);
-  __nv_bfloat16* copy = static_cast<__nv_bfloat16*>(t.copy[lo]);
-  for (int j = threadIdx.x >> 5; j < AT_CHUNK; j += AT_WARPS) {
-    const long long at = (first + j) * AT_BLOCK, left = numel - at;
-    if (left <= 0) return;
-    const int n = static_cast<int>(left < AT_BLOCK ? left : AT_BLOCK);
-    __nv_bfloat16* c = copy == nullptr ? nullptr : copy + at;
-    if (aligned && n == AT_BLOCK)
-      at_block<P, G, BITS, true>(p + at, g + at, c, n, m_all, v_all, scales, blocks, t.block[lo] + first + j, s, decays, lane);
-    else
-      at_block<P, G, BITS, false>(p + at, g + at, c, n, m_all, v_all, scales, blocks, t.block[lo] + first + j, s, decays, lane);
-  }
+  return s;
 }
 
-// The values of all codes, both moments in one launch: four codes a thread.
+template <typename P, typename G>
+__global__ void __launch_bounds__(AT_WARPS * 32, 4)
+adamw_tensors_kernel(const __grid_constant__ AdamTensors t, float* m, float* v, const float* __restrict__ hyper,
+                     const float* __restrict__ sumsq) {
+  grid_chain();
+  const int lane = threadIdx.x & 31;
+  AtPlace<P, G> at;
+  at.find(t, blockIdx.x, warp_index());
+  if (at.rest <= 0) return;
+  const AdamScalars s = at_scalars(hyper, sumsq, nullptr);
+  do at_block(at, m, v, s, lane);
+  while (at.next());
+}
+
+// With 8-bit moments a warp's next block is on its way to shared memory while it works on one: there is about as much to
+// compute as to move, and registers for only half the warps. The exponents of the chunk are read before and written after all
+// else, in one access each: single bytes, written by one warp into sectors that others were about to read, took as long again
+// as the whole rest (113 M elements: 655 us, without them 300).
+template <typename P, typename G>
+__global__ void __launch_bounds__(AT_WARPS * 32, 4)
+adamw_tensors_8bit_kernel(const __grid_constant__ AdamTensors t, uint8_t* m, uint8_t* v, uint8_t* scales, long long blocks,
+                          const float* __restrict__ hyper, const float* __restrict__ sumsq, const long long* __restrict__ rng) {
+  extern __shared__ __align__(128) uint8_t at_smem[];
+  __shared__ uint8_t exponents[2][AT_CHUNK];
+  grid_chain();
+  const int lane = threadIdx.x & 31, warp = warp_index();
+  AtStage<P, G>* ring = reinterpret_cast<AtStage<P, G>*>(at_smem) + warp * AT_STAGES;
+  auto fetch = [&](const AtPlace<P, G>& at, AtStage<P, G>& to) {
+    if (at.vec()) {
+      at_fetch(to.p, at.p, lane);
+      at_fetch(to.g, at.g, lane);
+    } else {      // (there for the warp after its next __syncwarp)
+      const int n = at.n();
+      P pv[8];
+      G gv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pv[e] = e * 32 + lane < n ? at.p[e * 32 + lane] : P(0.f);
+        gv[e] = e * 32 + lane < n ? at.g[e * 32 + lane] : G(0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        to.p[e * 32 + lane] = pv[e];
+        to.g[e * 32 + lane] = gv[e];
+      }
+    }
+    const long long first = static_cast<long long>(at.block) * AT_BLOCK;
+    if (lane < 16) at_copy_16(to.m + lane * 16, m + first + lane * 16);
+    else at_copy_16(to.v + lane * 16 - AT_BLOCK, v + first + lane * 16 - AT_BLOCK);
+  };
+  AtPlace<P, G> at;
+  at.find(t, blockIdx.x, warp);
+  bool more = at.rest > 0;
+  const int of_chunk = at.block - warp;       // the chunk's first block, and how many it has
+  const int held = min(t.per_chunk, static_cast<int>(min((at.rest + warp * AT_BLOCK + AT_BLOCK - 1LL) / AT_BLOCK, 1LL * AT_CHUNK)));
+  if (more) fetch(at, ring[0]);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  if (warp < 2 && lane < held) exponents[warp][lane] = scales[warp * blocks + of_chunk + lane];
+  const AdamScalars s = at_scalars(hyper, sumsq, rng);
+  __syncthreads();
+  int stage = 0;
+  for (int j = warp; more; j += AT_WARPS) {
+    const AtPlace<P, G> now = at;
+    more = at.next();
+    __syncwarp();     // every lane has read the stage that is filled now
+    if (more) fetch(at, ring[stage ^ 1]);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    uint32_t em = exponents[0][j], ev = exponents[1][j];
+    at_block(ring[stage], now, m, v, em, ev, s, lane);
+    if (lane == 0) {
+      exponents[0][j] = static_cast<uint8_t>(em);
+      exponents[1][j] = static_cast<uint8_t>(ev);
+    }
+    stage ^= 1;
+  }
+  __syncthreads();
+  if (warp < 2 && lane < held) scales[warp * blocks + of_chunk + lane] = exponents[warp][lane];
+}
+
+// The values of all codes, both moments in one launch: eight codes a thread.
 template <typename O>
 __global__ void __launch_bounds__(256)
-moment_values_kernel(const uint32_t* __restrict__ mc, const uint32_t* __restrict__ vc, const uint8_t* __restrict__ scales,
+moment_values_kernel(const uint2* __restrict__ mc, const uint2* __restrict__ vc, const uint8_t* __restrict__ scales,
                      long long blocks, O* __restrict__ m, O* __restrict__ v) {
   grid_chain();
-  const long long n = blocks * (AT_BLOCK / 4);
+  const long long n = blocks * (AT_BLOCK / 8);
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
-    const long long block = i / (AT_BLOCK / 4);
-    const uint32_t a = mc[i], b = vc[i];
-    const uint32_t bm = at_base<true>(scales[block]), bv = at_base<false>(scales[blocks + block]);
-    AtVec<O, 4> x, y;
+    const long long block = i / (AT_BLOCK / 8);
+    const uint2 a = mc[i], b = vc[i];
+    const uint32_t bm = at_base<true>(scales[block]) << 20, bv = at_base<false>(scales[blocks + block]) << 20;
+    float f[8], g[8];
+    at_decode<true>(a.x, bm, f);
+    at_decode<true>(a.y, bm, f + 4);
+    at_decode<false>(b.x, bv, g);
+    at_decode<false>(b.y, bv, g + 4);
+    AtVec<O, 8> x, y;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x.v[e] = at_put<O>(at_decode<true>(a >> 8 * e & 255u, bm));
-      y.v[e] = at_put<O>(at_decode<false>(b >> 8 * e & 255u, bv));
+    for (int e = 0; e < 8; ++e) {
+      x.v[e] = at_put<O>(f[e]);
+      y.v[e] = at_put<O>(g[e]);
     }
-    *reinterpret_cast<AtVec<O, 4>*>(m + i * 4) = x;
-    *reinterpret_cast<AtVec<O, 4>*>(v + i * 4) = y;
+    *reinterpret_cast<AtVec<O, 8>*>(m + i * 8) = x;
+    *reinterpret_cast<AtVec<O, 8>*>(v + i * 8) = y;
   }
 }
 
@@ -312,8 +533,8 @@ moment_codes_kernel(const float* __restrict__ m, const float* __restrict__ v, ui
   for (long long block = blockIdx.x * 8LL + (threadIdx.x >> 5); block < blocks; block += gridDim.x * 8LL) {
     const long long at = block * AT_BLOCK;
     float x[8], y[8];
-    at_load<true>(m + at, lane, AT_BLOCK, x);
-    at_load<true>(v + at, lane, AT_BLOCK, y);
+    at_load(m + at, lane, AT_BLOCK, true, x);
+    at_load(v + at, lane, AT_BLOCK, true, y);
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -321,17 +542,12 @@ moment_codes_kernel(const float* __restrict__ m, const float* __restrict__ v, ui
       top_v = max(top_v, __float_as_uint(y[e]) & 0x7fffffffu);
     }
     const uint32_t em = at_exponent(__reduce_max_sync(0xffffffffu, top_m)), ev = at_exponent(__reduce_max_sync(0xffffffffu, top_v));
-    const uint32_t bm = at_base<true>(em), bv = at_base<false>(ev);
+    const uint32_t bm = at_base<true>(em) << 20, bv = at_base<false>(ev) << 20;
+    const uint32_t half[4] = {0x80000u, 0x80000u, 0x80000u, 0x80000u};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      uint32_t a = 0, b = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a |= at_encode<true>(x[j * 4 + e], bm, 0x80000u) << 8 * e;
-        b |= at_encode<false>(y[j * 4 + e], bv, 0x80000u) << 8 * e;
-      }
-      *reinterpret_cast<uint32_t*>(mc + at + j * 128 + lane * 4) = a;
-      *reinterpret_cast<uint32_t*>(vc + at + j * 128 + lane * 4) = b;
+      *reinterpret_cast<uint32_t*>(mc + at + j * 128 + lane * 4) = at_codes<true>(x + j * 4, half, bm);
+      *reinterpret_cast<uint32_t*>(vc + at + j * 128 + lane * 4) = at_codes<false>(y + j * 4, half, bv);
     }
     if (lane == 0) {
       scales[block] = static_cast<uint8_t>(em);
@@ -341,13 +557,24 @@ moment_codes_kernel(const float* __restrict__ m, const float* __restrict__ v, ui
 }
 
 template <typename P, typename G>
-static cudaError_t at_launch(const AdamTensors& t, int bits, long long elements, void* m, void* v, uint8_t* scales,
-                             long long blocks, const float* hyper, const float* sumsq, const long long* rng, cudaStream_t st) {
-  const int grid = t.chunk[t.n];
+static int at_launch(const AdamTensors& t, int bits, long long elements, void* m, void* v, uint8_t* scales, long long blocks,
+                     const float* hyper, const float* sumsq, const long long* rng, cudaStream_t st) {
   const bool chained = elements <= CHAIN_ELEMENTS;
-  if (bits == 8)
-    return launch_when(chained, adamw_tensors_kernel<P, G, 8>, grid, AT_WARPS * 32, 0, st, t, m, v, scales, blocks, hyper, sumsq, rng);
-  return launch_when(chained, adamw_tensors_kernel<P, G, 32>, grid, AT_WARPS * 32, 0, st, t, m, v, scales, blocks, hyper, sumsq, rng);
+  const int grid = t.chunk[t.n];
+  if (bits == 32)
+    return static_cast<int>(launch_when(chained, adamw_tensors_kernel<P, G>, grid, AT_WARPS * 32, 0, st, t, static_cast<float*>(m),
+                                        static_cast<float*>(v), hyper, sumsq));
+  auto kern = adamw_tensors_8bit_kernel<P, G>;
+  constexpr int smem = AT_WARPS * AT_STAGES * sizeof(AtStage<P, G>);
+  static bool configured_on[MAX_DEVICES];
+  const int dev = current_device_slot();
+  if (dev < 0) return -4;
+  if (!configured_on[dev]) {
+    NPLM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    configured_on[dev] = true;
+  }
+  return static_cast<int>(launch_when(chained, kern, grid, AT_WARPS * 32, smem, st, t, static_cast<uint8_t*>(m),
+                                      static_cast<uint8_t*>(v), scales, blocks, hyper, sumsq, rng));
 }
 
 }  // namespace nplm
@@ -363,6 +590,11 @@ extern "C" int nplm_adamw_tensors(void* const* p, const void* const* g, void* co
   if (n < 0 || (p_type != 0 && p_type != 2) || (g_type != 0 && g_type != 2) || (bits != 8 && bits != 32)) return -1;
   if (bits == 8 && (scales == nullptr || rng == nullptr)) return -1;
   AdamTensors t;
+  // A thread block takes 32 blocks in a row, so that looking up their tensor counts little; 8 while that leaves multiprocessors
+  // without work.
+  long long all = 0;
+  for (int k = 0; k < n; ++k) all += (numel[k] + AT_BLOCK - 1) / AT_BLOCK;
+  t.per_chunk = all >= 148LL * 4 * AT_CHUNK ? AT_CHUNK : AT_WARPS;
   int i = 0;
   while (i < n) {
     t.n = 0;
@@ -371,8 +603,8 @@ extern "C" int nplm_adamw_tensors(void* const* p, const void* const* g, void* co
     for (; i < n && t.n < AT_TENSORS; ++i) {
       if (numel[i] == 0) continue;
       const long long has = (numel[i] + AT_BLOCK - 1) / AT_BLOCK;
-      if (numel[i] < 0 || block[i] < 0 || block[i] + has > blocks) return -2;
-      const long long more = (has + AT_CHUNK - 1) / AT_CHUNK;
+      if (numel[i] < 0 || block[i] < 0 || block[i] + has > blocks || blocks > 0x7fffffffLL) return -2;
+      const long long more = (has + t.per_chunk - 1) / t.per_chunk;
       if (more > 0x7fffffffLL) return -2;
       if (chunks + more > 0x7fffffffLL) break;    // the rest in another launch
       const int k = t.n++;
@@ -390,12 +622,12 @@ extern "C" int nplm_adamw_tensors(void* const* p, const void* const* g, void* co
     }
     if (t.n == 0) break;
     uint8_t* sc = static_cast<uint8_t*>(scales);
-    cudaError_t e;
+    int e;
     if (p_type == 2 && g_type == 2) e = at_launch<float, float>(t, bits, elements, m, v, sc, blocks, hyper, sumsq, rng, st);
     else if (p_type == 2) e = at_launch<float, __nv_bfloat16>(t, bits, elements, m, v, sc, blocks, hyper, sumsq, rng, st);
     else if (g_type == 2) e = at_launch<__nv_bfloat16, float>(t, bits, elements, m, v, sc, blocks, hyper, sumsq, rng, st);
     else e = at_launch<__nv_bfloat16, __nv_bfloat16>(t, bits, elements, m, v, sc, blocks, hyper, sumsq, rng, st);
-    if (e != cudaSuccess) return static_cast<int>(e);
+    if (e) return e;
   }
   return static_cast<int>(cudaGetLastError());
 }
@@ -410,13 +642,13 @@ extern "C" int nplm_moment_values(const void* mc, const void* vc, const void* sc
                                   int out_type, cudaStream_t st) {
   if (blocks < 0 || (out_type != 0 && out_type != 2)) return -1;
   if (blocks == 0) return 0;
-  const uint32_t *a = static_cast<const uint32_t*>(mc), *b = static_cast<const uint32_t*>(vc);
+  const uint2 *a = static_cast<const uint2*>(mc), *b = static_cast<const uint2*>(vc);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
   const bool chained = blocks * AT_BLOCK <= CHAIN_ELEMENTS;
   const cudaError_t e =
-      out_type == 2 ? launch_when(chained, moment_values_kernel<float>, at_grid(blocks, 4), 256, 0, st, a, b, s, blocks,
+      out_type == 2 ? launch_when(chained, moment_values_kernel<float>, at_grid(blocks, 8), 256, 0, st, a, b, s, blocks,
                                   static_cast<float*>(m), static_cast<float*>(v))
-                    : launch_when(chained, moment_values_kernel<__nv_bfloat16>, at_grid(blocks, 4), 256, 0, st, a, b, s, blocks,
+                    : launch_when(chained, moment_values_kernel<__nv_bfloat16>, at_grid(blocks, 8), 256, 0, st, a, b, s, blocks,
                                   static_cast<__nv_bfloat16*>(m), static_cast<__nv_bfloat16*>(v));
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
