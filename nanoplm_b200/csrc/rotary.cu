@@ -17,7 +17,8 @@ namespace nplm {
 
 constexpr int ROT_THREADS = 256;
 constexpr int ROT_PAIRS = 2048;     // cos and sin of a block's tokens: 16 KB
-constexpr int ROT_UNROLL = 4;       // heads that a thread has in flight
+// Items that a thread has in flight.
+__host__ __device__ constexpr int rot_unroll(int bytes) { return bytes >= 16 ? 2 : 4; }
 
 struct RotaryArgs {
   const void* x[2];                 // queries, keys (keys may have no heads)
@@ -35,59 +36,85 @@ struct RotaryArgs {
   int in_place;                     // the channels from R on are there already
 };
 
-template <typename T, int VE>
-struct alignas(sizeof(T) * VE) RotVec {
-  T v[VE];
-};
+// An access as it is moved, and its VE values.
+template <int BYTES>
+struct RotRaw;
+template <>
+struct RotRaw<16> { using type = uint4; };
+template <>
+struct RotRaw<8> { using type = uint2; };
+template <>
+struct RotRaw<4> { using type = uint32_t; };
+template <>
+struct RotRaw<2> { using type = unsigned short; };
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+__device__ __forceinline__ float2 rot_pair(uint32_t w, __nv_bfloat16) { return unpack_bf16x2(w); }
+__device__ __forceinline__ float2 rot_pair(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+__device__ __forceinline__ uint32_t rot_word(float2 v, __nv_bfloat16) { return pack_bf16x2(v.x, v.y); }
+__device__ __forceinline__ uint32_t rot_word(float2 v, __half) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int VE>
+struct RotVec {
+  using Raw = typename RotRaw<sizeof(T) * VE>::type;
+  Raw raw;
+  __device__ __forceinline__ void get(float (&v)[VE]) const {
+    if constexpr (sizeof(T) == 4) {
+      const float* w = reinterpret_cast<const float*>(&raw);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = w[e];
+    } else if constexpr (VE == 1) {
+      v[0] = rot_pair(raw, T()).x;
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+#pragma unroll
+      for (int e = 0; e < VE; e += 2) {
+        const float2 p = rot_pair(w[e / 2], T());
+        v[e] = p.x;
+        v[e + 1] = p.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&v)[VE]) {
+    if constexpr (sizeof(T) == 4) {
+      float* w = reinterpret_cast<float*>(&raw);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) w[e] = v[e];
+    } else if constexpr (VE == 1) {
+      raw = static_cast<unsigned short>(rot_word(make_float2(v[0], 0.f), T()));
+    } else {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&raw);
+#pragma unroll
+      for (int e = 0; e < VE; e += 2) w[e / 2] = rot_word(make_float2(v[e], v[e + 1]), T());
+    }
+  }
+};
 
 // VE: elements an access, a divisor of R / 2, of D - R and of all strides, with the addresses on its multiples. A thread's
 // item is VE pairs of a head (two accesses) or up to 2 VE channels behind the rotated ones. Its place in the head stays the
 // same, so that only token and head advance from item to item.
 template <typename T, int VE, bool INTER>
-__global__ void __launch_bounds__(ROT_THREADS)
+__global__ void __launch_bounds__(ROT_THREADS, 4)
 rotary_kernel(const __grid_constant__ RotaryArgs a) {
   using Vec = RotVec<T, VE>;
+  using Raw = typename Vec::Raw;
+  constexpr int ROT_UNROLL = rot_unroll(sizeof(T) * VE);
   __shared__ __align__(16) float sm_cos[ROT_PAIRS], sm_sin[ROT_PAIRS];
   grid_chain();
   const int half = a.R >> 1;
   const long long t0 = static_cast<long long>(blockIdx.x) * a.tile;
   const int tokens = static_cast<int>(min(static_cast<long long>(a.tile), a.tokens - t0));
-  for (int j = threadIdx.x; j < tokens * half; j += ROT_THREADS) {
-    const int tok = j / half, i = j - tok * half;
-    const long long t = t0 + tok, b = t / a.seq, s = t - b * a.seq;
-    const long long at = b * a.pb + s * a.pt;
-    const double p = a.pos64 ? static_cast<double>(static_cast<const long long*>(a.pos)[at])
-                             : static_cast<double>(static_cast<const int*>(a.pos)[at]);
-    const double turns = p * (a.freq[i] * 0.15915494309189535);   // 1 / (2 pi)
-    const float rest = static_cast<float>(turns - rint(turns));
-    float sn, cs;
-    sincospif(2.f * rest, &sn, &cs);
-    sm_cos[j] = a.factor * cs;
-    sm_sin[j] = a.factor * a.sign * sn;
-  }
-  __syncthreads();
-
   const int rot = half / VE;                                          // items a head: pairs,
   const int behind = a.in_place ? 0 : (a.D - a.R + 2 * VE - 1) / (2 * VE);   // and what is copied
   const int per_head = rot + behind;
   const int stride = ROT_THREADS / per_head;                          // heads that the block takes at a time
   const int first = threadIdx.x / per_head, c = threadIdx.x - first * per_head;
-  if (first >= stride) return;
-  const int heads = a.heads[0] + a.heads[1], rows = tokens * heads;
+  const int heads = a.heads[0] + a.heads[1];
+  const int rows = first < stride ? tokens * heads : 0;
   const int step_t = stride / heads, step_h = stride - step_t * heads;
-  int tok = first / heads, h = first - tok * heads;
+  int tok = first / heads, h = first - tok * heads, row = first;
   const bool pairs = c < rot;
   // offsets of the two accesses in a head
   const int i = c * VE;
@@ -95,14 +122,14 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
   const int o1 = pairs ? (INTER ? 2 * i + VE : i + half) : o0 + VE;
   const bool second = o1 < a.D;
 
-  for (int row = first; row < rows; row += ROT_UNROLL * stride) {
-    Vec v0[ROT_UNROLL], v1[ROT_UNROLL];
-    T* to[ROT_UNROLL];
-    int at[ROT_UNROLL];
+  Vec v0[ROT_UNROLL], v1[ROT_UNROLL];
+  T* to[ROT_UNROLL];
+  int at[ROT_UNROLL];
+  auto load = [&]() {
 #pragma unroll
     for (int u = 0; u < ROT_UNROLL; ++u) {
       to[u] = nullptr;
-      if (row + u * stride < rows) {
+      if (row < rows) {
         const int k = h >= a.heads[0];
         const int hh = h - (k ? a.heads[0] : 0);
         const long long t = t0 + tok;
@@ -114,8 +141,8 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
         const T* from = static_cast<const T*>(a.x[k]) + b * a.xb[k] + s * a.xt[k] + hh * a.xh[k];
         to[u] = static_cast<T*>(a.y[k]) + b * a.yb[k] + s * a.yt[k] + hh * a.yh[k];
         at[u] = tok * half + i;
-        v0[u] = *reinterpret_cast<const Vec*>(from + o0);
-        if (second) v1[u] = *reinterpret_cast<const Vec*>(from + o1);
+        v0[u].raw = *reinterpret_cast<const Raw*>(from + o0);
+        if (second) v1[u].raw = *reinterpret_cast<const Raw*>(from + o1);
         tok += step_t;
         h += step_h;
         if (h >= heads) {
@@ -123,30 +150,79 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
           ++tok;
         }
       }
+      row += stride;
     }
+  };
+  load();     // on its way while cos and sin are formed
+  for (int j = threadIdx.x; j < tokens * half; j += ROT_THREADS) {
+    const int tk = j / half, p2 = j - tk * half;
+    const long long t = t0 + tk;
+    long long b = 0, s = t;
+    if (a.seq != a.tokens) {
+      b = t / a.seq;
+      s = t - b * a.seq;
+    }
+    const long long from = b * a.pb + s * a.pt;
+    const double p = a.pos64 ? static_cast<double>(static_cast<const long long*>(a.pos)[from])
+                             : static_cast<double>(static_cast<const int*>(a.pos)[from]);
+    const double turns = p * (a.freq[p2] * 0.15915494309189535);   // 1 / (2 pi)
+    const float rest = static_cast<float>(turns - rint(turns));
+    float sn, cs;
+    sincospif(2.f * rest, &sn, &cs);
+    sm_cos[j] = a.factor * cs;
+    sm_sin[j] = a.factor * a.sign * sn;
+  }
+  __syncthreads();
+  while (true) {
 #pragma unroll
     for (int u = 0; u < ROT_UNROLL; ++u) {
       if (to[u] != nullptr) {
         if (pairs) {
-          Vec w0, w1;
+          float cs[VE], sn[VE];
+          if constexpr (VE >= 4) {
+#pragma unroll
+            for (int e = 0; e < VE; e += 4) {
+              const float4 cc = *reinterpret_cast<const float4*>(sm_cos + at[u] + e);
+              const float4 ss = *reinterpret_cast<const float4*>(sm_sin + at[u] + e);
+              cs[e] = cc.x; cs[e + 1] = cc.y; cs[e + 2] = cc.z; cs[e + 3] = cc.w;
+              sn[e] = ss.x; sn[e + 1] = ss.y; sn[e + 2] = ss.z; sn[e + 3] = ss.w;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              cs[e] = sm_cos[at[u] + e];
+              sn[e] = sm_sin[at[u] + e];
+            }
+          }
+          float x[2 * VE], lo[VE], hi[VE];
+          v0[u].get(lo);
+          v1[u].get(hi);
 #pragma unroll
           for (int e = 0; e < VE; ++e) {
-            const float cs = sm_cos[at[u] + e], sn = sm_sin[at[u] + e];
-            // the two members of pair e of this item
-            const int j0 = INTER ? 2 * e : e, j1 = INTER ? 2 * e + 1 : VE + e;
-            const float x1 = to_f32(j0 < VE ? v0[u].v[j0 % VE] : v1[u].v[j0 % VE]);
-            const float x2 = to_f32(j1 < VE ? v0[u].v[j1 % VE] : v1[u].v[j1 % VE]);
-            const T y1 = from_f32<T>(x1 * cs - x2 * sn), y2 = from_f32<T>(x2 * cs + x1 * sn);
-            if (j0 < VE) w0.v[j0 % VE] = y1; else w1.v[j0 % VE] = y1;
-            if (j1 < VE) w0.v[j1 % VE] = y2; else w1.v[j1 % VE] = y2;
+            x[e] = lo[e];
+            x[VE + e] = hi[e];
           }
-          v0[u] = w0;
-          v1[u] = w1;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {      // the two members of pair e of this item
+            const int j0 = INTER ? 2 * e : e, j1 = INTER ? 2 * e + 1 : VE + e;
+            const float x1 = x[j0], x2 = x[j1];
+            x[j0] = x1 * cs[e] - x2 * sn[e];
+            x[j1] = x2 * cs[e] + x1 * sn[e];
+          }
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            lo[e] = x[e];
+            hi[e] = x[VE + e];
+          }
+          v0[u].set(lo);
+          v1[u].set(hi);
         }
-        *reinterpret_cast<Vec*>(to[u] + o0) = v0[u];
-        if (second) *reinterpret_cast<Vec*>(to[u] + o1) = v1[u];
+        *reinterpret_cast<Raw*>(to[u] + o0) = v0[u].raw;
+        if (second) *reinterpret_cast<Raw*>(to[u] + o1) = v1[u].raw;
       }
     }
+    if (row >= rows) break;
+    load();
   }
 }
 
@@ -205,9 +281,11 @@ extern "C" int nplm_rotary_qk(const void* q, void* q_out, const void* k, void* k
   while (ve > 1 && !fits(ve)) ve /= 2;
   const int half = R / 2;
   const int per_token = (q_heads + k_heads) * (half / ve + (a.in_place ? 0 : (D - R + 2 * ve - 1) / (2 * ve)));
-  // enough tokens that every thread has its unrolled items, as long as their cos and sin fit
-  int tile = (ROT_THREADS * ROT_UNROLL + per_token - 1) / per_token;
+  // as many tokens as the unrolled items of all threads, at least one, as long as their cos and sin fit
+  const int per_head = per_token / (q_heads + k_heads);
+  int tile = ROT_THREADS / per_head * rot_unroll(ve * size) / (q_heads + k_heads);
   if (tile > ROT_PAIRS / half) tile = ROT_PAIRS / half;
+  if (tile < 1) tile = 1;
   a.tile = tile;
   const long long blocks = (a.tokens + tile - 1) / tile;
   if (blocks > 0x7fffffffLL) return -2;
