@@ -18,8 +18,9 @@
 
 namespace nplm {
 
-constexpr int SW_STAGES = 2;        // rows that a group has on their way
+constexpr int SW_STAGES = 2;        // steps ahead of which a group's rows are fetched; 1 where shared memory holds no more
 constexpr int SW_MAX_C = 4096;
+constexpr size_t SW_MAX_SMEM = 227 * 1024;
 
 enum : int { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_TOKEN = 2, GATE_SIGMOID = 3 };
 
@@ -29,10 +30,11 @@ struct SandwichArgs {
   const void *post, *next, *scale;                    // [C] each; post, next null: 1; scale null: 1
   void *y, *h;                                        // forward outputs, contiguous rows; h may be null
   void *dx, *df, *dg;                                 // backward outputs, contiguous rows; dg only for gates of tokens
-  float* stats;                                       // [4][T]: mean f, 1 / std f, mean y, 1 / std y; null: not kept
+  float4* stats;                                      // [T]: mean f, 1 / std f, mean y, 1 / std y; null: not kept
   float* partial;                                     // [4][blocks][C]: dw_next, dw_post, dr, dg
   long long T;
   int C, tpr, groups;                                 // threads a row, rows that a block works on at a time
+  uint32_t stages;
   float eps;
   int rms, gate_mode, param32;                        // param32: the [C] weights are fp32, else of the rows' type
   int want;                                           // bit k: column sum k is wanted
@@ -59,92 +61,169 @@ struct Io<__half> {
 __device__ __forceinline__ void sw_cp_async_16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
+__device__ __forceinline__ void sw_cp_async_4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 __device__ __forceinline__ void sw_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void sw_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Eight values of a type, as they lie in memory.
-template <typename T>
-struct alignas(16) Eight {
-  T v[8];
+// A thread's eight channels as four pairs, for the packed fp32 instructions.
+struct Eight {
+  float2 p[4];
 };
+__device__ __forceinline__ float2 sw_both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float sw_total(const Eight& v) {
+  const float2 s = add2(add2(v.p[0], v.p[1]), add2(v.p[2], v.p[3]));
+  return s.x + s.y;
+}
+__device__ __forceinline__ float sw_dot(const Eight& a, const Eight& b) {
+  float2 s = mul2(a.p[0], b.p[0]);
+#pragma unroll
+  for (int k = 1; k < 4; ++k) s = fma2(a.p[k], b.p[k], s);
+  return s.x + s.y;
+}
+__device__ __forceinline__ float2 sw_unpack(uint32_t w, __nv_bfloat16) { return unpack_bf16x2(w); }
+__device__ __forceinline__ float2 sw_unpack(uint32_t w, __half) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+__device__ __forceinline__ uint32_t sw_pack(float2 v, __nv_bfloat16) { return pack_bf16x2(v.x, v.y); }
+__device__ __forceinline__ uint32_t sw_pack(float2 v, __half) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 
-// What a thread knows of its place: its group's row slots, its eight channels.
-template <typename T, bool ALIGNED>
+// How a row lies in a group's threads. STRIDED: any width, addresses and strides, a thread has every tpr-th channel. ALIGNED: widths
+// and addresses on 16 bytes, a thread has eight neighbouring channels, or none. FULL: the same, and no thread has none.
+enum : int { STRIDED = 0, ALIGNED = 1, FULL = 2 };
+
+template <typename T, int MODE>
 struct Place {
   int lane, group, tpr, C;
-  __device__ __forceinline__ int channel(int e) const { return ALIGNED ? lane * 8 + e : e * tpr + lane; }
-  __device__ __forceinline__ bool on(int e) const { return channel(ALIGNED ? 0 : e) < C; }
+  bool any;
+  __device__ __forceinline__ Place(int tpr_, int C_) : tpr(tpr_), C(C_) {
+    group = threadIdx.x / tpr;
+    lane = threadIdx.x - group * tpr;
+    any = MODE == FULL || channel(0) < C;
+  }
+  __device__ __forceinline__ int channel(int e) const { return MODE != STRIDED ? lane * 8 + e : e * tpr + lane; }
+  __device__ __forceinline__ bool on(int e) const { return MODE == FULL ? true : MODE == ALIGNED ? any : channel(e) < C; }
   // the slot of a [C] table in shared memory: two halves of four channels a thread, so that a warp's 16-byte reads are
   // consecutive
   __device__ __forceinline__ int slot(int e) const { return (e >> 2) * tpr * 4 + lane * 4 + (e & 3); }
-  __device__ __forceinline__ void load(const T* row, float (&v)[8]) const {
-    if (ALIGNED) {
-      if (on(0)) {
-        const Eight<T> p = *reinterpret_cast<const Eight<T>*>(row + lane * 8);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = Io<T>::get(p.v[e]);
+  // The thread's channels of a row; `mine` is where its first one lies.
+  __device__ __forceinline__ Eight load(const T* mine) const {
+    Eight v;
+    if (MODE != STRIDED) {
+      if (MODE == FULL || any) {
+        if constexpr (sizeof(T) == 2) {
+          const uint4 u = *reinterpret_cast<const uint4*>(mine);
+          v.p[0] = sw_unpack(u.x, T());
+          v.p[1] = sw_unpack(u.y, T());
+          v.p[2] = sw_unpack(u.z, T());
+          v.p[3] = sw_unpack(u.w, T());
+        } else {
+          const float4 a = *reinterpret_cast<const float4*>(mine), b = *reinterpret_cast<const float4*>(mine + 4);
+          v.p[0] = make_float2(a.x, a.y);
+          v.p[1] = make_float2(a.z, a.w);
+          v.p[2] = make_float2(b.x, b.y);
+          v.p[3] = make_float2(b.z, b.w);
+        }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        for (int k = 0; k < 4; ++k) v.p[k] = sw_both(0.f);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = on(e) ? Io<T>::get(row[e * tpr + lane]) : 0.f;
+      for (int k = 0; k < 4; ++k) {
+        v.p[k].x = on(2 * k) ? Io<T>::get(mine[2 * k * tpr]) : 0.f;
+        v.p[k].y = on(2 * k + 1) ? Io<T>::get(mine[(2 * k + 1) * tpr]) : 0.f;
+      }
     }
+    return v;
   }
-  __device__ __forceinline__ void store(T* row, const float (&v)[8]) const {
-    if (ALIGNED) {
-      if (on(0)) {
-        Eight<T> p;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p.v[e] = Io<T>::put(v[e]);
-        *reinterpret_cast<Eight<T>*>(row + lane * 8) = p;
+  __device__ __forceinline__ void store(T* mine, const Eight& v) const {
+    if (MODE != STRIDED) {
+      if (MODE == FULL || any) {
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint4*>(mine) =
+              make_uint4(sw_pack(v.p[0], T()), sw_pack(v.p[1], T()), sw_pack(v.p[2], T()), sw_pack(v.p[3], T()));
+        } else {
+          *reinterpret_cast<float4*>(mine) = make_float4(v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y);
+          *reinterpret_cast<float4*>(mine + 4) = make_float4(v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y);
+        }
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (on(e)) row[e * tpr + lane] = Io<T>::put(v[e]);
+      for (int k = 0; k < 4; ++k) {
+        if (on(2 * k)) mine[2 * k * tpr] = Io<T>::put(v.p[k].x);
+        if (on(2 * k + 1)) mine[(2 * k + 1) * tpr] = Io<T>::put(v.p[k].y);
+      }
     }
   }
-  __device__ __forceinline__ void table(const float* t, float (&v)[8]) const {
-    const float4 a = *reinterpret_cast<const float4*>(t + lane * 4);
-    const float4 b = *reinterpret_cast<const float4*>(t + tpr * 4 + lane * 4);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  __device__ __forceinline__ Eight table(const float* t) const {
+    const float4 a = *reinterpret_cast<const float4*>(t + lane * 4), b = *reinterpret_cast<const float4*>(t + tpr * 4 + lane * 4);
+    return Eight{{make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)}};
+  }
+  // (v - mean) with zeros behind the row
+  __device__ __forceinline__ Eight centred(const Eight& v, float mean) const {
+    Eight r;
+    const float2 m = sw_both(MODE == ALIGNED && !any ? 0.f : -mean);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      r.p[k] = add2(v.p[k], m);
+      if (MODE == STRIDED && !on(2 * k)) r.p[k].x = 0.f;
+      if (MODE == STRIDED && !on(2 * k + 1)) r.p[k].y = 0.f;
+    }
+    return r;
   }
 };
 
-// Sums over the threads of a group, in every one of them and in the same order. slots: [2][16] pairs of the group; the barrier
-// of one sum keeps the slots of the one before it from being overwritten too early, so two sets are enough.
+// Whether rows are fetched to shared memory ahead of their use: in words of 4 bytes at least, each thread its own channels.
+template <typename T, int MODE>
+constexpr bool SW_RING = MODE != STRIDED || sizeof(T) == 4;
+
+template <typename T, int MODE>
+__device__ __forceinline__ void sw_fetch(const Place<T, MODE>& at, uint8_t* to, const T* from) {
+  if (MODE != STRIDED) {
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(8 * sizeof(T)); j += 16) sw_cp_async_16(to + j, reinterpret_cast<const uint8_t*>(from) + j);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (at.on(e)) sw_cp_async_4(to + e * at.tpr * sizeof(T), from + e * at.tpr);
+  }
+}
+
+// Sums of two numbers over the threads of a group, in every one of them and in the same order. Within a warp one exchange gives
+// either number to half of the lanes, which then add it up in four; the warps' sums meet in slots: [2][2][16] of the group,
+// the ones behind the last warp zero. The barrier of one sum keeps the slots of the one before it from being
+// overwritten too early, so two sets are enough.
 struct GroupSum {
-  float2* slots;
+  float* slots;
   int warps, warp, bar, threads, phase;
   __device__ __forceinline__ void two(float& a, float& b) {
-    a = warp_sum(a);
-    b = warp_sum(b);
-    if (warps == 1) return;
-    float2* s = slots + phase * 16;
-    phase ^= 1;
-    if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
-    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
-    a = b = 0.f;
-    for (int w = 0; w < warps; ++w) {
-      const float2 v = s[w];
-      a += v.x;
-      b += v.y;
+    const int lane = threadIdx.x & 31;
+    const bool high = lane & 16;
+    const float keep = high ? b : a, give = high ? a : b;
+    float v = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (warps == 1) {
+      a = __shfl_sync(0xffffffffu, v, 0);
+      b = __shfl_sync(0xffffffffu, v, 16);
+      return;
     }
-  }
-  __device__ __forceinline__ float one(float a) {
-    float b = 0.f;
-    a = warp_sum(a);
-    if (warps == 1) return a;
-    float2* s = slots + phase * 16;
+    float* s = slots + phase * 32;
     phase ^= 1;
-    if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, 0.f);
+    if ((lane & 15) == 0) s[lane + warp] = v;     // lane 0: the first sixteen, lane 16: the others
     asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(threads) : "memory");
-    for (int w = 0; w < warps; ++w) b += s[w].x;
-    return b;
+    const float4 x = *reinterpret_cast<const float4*>(s), y = *reinterpret_cast<const float4*>(s + 16);
+    a = (x.x + x.y) + (x.z + x.w);
+    b = (y.x + y.y) + (y.z + y.w);
+    for (int w = 4; w < warps; w += 4) {
+      const float4 x2 = *reinterpret_cast<const float4*>(s + w), y2 = *reinterpret_cast<const float4*>(s + 16 + w);
+      a += (x2.x + x2.y) + (x2.z + x2.w);
+      b += (y2.x + y2.y) + (y2.z + y2.w);
+    }
   }
 };
 
@@ -154,323 +233,389 @@ __device__ __forceinline__ float sw_param(const void* p, int c, int param32) {
   return param32 ? static_cast<const float*>(p)[c] : Io<T>::get(static_cast<const T*>(p)[c]);
 }
 
-// Shared memory: tables post, next, scale, gate [4][tpr * 8] fp32 | sums [groups][2][16] float2 | ring [groups][stages][parts][C]
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ void sw_tables(const SandwichArgs& a, const Place<T, ALIGNED>& at, float* tables) {
-  if (at.group == 0) {
-    const int wide = a.tpr * 8;
+// Shared memory: tables post, next, scale, gate [4][tpr * 8] fp32 | sums [groups][2][2][16] | ring [groups][stages][rows][parts][C]
+template <typename T, int MODE>
+__device__ __forceinline__ void sw_tables(const SandwichArgs& a, const Place<T, MODE>& at, float* tables, float* sums) {
+  const int wide = a.tpr * 8;
+  const void* of[4] = {a.post, a.next, a.scale, a.gate_mode == GATE_CHANNEL ? a.gate : nullptr};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (k % a.groups != at.group) continue;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int c = at.channel(e);
-      const bool on = c < a.C;
-      const int s = at.slot(e);
-      tables[s] = on ? sw_param<T>(a.post, c, a.param32) : 0.f;
-      tables[wide + s] = on ? sw_param<T>(a.next, c, a.param32) : 0.f;
-      tables[2 * wide + s] = on ? sw_param<T>(a.scale, c, a.param32) : 0.f;
-      tables[3 * wide + s] = !on ? 0.f : a.gate_mode == GATE_CHANNEL ? sw_param<T>(a.gate, c, a.param32) : 1.f;
+      tables[k * wide + at.slot(e)] = c < a.C ? sw_param<T>(of[k], c, a.param32) : 0.f;
     }
   }
+  for (int i = threadIdx.x; i < a.groups * 64; i += blockDim.x) sums[i] = 0.f;
   __syncthreads();
 }
 
-__device__ __forceinline__ float sw_sigmoid(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// 1 / (1 + e^-v) by the approximate exponential and reciprocal: 2^-21 of the value for |v| up to 8; 0 where e^-v overflows.
+__device__ __forceinline__ Eight sw_sigmoid(const Eight& v) {
+  Eight r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    float2 t = mul2(v.p[k], sw_both(-1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(t.y));
+    t = add2(t, sw_both(1.f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.p[k].x) : "f"(t.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.p[k].y) : "f"(t.y));
+  }
+  return r;
+}
+__device__ __forceinline__ Eight sw_mul(const Eight& a, const Eight& b) {
+  Eight r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r.p[k] = mul2(a.p[k], b.p[k]);
+  return r;
+}
+__device__ __forceinline__ Eight sw_scaled(const Eight& a, float s) {
+  Eight r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r.p[k] = mul2(a.p[k], sw_both(s));
+  return r;
+}
+__device__ __forceinline__ Eight sw_fma(const Eight& a, const Eight& b, const Eight& c) {
+  Eight r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r.p[k] = fma2(a.p[k], b.p[k], c.p[k]);
+  return r;
+}
+__device__ __forceinline__ Eight sw_add(const Eight& a, const Eight& b) {
+  Eight r;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r.p[k] = add2(a.p[k], b.p[k]);
+  return r;
+}
 
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(512, 2)
+// GATE: the gate's form, or -1 where it is looked up. (The full mode has a kernel for each form that reads different rows.)
+constexpr int GATE_ANY = -1;
+
+// Two rows at a time: their sums share the exchanges and barriers, and the tables are read once for both.
+template <typename T, int MODE, int GATE>
+__global__ void __maxnreg__(MODE == STRIDED ? 128 : 80)
 sandwich_fwd_kernel(const __grid_constant__ SandwichArgs a) {
   extern __shared__ __align__(128) uint8_t sw_smem[];
-  const int group = threadIdx.x / a.tpr;
-  const Place<T, ALIGNED> at{static_cast<int>(threadIdx.x) - group * a.tpr, group, a.tpr, a.C};
+  const Place<T, MODE> at(a.tpr, a.C);
   float* tables = reinterpret_cast<float*>(sw_smem);
   const int wide = a.tpr * 8;
-  float2* sums = reinterpret_cast<float2*>(tables + 4 * wide);
-  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + a.groups * 32);
-  GroupSum sum{sums + group * 32, a.tpr >> 5, at.lane >> 5, 1 + group, a.tpr, 0};
-  const bool token_gate = a.gate_mode >= GATE_TOKEN;
-  const int parts = token_gate ? 3 : 2;
-  const size_t row_bytes = static_cast<size_t>(a.C) * sizeof(T);
-  ring += static_cast<size_t>(group) * SW_STAGES * parts * row_bytes;
+  float* sums = tables + 4 * wide;
+  GroupSum sum{sums + at.group * 64, a.tpr >> 5, at.lane >> 5, 1 + at.group, a.tpr, 0};
+  const int gate_mode = GATE == GATE_ANY ? a.gate_mode : GATE == GATE_NONE ? (a.gate_mode ? GATE_CHANNEL : GATE_NONE) : GATE;
+  const bool token_gate = GATE == GATE_ANY ? gate_mode >= GATE_TOKEN : GATE >= GATE_TOKEN;
+  const uint32_t row_bytes = static_cast<uint32_t>(a.C) * sizeof(T), parts = token_gate ? 3 : 2;
+  const uint32_t step_bytes = 2 * parts * row_bytes;      // two rows of all parts
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + a.groups * 64) + at.group * a.stages * step_bytes + at.channel(0) * sizeof(T);
   grid_chain();
-  const long long row0 = static_cast<long long>(blockIdx.x) * a.groups + group;
+  const long long row0 = static_cast<long long>(blockIdx.x) * a.groups + at.group;
   const long long stride = static_cast<long long>(gridDim.x) * a.groups;
-  const T *x = static_cast<const T*>(a.x), *f = static_cast<const T*>(a.f), *gate = static_cast<const T*>(a.gate);
-  auto fetch = [&](long long row, int stage) {
-    if (ALIGNED) {
-      if (row < a.T && at.on(0)) {
-        uint8_t* d = ring + static_cast<size_t>(stage) * parts * row_bytes + at.lane * sizeof(Eight<T>);
+  // where the thread's channels of the row to fetch next lie, and how far the next row is
+  const T *x = static_cast<const T*>(a.x) + row0 * a.xs + at.channel(0), *f = static_cast<const T*>(a.f) + row0 * a.fs + at.channel(0);
+  const T* gate = token_gate ? static_cast<const T*>(a.gate) + row0 * a.gs + at.channel(0) : nullptr;
+  const long long dx = stride * a.xs, df = stride * a.fs, dg = stride * a.gs, dy = stride * a.C;
+  T *y = static_cast<T*>(a.y) + row0 * a.C + at.channel(0), *h = static_cast<T*>(a.h) + row0 * a.C + at.channel(0);
+  const bool with_next = a.h != nullptr;
+  long long ahead = row0;     // the row that `x` and the others are at
+  auto fetch = [&](uint32_t stage) {
+    if (SW_RING<T, MODE>) {
+      uint8_t* d = ring + stage * step_bytes;
 #pragma unroll
-        for (int j = 0; j < static_cast<int>(sizeof(Eight<T>)); j += 16) {
-          sw_cp_async_16(d + j, reinterpret_cast<const uint8_t*>(x + row * a.xs + at.lane * 8) + j);
-          sw_cp_async_16(d + row_bytes + j, reinterpret_cast<const uint8_t*>(f + row * a.fs + at.lane * 8) + j);
-          if (token_gate)
-            sw_cp_async_16(d + 2 * row_bytes + j, reinterpret_cast<const uint8_t*>(gate + row * a.gs + at.lane * 8) + j);
+      for (int k = 0; k < 2; ++k) {
+        if (ahead < a.T && at.any) {
+          sw_fetch(at, d, x);
+          sw_fetch(at, d + row_bytes, f);
+          if (token_gate) sw_fetch(at, d + 2 * row_bytes, gate);
         }
+        d += parts * row_bytes;
+        x += dx;
+        f += df;
+        if (token_gate) gate += dg;
+        ahead += stride;
       }
       sw_cp_commit();
     }
   };
-#pragma unroll
-  for (int i = 0; i < SW_STAGES; ++i) fetch(row0 + i * stride, i);
-  sw_tables<T, ALIGNED>(a, at, tables);
+  for (int i = 0; i < a.stages; ++i) fetch(i);
+  sw_tables<T, MODE>(a, at, tables, sums);
   const float inv_c = 1.f / a.C;
-  int stage = 0;
-  for (long long row = row0; row < a.T; row += stride) {
-    float v[8], xv[8], w[8];
-    const T *px, *pf, *pg;
-    if (ALIGNED) {
-      sw_cp_wait<SW_STAGES - 1>();
-      const uint8_t* s = ring + static_cast<size_t>(stage) * parts * row_bytes;
-      px = reinterpret_cast<const T*>(s);
-      pf = reinterpret_cast<const T*>(s + row_bytes);
-      pg = reinterpret_cast<const T*>(s + 2 * row_bytes);
+  uint32_t stage = 0;
+  for (long long row = row0; row < a.T; row += 2 * stride) {
+    const bool two = row + stride < a.T;     // (a second row that is not there holds what the memory did, and is not stored)
+    const T *px[2], *pf[2], *pg[2];
+    if (SW_RING<T, MODE>) {
+      const uint8_t* s = ring + stage * step_bytes;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        px[k] = reinterpret_cast<const T*>(s + k * parts * row_bytes);
+        pf[k] = reinterpret_cast<const T*>(s + k * parts * row_bytes + row_bytes);
+        pg[k] = reinterpret_cast<const T*>(s + k * parts * row_bytes + 2 * row_bytes);
+      }
+      if (a.stages > 1) sw_cp_wait<1>();
+      else sw_cp_wait<0>();
     } else {
-      px = x + row * a.xs;
-      pf = f + row * a.fs;
-      pg = gate + row * a.gs;
+      px[0] = x;
+      pf[0] = f;
+      pg[0] = gate;
+      px[1] = two ? x + dx : x;
+      pf[1] = two ? f + df : f;
+      pg[1] = two ? gate + dg : gate;
     }
-    at.load(pf, v);
-    at.load(px, xv);
     // norm of the block's output
-    float mean_f = 0.f, s = 0.f;
+    Eight v[2];
+    v[0] = at.load(pf[0]);
+    v[1] = at.load(pf[1]);
+    float mean_f[2] = {0.f, 0.f}, rstd_f[2];
     if (!a.rms) {
+      mean_f[0] = sw_total(v[0]);
+      mean_f[1] = sw_total(v[1]);
+      sum.two(mean_f[0], mean_f[1]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += v[e];
-      mean_f = sum.one(s) * inv_c;
+      for (int k = 0; k < 2; ++k) {
+        mean_f[k] *= inv_c;
+        v[k] = at.centred(v[k], mean_f[k]);
+      }
     }
-    s = 0.f;
+    rstd_f[0] = sw_dot(v[0], v[0]);
+    rstd_f[1] = sw_dot(v[1], v[1]);
+    sum.two(rstd_f[0], rstd_f[1]);
+    {
+      const Eight w = at.table(tables);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = at.on(e) ? v[e] - mean_f : 0.f;
-      s += v[e] * v[e];
+      for (int k = 0; k < 2; ++k) {
+        rstd_f[k] = rsqrtf(fmaf(rstd_f[k], inv_c, a.eps));
+        v[k] = sw_mul(sw_scaled(v[k], rstd_f[k]), w);
+      }
     }
-    const float rstd_f = rsqrtf(sum.one(s) * inv_c + a.eps);
-    at.table(tables, w);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * rstd_f * w[e];
     // gate, residual scale, sum
     if (token_gate) {
-      at.load(pg, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= a.gate_mode == GATE_SIGMOID ? sw_sigmoid(w[e]) : w[e];
-    } else if (a.gate_mode == GATE_CHANNEL) {
-      at.table(tables + 3 * wide, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= w[e];
+      for (int k = 0; k < 2; ++k) {
+        const Eight g = at.load(pg[k]);
+        v[k] = sw_mul(v[k], gate_mode == GATE_SIGMOID ? sw_sigmoid(g) : g);
+      }
+    } else if (gate_mode == GATE_CHANNEL) {
+      const Eight g = at.table(tables + 3 * wide);
+      v[0] = sw_mul(v[0], g);
+      v[1] = sw_mul(v[1], g);
     }
     if (a.scale != nullptr) {
-      at.table(tables + 2 * wide, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += w[e] * xv[e];
+      const Eight r = at.table(tables + 2 * wide);
+      v[0] = sw_fma(r, at.load(px[0]), v[0]);
+      v[1] = sw_fma(r, at.load(px[1]), v[1]);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += xv[e];
+      v[0] = sw_add(at.load(px[0]), v[0]);
+      v[1] = sw_add(at.load(px[1]), v[1]);
     }
-    at.store(static_cast<T*>(a.y) + row * a.C, v);
-    fetch(row + SW_STAGES * stride, stage);
-    if (++stage == SW_STAGES) stage = 0;
-    float mean_y = 0.f, rstd_y = 0.f;
-    if (a.h != nullptr) {       // the next block's norm
-      s = 0.f;
+    at.store(y, v[0]);
+    if (two) at.store(y + dy, v[1]);
+    y += 2 * dy;
+    if (SW_RING<T, MODE>) {
+      fetch(stage);
+      if (++stage == a.stages) stage = 0;
+    } else {
+      x += 2 * dx;
+      f += 2 * df;
+      if (token_gate) gate += 2 * dg;
+    }
+    float mean_y[2] = {0.f, 0.f}, rstd_y[2] = {0.f, 0.f};
+    if (with_next) {       // the next block's norm
       if (!a.rms) {
+        mean_y[0] = sw_total(v[0]);
+        mean_y[1] = sw_total(v[1]);
+        sum.two(mean_y[0], mean_y[1]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += v[e];
-        mean_y = sum.one(s) * inv_c;
+        for (int k = 0; k < 2; ++k) {
+          mean_y[k] *= inv_c;
+          v[k] = at.centred(v[k], mean_y[k]);
+        }
       }
-      s = 0.f;
+      rstd_y[0] = sw_dot(v[0], v[0]);
+      rstd_y[1] = sw_dot(v[1], v[1]);
+      sum.two(rstd_y[0], rstd_y[1]);
+      const Eight w = at.table(tables + wide);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = at.on(e) ? v[e] - mean_y : 0.f;
-        s += v[e] * v[e];
+      for (int k = 0; k < 2; ++k) {
+        rstd_y[k] = rsqrtf(fmaf(rstd_y[k], inv_c, a.eps));
+        v[k] = sw_mul(sw_scaled(v[k], rstd_y[k]), w);
       }
-      rstd_y = rsqrtf(sum.one(s) * inv_c + a.eps);
-      at.table(tables + wide, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] * rstd_y * w[e];
-      at.store(static_cast<T*>(a.h) + row * a.C, v);
+      at.store(h, v[0]);
+      if (two) at.store(h + dy, v[1]);
+      h += 2 * dy;
     }
     if (a.stats != nullptr && at.lane == 0) {
-      a.stats[row] = mean_f;
-      a.stats[a.T + row] = rstd_f;
-      a.stats[2 * a.T + row] = mean_y;
-      a.stats[3 * a.T + row] = rstd_y;
+      a.stats[row] = make_float4(mean_f[0], rstd_f[0], mean_y[0], rstd_y[0]);
+      if (two) a.stats[row + stride] = make_float4(mean_f[1], rstd_f[1], mean_y[1], rstd_y[1]);
     }
   }
 }
 
-template <typename T, bool ALIGNED>
+template <typename T, int MODE, int GATE>
 __global__ void __launch_bounds__(512)
 sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
   extern __shared__ __align__(128) uint8_t sw_smem[];
-  const int group = threadIdx.x / a.tpr;
-  const Place<T, ALIGNED> at{static_cast<int>(threadIdx.x) - group * a.tpr, group, a.tpr, a.C};
+  const Place<T, MODE> at(a.tpr, a.C);
   float* tables = reinterpret_cast<float*>(sw_smem);
   const int wide = a.tpr * 8;
-  float2* sums = reinterpret_cast<float2*>(tables + 4 * wide);
-  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + a.groups * 32);
-  GroupSum sum{sums + group * 32, a.tpr >> 5, at.lane >> 5, 1 + group, a.tpr, 0};
-  const bool token_gate = a.gate_mode >= GATE_TOKEN, has_dy = a.dy != nullptr, has_dh = a.dh != nullptr;
-  const int parts = 2 + token_gate + has_dy + has_dh;
-  const size_t row_bytes = static_cast<size_t>(a.C) * sizeof(T);
-  uint8_t* mine = ring + static_cast<size_t>(group) * SW_STAGES * parts * row_bytes;
+  float* sums = tables + 4 * wide;
+  GroupSum sum{sums + at.group * 64, a.tpr >> 5, at.lane >> 5, 1 + at.group, a.tpr, 0};
+  const int gate_mode = GATE == GATE_ANY ? a.gate_mode : GATE;      // (none and a weight are the same: the table has the ones)
+  const bool token_gate = gate_mode >= GATE_TOKEN;
+  const bool has_dy = a.dy != nullptr, has_dh = a.dh != nullptr;
+  const uint32_t row_bytes = static_cast<uint32_t>(a.C) * sizeof(T);
+  const uint32_t o_dy = 2 * row_bytes, o_dh = o_dy + has_dy * row_bytes, o_g = o_dh + has_dh * row_bytes;
+  const uint32_t step_bytes = o_g + token_gate * row_bytes;
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + a.groups * 64) + at.group * a.stages * step_bytes + at.channel(0) * sizeof(T);
   grid_chain();
-  const long long row0 = static_cast<long long>(blockIdx.x) * a.groups + group;
+  const long long row0 = static_cast<long long>(blockIdx.x) * a.groups + at.group;
   const long long stride = static_cast<long long>(gridDim.x) * a.groups;
-  const T *x = static_cast<const T*>(a.x), *f = static_cast<const T*>(a.f), *gate = static_cast<const T*>(a.gate);
-  const T *dy = static_cast<const T*>(a.dy), *dh = static_cast<const T*>(a.dh);
-  const size_t o_dy = 2 * row_bytes, o_dh = o_dy + has_dy * row_bytes, o_g = o_dh + has_dh * row_bytes;
-  auto fetch = [&](long long row, int stage) {
-    if (ALIGNED) {
-      if (row < a.T && at.on(0)) {
-        uint8_t* d = mine + static_cast<size_t>(stage) * parts * row_bytes + at.lane * sizeof(Eight<T>);
-        const int c = at.lane * 8;
-#pragma unroll
-        for (int j = 0; j < static_cast<int>(sizeof(Eight<T>)); j += 16) {
-          sw_cp_async_16(d + j, reinterpret_cast<const uint8_t*>(x + row * a.xs + c) + j);
-          sw_cp_async_16(d + row_bytes + j, reinterpret_cast<const uint8_t*>(f + row * a.fs + c) + j);
-          if (has_dy) sw_cp_async_16(d + o_dy + j, reinterpret_cast<const uint8_t*>(dy + row * a.dys + c) + j);
-          if (has_dh) sw_cp_async_16(d + o_dh + j, reinterpret_cast<const uint8_t*>(dh + row * a.dhs + c) + j);
-          if (token_gate) sw_cp_async_16(d + o_g + j, reinterpret_cast<const uint8_t*>(gate + row * a.gs + c) + j);
-        }
+  const int c0 = at.channel(0);
+  const T *x = static_cast<const T*>(a.x) + row0 * a.xs + c0, *f = static_cast<const T*>(a.f) + row0 * a.fs + c0;
+  const T* gate = token_gate ? static_cast<const T*>(a.gate) + row0 * a.gs + c0 : nullptr;
+  const T* dy = has_dy ? static_cast<const T*>(a.dy) + row0 * a.dys + c0 : nullptr;
+  const T* dh = has_dh ? static_cast<const T*>(a.dh) + row0 * a.dhs + c0 : nullptr;
+  const long long nx = stride * a.xs, nf = stride * a.fs, ng = stride * a.gs, ndy = stride * a.dys, ndh = stride * a.dhs;
+  const long long nout = stride * a.C;
+  long long out = row0 * a.C + c0;
+  long long ahead = row0;
+  auto advance = [&]() {
+    x += nx;
+    f += nf;
+    if (has_dy) dy += ndy;
+    if (has_dh) dh += ndh;
+    if (token_gate) gate += ng;
+  };
+  auto fetch = [&](uint32_t stage) {
+    if (SW_RING<T, MODE>) {
+      if (ahead < a.T && at.any) {
+        uint8_t* d = ring + stage * step_bytes;
+        sw_fetch(at, d, x);
+        sw_fetch(at, d + row_bytes, f);
+        if (has_dy) sw_fetch(at, d + o_dy, dy);
+        if (has_dh) sw_fetch(at, d + o_dh, dh);
+        if (token_gate) sw_fetch(at, d + o_g, gate);
       }
+      advance();
+      ahead += stride;
       sw_cp_commit();
     }
   };
-#pragma unroll
-  for (int i = 0; i < SW_STAGES; ++i) fetch(row0 + i * stride, i);
-  sw_tables<T, ALIGNED>(a, at, tables);
+  for (int i = 0; i < a.stages; ++i) fetch(i);
+  sw_tables<T, MODE>(a, at, tables, sums);
   const float inv_c = 1.f / a.C;
-  float acc[4][8];
+  Eight acc[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[k][e] = 0.f;
-  int stage = 0;
+    for (int e = 0; e < 4; ++e) acc[k].p[e] = sw_both(0.f);
+  uint32_t stage = 0;
+  float4 st = make_float4(0.f, 0.f, 0.f, 0.f);      // statistics of the next row
+  if (row0 < a.T) st = a.stats[row0];
   for (long long row = row0; row < a.T; row += stride) {
-    const float mean_f = a.stats[row], rstd_f = a.stats[a.T + row];
-    const float mean_y = a.stats[2 * a.T + row], rstd_y = a.stats[3 * a.T + row];
+    const float mean_f = st.x, rstd_f = st.y, mean_y = st.z, rstd_y = st.w;
+    if (row + stride < a.T) st = a.stats[row + stride];
     const T *px, *pf, *pdy, *pdh, *pg;
-    if (ALIGNED) {
-      sw_cp_wait<SW_STAGES - 1>();
-      const uint8_t* s = mine + static_cast<size_t>(stage) * parts * row_bytes;
+    if (SW_RING<T, MODE>) {
+      const uint8_t* s = ring + stage * step_bytes;
       px = reinterpret_cast<const T*>(s);
       pf = reinterpret_cast<const T*>(s + row_bytes);
       pdy = reinterpret_cast<const T*>(s + o_dy);
       pdh = reinterpret_cast<const T*>(s + o_dh);
       pg = reinterpret_cast<const T*>(s + o_g);
+      if (a.stages > 1) sw_cp_wait<1>();
+      else sw_cp_wait<0>();
     } else {
-      px = x + row * a.xs;
-      pf = f + row * a.fs;
-      pdy = dy + row * a.dys;
-      pdh = dh + row * a.dhs;
-      pg = gate + row * a.gs;
+      px = x;
+      pf = f;
+      pdy = dy;
+      pdh = dh;
+      pg = gate;
     }
-    float uf[8], g[8], t[8], w[8];      // u(f), the gate, t
-    at.load(pf, uf);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) uf[e] = at.on(e) ? (uf[e] - mean_f) * rstd_f : 0.f;
+    const Eight uf = sw_scaled(at.centred(at.load(pf), mean_f), rstd_f);       // u(f)
+    Eight g, t;
     if (token_gate) {
-      at.load(pg, g);
-      if (a.gate_mode == GATE_SIGMOID) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = sw_sigmoid(g[e]);
-      }
+      g = at.load(pg);
+      if (gate_mode == GATE_SIGMOID) g = sw_sigmoid(g);
     } else {
-      at.table(tables + 3 * wide, g);
+      g = at.table(tables + 3 * wide);
     }
     if (has_dh) {
-      float uy[8], v[8];
-      at.table(tables, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) uy[e] = g[e] * (uf[e] * w[e]);
-      at.load(px, v);
-      at.table(tables + 2 * wide, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) uy[e] = at.on(e) ? (uy[e] + w[e] * v[e] - mean_y) * rstd_y : 0.f;
-      at.load(pdh, v);
-      at.table(tables + wide, w);
-      float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        acc[0][e] += v[e] * uy[e];
-        t[e] = v[e] * w[e];
-        s1 += t[e];
-        s2 += t[e] * uy[e];
-      }
+      Eight uy = sw_mul(g, sw_mul(uf, at.table(tables)));
+      uy = sw_fma(at.table(tables + 2 * wide), at.load(px), uy);
+      uy = sw_scaled(at.centred(uy, mean_y), rstd_y);
+      const Eight d = at.load(pdh);
+      acc[0] = sw_fma(d, uy, acc[0]);
+      t = sw_mul(d, at.table(tables + wide));
+      float s1 = sw_total(t), s2 = sw_dot(t, uy);
       sum.two(s1, s2);
-      s1 = a.rms ? 0.f : s1 * inv_c;
-      s2 *= inv_c;
+      s1 = a.rms ? 0.f : -s1 * inv_c * rstd_y;
+      s2 *= -inv_c * rstd_y;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = rstd_y * (t[e] - s1 - uy[e] * s2);
-      if (has_dy) {
-        at.load(pdy, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] += v[e];
-      }
+      for (int k = 0; k < 4; ++k) t.p[k] = fma2(uy.p[k], sw_both(s2), fma2(t.p[k], sw_both(rstd_y), sw_both(s1)));
+      if (has_dy) t = sw_add(t, at.load(pdy));
     } else {
-      at.load(pdy, t);
+      t = at.load(pdy);
     }
     {   // dx, and the sum for the residual scale
-      float v[8], o[8];
-      at.load(px, v);
-      at.table(tables + 2 * wide, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (at.on(e)) acc[2][e] += t[e] * v[e];
-        o[e] = w[e] * t[e];
-      }
-      at.store(static_cast<T*>(a.dx) + row * a.C, o);
+      acc[2] = sw_fma(t, at.load(px), acc[2]);
+      at.store(static_cast<T*>(a.dx) + out, sw_mul(t, at.table(tables + 2 * wide)));
     }
-    at.table(tables, w);
-    float s1 = 0.f, s2 = 0.f;
+    const Eight w = at.table(tables);
+    const Eight tn = sw_mul(t, sw_mul(uf, w));      // t n
     if (token_gate) {
-      float o[8];
+      if (gate_mode == GATE_SIGMOID) {
+        Eight o;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        o[e] = t[e] * (uf[e] * w[e]);
-        if (a.gate_mode == GATE_SIGMOID) o[e] *= g[e] * (1.f - g[e]);
+        for (int k = 0; k < 4; ++k) {     // g (1 - g)
+          const float2 slope = fma2(make_float2(-g.p[k].x, -g.p[k].y), g.p[k], g.p[k]);
+          o.p[k] = mul2(tn.p[k], slope);
+        }
+        at.store(static_cast<T*>(a.dg) + out, o);
+      } else {
+        at.store(static_cast<T*>(a.dg) + out, tn);
       }
-      at.store(static_cast<T*>(a.dg) + row * a.C, o);
     } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (at.on(e)) acc[3][e] += t[e] * (uf[e] * w[e]);
+      acc[3] = sw_add(acc[3], tn);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      t[e] = at.on(e) ? t[e] * g[e] : 0.f;
-      acc[1][e] += t[e] * uf[e];
-      t[e] *= w[e];
-      s1 += t[e];
-      s2 += t[e] * uf[e];
-    }
+    t = sw_mul(t, g);
+    acc[1] = sw_fma(t, uf, acc[1]);
+    t = sw_mul(t, w);
+    float s1 = sw_total(t), s2 = sw_dot(t, uf);
     sum.two(s1, s2);
-    s1 = a.rms ? 0.f : s1 * inv_c;
-    s2 *= inv_c;
+    s1 = a.rms ? 0.f : -s1 * inv_c * rstd_f;
+    s2 *= -inv_c * rstd_f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = rstd_f * (t[e] - s1 - uf[e] * s2);
-    at.store(static_cast<T*>(a.df) + row * a.C, t);
-    fetch(row + SW_STAGES * stride, stage);
-    if (++stage == SW_STAGES) stage = 0;
+    for (int k = 0; k < 4; ++k) t.p[k] = fma2(uf.p[k], sw_both(s2), fma2(t.p[k], sw_both(rstd_f), sw_both(s1)));
+    at.store(static_cast<T*>(a.df) + out, t);
+    out += nout;
+    if (SW_RING<T, MODE>) {
+      fetch(stage);
+      if (++stage == a.stages) stage = 0;
+    } else {
+      advance();
+    }
   }
   if (a.want == 0) return;
   // the groups' column sums meet in the tables' memory, one kind at a time, and leave as this block's partial sums
-  if (ALIGNED) sw_cp_wait<0>();
+  if (SW_RING<T, MODE>) sw_cp_wait<0>();
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (!(a.want >> k & 1)) continue;
     float* out = a.partial + (static_cast<size_t>(k) * gridDim.x + blockIdx.x) * a.C;
     for (int j = 0; j < a.groups; ++j) {
       __syncthreads();
-      if (group == j) {
+      if (at.group == j) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int s = at.slot(e);
-          tables[s] = j ? tables[s] + acc[k][e] : acc[k][e];
+          const int q = at.slot(e);
+          const float v = e & 1 ? acc[k].p[e / 2].y : acc[k].p[e / 2].x;
+          tables[q] = j ? tables[q] + v : v;
         }
       }
     }
     __syncthreads();
-    if (group == 0) {
+    if (at.group == 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (at.channel(e) < a.C) out[at.channel(e)] = tables[at.slot(e)];
@@ -484,48 +629,66 @@ struct ColumnSums {
   int kind[4];
 };
 
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(1024)
 sandwich_columns_kernel(const float* __restrict__ partial, const __grid_constant__ ColumnSums to, int blocks, int C) {
   grid_chain();
-  __shared__ float part[16][33];
+  __shared__ float part[32][33];
   const int k = blockIdx.y, c = blockIdx.x * 32 + threadIdx.x;
   if (to.kind[k] == 0) return;
   float s = 0.f;
-  if (c < C)
-    for (int b = threadIdx.y; b < blocks; b += 16) s += partial[(static_cast<size_t>(k) * blocks + b) * C + c];
+  if (c < C) {
+    const float* p = partial + (static_cast<size_t>(k) * blocks + threadIdx.y) * C + c;
+    const size_t step = static_cast<size_t>(32) * C;
+    int b = threadIdx.y;
+    for (; b + 96 < blocks; b += 128, p += 4 * step) s += (p[0] + p[step]) + (p[2 * step] + p[3 * step]);
+    for (; b < blocks; b += 32, p += step) s += *p;
+  }
   part[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && c < C) {
-    s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) s += part[j][threadIdx.x];
-    if (to.kind[k] == 1) static_cast<__nv_bfloat16*>(to.out[k])[c] = __float2bfloat16_rn(s);
-    else if (to.kind[k] == 2) static_cast<__half*>(to.out[k])[c] = __float2half_rn(s);
-    else if (to.kind[k] == 3) static_cast<float*>(to.out[k])[c] = s;
-    else static_cast<float*>(to.out[k])[c] += s;
+  // warp y adds up column y
+  s = part[threadIdx.x][threadIdx.y];
+  s = warp_sum(s);
+  const int mine = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && mine < C) {
+    if (to.kind[k] == 1) static_cast<__nv_bfloat16*>(to.out[k])[mine] = __float2bfloat16_rn(s);
+    else if (to.kind[k] == 2) static_cast<__half*>(to.out[k])[mine] = __float2half_rn(s);
+    else if (to.kind[k] == 3) static_cast<float*>(to.out[k])[mine] = s;
+    else static_cast<float*>(to.out[k])[mine] += s;
   }
 }
 
-static int sw_shape(int C, int* tpr, int* groups) {
-  if (C < 1 || C > SW_MAX_C) return -3;
-  *tpr = ((C + 7) / 8 + 31) / 32 * 32;
-  *groups = *tpr >= 256 ? 1 : 256 / *tpr;
+// Threads a row, rows a block and blocks of a pass. An SM holds 512 threads of 128 registers (backward, and rows that are read
+// channel by channel), in one block where that can be: fewer partial sums, tables and prologues. Forward 768 of 80: two blocks of 384
+// (55 424 x 1024 with a gate of tokens, forward and backward: 282 us with 512 a multiprocessor forward, 263 with 768). Few rows
+// are spread over all multiprocessors.
+static int sw_shape(SandwichArgs& a, bool backward, int mode, unsigned* blocks) {
+  if (a.C < 1 || a.C > SW_MAX_C) return -3;
+  a.tpr = ((a.C + 7) / 8 + 31) / 32 * 32;
+  const bool wide = !backward && mode != STRIDED;
+  const int most = wide ? 384 : 512;
+  a.groups = a.tpr > most ? 1 : most / a.tpr;
+  const long long spread = (a.T + 147) / 148;
+  if (a.groups > spread) a.groups = static_cast<int>(spread < 1 ? 1 : spread);
+  int per_sm = (wide ? 768 : 512) / (a.tpr * a.groups);
+  if (per_sm < 1) per_sm = 1;
+  const long long all = (a.T + a.groups - 1) / a.groups, room = 148LL * per_sm;
+  *blocks = static_cast<unsigned>(all < room ? all : room);
   return 0;
 }
 
-static size_t sw_smem_bytes(const SandwichArgs& a, int parts, int size, bool aligned) {
-  return static_cast<size_t>(a.tpr) * 8 * 4 * 4 + static_cast<size_t>(a.groups) * 32 * 8 +
-         (aligned ? static_cast<size_t>(a.groups) * SW_STAGES * parts * a.C * size : 0);
+static size_t sw_smem_bytes(const SandwichArgs& a, int rows, int parts, int size, bool ring) {
+  return static_cast<size_t>(a.tpr) * 8 * 4 * 4 + static_cast<size_t>(a.groups) * 64 * 4 +
+         (ring ? static_cast<size_t>(a.groups) * a.stages * rows * parts * a.C * size : 0);
 }
 
-template <typename T, bool ALIGNED>
+template <typename T, int MODE, int GATE>
 static int sw_launch(const SandwichArgs& a, bool backward, unsigned blocks, size_t smem, cudaStream_t st) {
-  auto kern = backward ? sandwich_bwd_kernel<T, ALIGNED> : sandwich_fwd_kernel<T, ALIGNED>;
+  auto kern = backward ? sandwich_bwd_kernel<T, MODE, GATE> : sandwich_fwd_kernel<T, MODE, GATE>;
   static bool configured_on[2][MAX_DEVICES];
   const int dev = current_device_slot();
   if (dev < 0) return -4;
   if (!configured_on[backward][dev]) {
-    NPLM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    NPLM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(SW_MAX_SMEM)));
     configured_on[backward][dev] = true;
   }
   const cudaError_t e = launch_when(a.T * a.C <= CHAIN_ELEMENTS, kern, blocks, a.tpr * a.groups, smem, st, a);
@@ -533,29 +696,41 @@ static int sw_launch(const SandwichArgs& a, bool backward, unsigned blocks, size
   return static_cast<int>(cudaGetLastError());
 }
 
-static int sw_run(const SandwichArgs& a, bool backward, int dtype, unsigned blocks, cudaStream_t st) {
+template <typename T>
+static int sw_launch(const SandwichArgs& a, bool backward, int mode, unsigned blocks, size_t smem, cudaStream_t st) {
+  if (mode == STRIDED) return sw_launch<T, STRIDED, GATE_ANY>(a, backward, blocks, smem, st);
+  if (mode == ALIGNED) return sw_launch<T, ALIGNED, GATE_ANY>(a, backward, blocks, smem, st);
+  if (a.gate_mode == GATE_SIGMOID) return sw_launch<T, FULL, GATE_SIGMOID>(a, backward, blocks, smem, st);
+  if (a.gate_mode == GATE_TOKEN) return sw_launch<T, FULL, GATE_TOKEN>(a, backward, blocks, smem, st);
+  return sw_launch<T, FULL, GATE_NONE>(a, backward, blocks, smem, st);
+}
+
+static int sw_run(SandwichArgs& a, bool backward, int dtype, unsigned* blocks, cudaStream_t st) {
   const int size = dtype == 2 ? 4 : 2;
   const void* rows[] = {a.x, a.f, a.gate_mode >= GATE_TOKEN ? a.gate : nullptr, a.dy, a.dh, a.y, a.h, a.dx, a.df, a.dg};
   const long long strides[] = {a.xs, a.fs, a.gate_mode >= GATE_TOKEN ? a.gs : 0, a.dys, a.dhs};
   bool aligned = a.C % 8 == 0;
   for (const void* p : rows) aligned &= reinterpret_cast<uintptr_t>(p) % 16 == 0;
   for (long long s : strides) aligned &= s * size % 16 == 0;
+  const int mode = !aligned ? STRIDED : a.C % 256 == 0 ? FULL : ALIGNED;
+  const int rc = sw_shape(a, backward, mode, blocks);
+  if (rc) return rc;
   const int parts = 2 + (a.gate_mode >= GATE_TOKEN) + (a.dy != nullptr) + (a.dh != nullptr);
-  const size_t smem = sw_smem_bytes(a, parts, size, aligned);
-  if (dtype == 0) return aligned ? sw_launch<__nv_bfloat16, true>(a, backward, blocks, smem, st)
-                                 : sw_launch<__nv_bfloat16, false>(a, backward, blocks, smem, st);
-  if (dtype == 1) return aligned ? sw_launch<__half, true>(a, backward, blocks, smem, st)
-                                 : sw_launch<__half, false>(a, backward, blocks, smem, st);
-  return aligned ? sw_launch<float, true>(a, backward, blocks, smem, st) : sw_launch<float, false>(a, backward, blocks, smem, st);
-}
-
-// Blocks of a pass: all rows at once where they fit, else as many blocks as the multiprocessors hold.
-static unsigned sw_blocks(const SandwichArgs& a, int threads_an_sm) {
-  const long long all = (a.T + a.groups - 1) / a.groups;
-  int per_sm = threads_an_sm / (a.tpr * a.groups);
-  if (per_sm < 1) per_sm = 1;
-  const long long most = 148LL * per_sm;
-  return static_cast<unsigned>(all < most ? all : most);
+  const bool ring = aligned || size == 4;
+  a.stages = SW_STAGES;
+  size_t smem = sw_smem_bytes(a, backward ? 1 : 2, parts, size, ring);
+  if (smem > SW_MAX_SMEM) {      // (fp32 rows of more than 3 500 channels with a gate)
+    a.stages = 1;
+    smem = sw_smem_bytes(a, backward ? 1 : 2, parts, size, ring);
+  }
+  if (smem > SW_MAX_SMEM) return -3;
+  if (!backward) {      // (no more blocks than shared memory holds at a time; 1 KB of it is the system's)
+    const unsigned room = 148 * static_cast<unsigned>((SW_MAX_SMEM + 1024) / (smem + 1024));
+    if (*blocks > room) *blocks = room;
+  }
+  if (dtype == 0) return sw_launch<__nv_bfloat16>(a, backward, mode, *blocks, smem, st);
+  if (dtype == 1) return sw_launch<__half>(a, backward, mode, *blocks, smem, st);
+  return sw_launch<float>(a, backward, mode, *blocks, smem, st);
 }
 
 }  // namespace nplm
@@ -567,12 +742,13 @@ extern "C" int nplm_sandwich_bwd_blocks(long long T, int C) {
   SandwichArgs a = {};
   a.T = T;
   a.C = C;
-  const int rc = sw_shape(C, &a.tpr, &a.groups);
-  return rc ? rc : static_cast<int>(sw_blocks(a, 512));
+  unsigned blocks = 0;
+  const int rc = sw_shape(a, true, FULL, &blocks);
+  return rc ? rc : static_cast<int>(blocks);
 }
 
 // dtype: 0 bf16, 1 fp16, 2 fp32. gate_mode: 0 none, 1 [C], 2 rows, 3 rows through a sigmoid. strides: rows of x, f, gate.
-// stats: fp32 [4][T] for the backward pass, or null. h null: no norm follows.
+// stats: fp32 [T][4] for the backward pass, or null. h null: no norm follows.
 extern "C" int nplm_sandwich_fwd(const void* x, const void* f, const void* gate, const void* post, const void* next,
                                  const void* scale, const long long* strides, void* y, void* h, float* stats, long long T,
                                  int C, float eps, int rms, int gate_mode, int dtype, int param32, cudaStream_t st) {
@@ -581,9 +757,9 @@ extern "C" int nplm_sandwich_fwd(const void* x, const void* f, const void* gate,
   SandwichArgs a = {};
   a.x = x; a.f = f; a.gate = gate; a.post = post; a.next = next; a.scale = scale;
   a.xs = strides[0]; a.fs = strides[1]; a.gs = strides[2];
-  a.y = y; a.h = h; a.stats = stats; a.T = T; a.C = C; a.eps = eps; a.rms = rms; a.gate_mode = gate_mode; a.param32 = param32;
-  const int rc = sw_shape(C, &a.tpr, &a.groups);
-  return rc ? rc : sw_run(a, false, dtype, sw_blocks(a, 1024), st);
+  a.y = y; a.h = h; a.stats = reinterpret_cast<float4*>(stats); a.T = T; a.C = C; a.eps = eps; a.rms = rms; a.gate_mode = gate_mode; a.param32 = param32;
+  unsigned blocks;
+  return sw_run(a, false, dtype, &blocks, st);
 }
 
 // dy or dh may be null. strides: rows of x, f, gate, dy, dh. partial: fp32 [4][blocks][C] scratch. sums / kinds: where the column
@@ -605,18 +781,15 @@ extern "C" int nplm_sandwich_bwd(const void* dy, const void* dh, const void* x, 
   }
   a.x = x; a.f = f; a.gate = gate; a.post = post; a.next = next; a.scale = scale; a.dy = dy; a.dh = dh;
   a.xs = strides[0]; a.fs = strides[1]; a.gs = strides[2]; a.dys = strides[3]; a.dhs = strides[4];
-  a.stats = const_cast<float*>(stats); a.dx = dx; a.df = df; a.dg = dg; a.partial = partial;
+  a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats)); a.dx = dx; a.df = df; a.dg = dg; a.partial = partial;
   a.T = T; a.C = C; a.rms = rms; a.gate_mode = gate_mode; a.param32 = param32;
-  int rc = sw_shape(C, &a.tpr, &a.groups);
-  if (rc) return rc;
   unsigned blocks = 0;      // (no rows: the column sums are zero)
   if (T > 0) {
-    blocks = sw_blocks(a, 512);
-    rc = sw_run(a, true, dtype, blocks, st);
+    const int rc = sw_run(a, true, dtype, &blocks, st);
     if (rc) return rc;
   }
   if (a.want) {
-    const cudaError_t e = launch_chained(sandwich_columns_kernel, dim3((C + 31) / 32, 4), dim3(32, 16), 0, st,
+    const cudaError_t e = launch_chained(sandwich_columns_kernel, dim3((C + 31) / 32, 4), dim3(32, 32), 0, st,
                                          static_cast<const float*>(partial), to, static_cast<int>(blocks), C);
     if (e != cudaSuccess) return static_cast<int>(e);
   }

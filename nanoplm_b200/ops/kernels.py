@@ -388,14 +388,14 @@ def sandwich_fwd(x, f, post, nxt, gate=None, scale=None, eps: float = 1e-5, rms:
                  with_next: bool = True, stats: bool = True):
     """y = scale x + g norm(f) post, h = norm(y) nxt for rows of up to 4 096 channels: (y, h, stats), h None without
     `with_next`. gate: None, [C], or like x (with `sigmoid` through one). post, nxt, scale: [C] or None, all of x's type
-    or all fp32. stats: fp32 [4, T] for `sandwich_bwd`."""
+    or all fp32. stats: fp32 [T, 4] for `sandwich_bwd`."""
     mode, param32 = check_sandwich(x, f, gate, post, nxt, scale, sigmoid)
     _sandwich_rows(x, f, gate)
     (T, C), kind = x.shape, ROW_TYPES[x.dtype]
     with _device_of(x, f, gate, post, nxt, scale):
         y = torch.empty((T, C), dtype=x.dtype, device=x.device)
         h = torch.empty_like(y) if with_next else None
-        st = torch.empty((4, T), dtype=torch.float32, device=x.device) if stats else None
+        st = torch.empty((T, 4), dtype=torch.float32, device=x.device) if stats else None
         if T:
             strides = (c_longlong * 3)(x.stride(0), f.stride(0), gate.stride(0) if mode >= GATE_TOKEN else 0)
             rc = typed("sandwich_norm", "nplm_sandwich_fwd", "pppppppppplifiiiip")(
@@ -422,8 +422,8 @@ def sandwich_bwd(dy, dh, x, f, stats, post, nxt, gate=None, scale=None, rms: boo
     for name, d in (("dy", dy), ("dh", dh)):
         if d is not None and (d.shape != x.shape or d.dtype != x.dtype):
             raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}, got {tuple(d.shape)} {d.dtype}")
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (4, T) or not stats.is_contiguous():
-        raise ValueError(f"stats must be the fp32 [4, {T}] of the forward pass")
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (T, 4) or not stats.is_contiguous():
+        raise ValueError(f"stats must be the fp32 [{T}, 4] of the forward pass")
     with _device_of(x, f, gate, post, nxt, scale, dy, dh, stats, *sums):
         dx, df = torch.empty((T, C), dtype=x.dtype, device=x.device), torch.empty((T, C), dtype=x.dtype, device=x.device)
         dg = torch.empty((T, C), dtype=x.dtype, device=x.device) if mode >= GATE_TOKEN else None
