@@ -245,27 +245,43 @@ static cudaError_t launch_rotary(const RotaryArgs& a, int ve, int interleaved, u
 
 using namespace nplm;
 
-// dtype: 0 bf16, 1 fp16, 2 fp32. strides: batch, token and head of q, then of its output, then the same of k. k may be null
-// (k_heads 0). pos: int32 or int64 (pos64), strides pb, pt. D at most 512.
-extern "C" int nplm_rotary_qk(const void* q, void* q_out, const void* k, void* k_out, const long long* strides, int q_heads,
-                              int k_heads, const void* pos, int pos64, long long pb, long long pt, const double* freq,
-                              float factor, int transposed, long long batch, long long seq, int D, int R, int dtype,
-                              int interleaved, cudaStream_t st) {
+// The arguments of a call, packed by the caller (ops/kernels.py has the same layout): one conversion on its side, not 20.
+// strides: batch, token and head of q, then of its output, then the same of k. k may be null (k_heads 0). pos: int32 or int64
+// (pos64), strides pb, pt. D at most 512. dtype: 0 bf16, 1 fp16, 2 fp32.
+struct RotaryCall {
+  const void* q;
+  void* q_out;
+  const void* k;
+  void* k_out;
+  long long strides[12];
+  const void* pos;
+  long long pb, pt;
+  const double* freq;
+  long long batch, seq;
+  int q_heads, k_heads, pos64, transposed, D, R, dtype, interleaved;
+  float factor;
+};
+
+extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
+  const RotaryCall& c = *call;
+  const int q_heads = c.q_heads, k_heads = c.k_heads, D = c.D, R = c.R, dtype = c.dtype;
+  const long long batch = c.batch, seq = c.seq;
   if (batch < 0 || seq < 0 || q_heads < 1 || k_heads < 0 || D < 2 || D > 512 || R < 2 || R > D || R % 2 || dtype < 0 ||
       dtype > 2)
     return -1;
   if (batch == 0 || seq == 0) return 0;
   RotaryArgs a;
-  a.x[0] = q; a.x[1] = k; a.y[0] = q_out; a.y[1] = k_out;
+  a.x[0] = c.q; a.x[1] = c.k; a.y[0] = c.q_out; a.y[1] = c.k_out;
   a.heads[0] = q_heads; a.heads[1] = k_heads;
   for (int j = 0; j < 2; ++j) {
-    a.xb[j] = strides[6 * j]; a.xt[j] = strides[6 * j + 1]; a.xh[j] = strides[6 * j + 2];
-    a.yb[j] = strides[6 * j + 3]; a.yt[j] = strides[6 * j + 4]; a.yh[j] = strides[6 * j + 5];
+    const long long* strides = c.strides + 6 * j;
+    a.xb[j] = strides[0]; a.xt[j] = strides[1]; a.xh[j] = strides[2];
+    a.yb[j] = strides[3]; a.yt[j] = strides[4]; a.yh[j] = strides[5];
   }
-  a.pos = pos; a.pos64 = pos64; a.pb = pb; a.pt = pt; a.freq = freq; a.factor = factor;
-  a.sign = transposed ? -1.f : 1.f;
+  a.pos = c.pos; a.pos64 = c.pos64; a.pb = c.pb; a.pt = c.pt; a.freq = c.freq; a.factor = c.factor;
+  a.sign = c.transposed ? -1.f : 1.f;
   a.tokens = batch * seq; a.seq = seq; a.D = D; a.R = R;
-  a.in_place = q == q_out && (k_heads == 0 || k == k_out);
+  a.in_place = c.q == c.q_out && (k_heads == 0 || c.k == c.k_out);
   // the widest access, up to 16 bytes, that sizes, strides and addresses allow
   const int size = dtype == 2 ? 4 : 2;
   int ve = 16 / size;
@@ -291,9 +307,9 @@ extern "C" int nplm_rotary_qk(const void* q, void* q_out, const void* k, void* k
   if (blocks > 0x7fffffffLL) return -2;
   const unsigned n = static_cast<unsigned>(blocks);
   cudaError_t e;
-  if (dtype == 0) e = launch_rotary<__nv_bfloat16>(a, ve, interleaved, n, st);
-  else if (dtype == 1) e = launch_rotary<__half>(a, ve, interleaved, n, st);
-  else e = launch_rotary<float>(a, ve, interleaved, n, st);
+  if (dtype == 0) e = launch_rotary<__nv_bfloat16>(a, ve, c.interleaved, n, st);
+  else if (dtype == 1) e = launch_rotary<__half>(a, ve, c.interleaved, n, st);
+  else e = launch_rotary<float>(a, ve, c.interleaved, n, st);
   if (e != cudaSuccess) return static_cast<int>(e);
   return static_cast<int>(cudaGetLastError());
 }

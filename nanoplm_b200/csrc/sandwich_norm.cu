@@ -747,50 +747,62 @@ extern "C" int nplm_sandwich_bwd_blocks(long long T, int C) {
   return rc ? rc : static_cast<int>(blocks);
 }
 
-// dtype: 0 bf16, 1 fp16, 2 fp32. gate_mode: 0 none, 1 [C], 2 rows, 3 rows through a sigmoid. strides: rows of x, f, gate.
-// stats: fp32 [T][4] for the backward pass, or null. h null: no norm follows.
-extern "C" int nplm_sandwich_fwd(const void* x, const void* f, const void* gate, const void* post, const void* next,
-                                 const void* scale, const long long* strides, void* y, void* h, float* stats, long long T,
-                                 int C, float eps, int rms, int gate_mode, int dtype, int param32, cudaStream_t st) {
-  if (T < 0 || dtype < 0 || dtype > 2 || gate_mode < 0 || gate_mode > 3 || (gate_mode != 0) != (gate != nullptr)) return -1;
-  if (T == 0) return 0;
-  SandwichArgs a = {};
-  a.x = x; a.f = f; a.gate = gate; a.post = post; a.next = next; a.scale = scale;
-  a.xs = strides[0]; a.fs = strides[1]; a.gs = strides[2];
-  a.y = y; a.h = h; a.stats = reinterpret_cast<float4*>(stats); a.T = T; a.C = C; a.eps = eps; a.rms = rms; a.gate_mode = gate_mode; a.param32 = param32;
-  unsigned blocks;
-  return sw_run(a, false, dtype, &blocks, st);
-}
+// The arguments of a call, packed by the caller (ops/kernels.py has the same layout): one conversion on its side, not 30.
+// dtype: 0 bf16, 1 fp16, 2 fp32. gate_mode: 0 none, 1 [C], 2 rows, 3 rows through a sigmoid. strides: rows of x, f, gate, dy, dh.
+// stats: fp32 [T][4] for the backward pass, or null. Forward: y, h (null: no norm follows). Backward: dy or dh may be
+// null; dx, df, dg; partial: fp32 [4][blocks][C] scratch; sums, kinds: where the column sums of w_next, w_post, the scale and a [C]
+// gate go, and as what (see ColumnSums).
+struct SandwichCall {
+  const void *x, *f, *gate, *post, *next, *scale, *dy, *dh;
+  void *y, *h, *dx, *df, *dg;
+  float *stats, *partial;
+  void* sums[4];
+  long long strides[5], T;
+  int kinds[4], C, rms, gate_mode, dtype, param32;
+  float eps;
+};
 
-// dy or dh may be null. strides: rows of x, f, gate, dy, dh. partial: fp32 [4][blocks][C] scratch. sums / kinds: where the column
-// sums of w_next, w_post, the scale and a [C] gate go, and as what (see ColumnSums).
-extern "C" int nplm_sandwich_bwd(const void* dy, const void* dh, const void* x, const void* f, const void* gate,
-                                 const void* post, const void* next, const void* scale, const float* stats,
-                                 const long long* strides, void* dx, void* df, void* dg, float* partial, void* const* sums,
-                                 const int* kinds, long long T, int C, int rms, int gate_mode, int dtype, int param32,
-                                 cudaStream_t st) {
-  if (T < 0 || dtype < 0 || dtype > 2 || gate_mode < 0 || gate_mode > 3 ||
-      (T > 0 && ((gate_mode != 0) != (gate != nullptr) || (dy == nullptr && dh == nullptr))))
+static int sw_args(const SandwichCall& c, SandwichArgs* out) {
+  if (c.T < 0 || c.dtype < 0 || c.dtype > 2 || c.gate_mode < 0 || c.gate_mode > 3 ||
+      (c.T > 0 && (c.gate_mode != 0) != (c.gate != nullptr)))
     return -1;
   SandwichArgs a = {};
+  a.x = c.x; a.f = c.f; a.gate = c.gate; a.post = c.post; a.next = c.next; a.scale = c.scale; a.dy = c.dy; a.dh = c.dh;
+  a.xs = c.strides[0]; a.fs = c.strides[1]; a.gs = c.strides[2]; a.dys = c.strides[3]; a.dhs = c.strides[4];
+  a.y = c.y; a.h = c.h; a.dx = c.dx; a.df = c.df; a.dg = c.dg;
+  a.stats = reinterpret_cast<float4*>(c.stats); a.partial = c.partial;
+  a.T = c.T; a.C = c.C; a.eps = c.eps; a.rms = c.rms; a.gate_mode = c.gate_mode; a.param32 = c.param32;
+  *out = a;
+  return 0;
+}
+
+extern "C" int nplm_sandwich_fwd(const SandwichCall* call, cudaStream_t st) {
+  SandwichArgs a;
+  const int rc = sw_args(*call, &a);
+  if (rc || a.T == 0) return rc;
+  unsigned blocks;
+  return sw_run(a, false, call->dtype, &blocks, st);
+}
+
+extern "C" int nplm_sandwich_bwd(const SandwichCall* call, cudaStream_t st) {
+  SandwichArgs a;
+  const int rc = sw_args(*call, &a);
+  if (rc) return rc;
+  if (a.T > 0 && a.dy == nullptr && a.dh == nullptr) return -1;
   ColumnSums to;
   for (int k = 0; k < 4; ++k) {
-    to.out[k] = sums[k];
-    to.kind[k] = kinds[k];
-    if (kinds[k]) a.want |= 1 << k;
+    to.out[k] = call->sums[k];
+    to.kind[k] = call->kinds[k];
+    if (to.kind[k]) a.want |= 1 << k;
   }
-  a.x = x; a.f = f; a.gate = gate; a.post = post; a.next = next; a.scale = scale; a.dy = dy; a.dh = dh;
-  a.xs = strides[0]; a.fs = strides[1]; a.gs = strides[2]; a.dys = strides[3]; a.dhs = strides[4];
-  a.stats = reinterpret_cast<float4*>(const_cast<float*>(stats)); a.dx = dx; a.df = df; a.dg = dg; a.partial = partial;
-  a.T = T; a.C = C; a.rms = rms; a.gate_mode = gate_mode; a.param32 = param32;
   unsigned blocks = 0;      // (no rows: the column sums are zero)
-  if (T > 0) {
-    const int rc = sw_run(a, true, dtype, &blocks, st);
-    if (rc) return rc;
+  if (a.T > 0) {
+    const int rc2 = sw_run(a, true, call->dtype, &blocks, st);
+    if (rc2) return rc2;
   }
   if (a.want) {
-    const cudaError_t e = launch_chained(sandwich_columns_kernel, dim3((C + 31) / 32, 4), dim3(32, 32), 0, st,
-                                         static_cast<const float*>(partial), to, static_cast<int>(blocks), C);
+    const cudaError_t e = launch_chained(sandwich_columns_kernel, dim3((a.C + 31) / 32, 4), dim3(32, 32), 0, st,
+                                         static_cast<const float*>(a.partial), to, static_cast<int>(blocks), a.C);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   return static_cast<int>(cudaGetLastError());

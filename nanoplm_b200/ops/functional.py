@@ -401,7 +401,8 @@ class _SandwichFn(torch.autograd.Function):
                                      stats=any(ctx.needs_input_grad))
         ctx.save_for_backward(x, f, post, nxt, gate, scale, stats)
         ctx.how = (rms, sigmoid)
-        ctx.refs = (nxt, post, scale, gate)     # (saved-tensor hooks may give back copies, without the running gradients)
+        # (saved-tensor hooks may give back copies, without the running gradients)
+        ctx.refs = (nxt, post, scale, gate if gate is not None and gate.dim() == 1 else None)
         return y, h
 
     @staticmethod
@@ -413,12 +414,12 @@ class _SandwichFn(torch.autograd.Function):
         rms, sigmoid = ctx.how
         rows = lambda t: t if t is None or t.stride(1) == 1 else t.contiguous()
         need = ctx.needs_input_grad
-        wanted = (need[3] and dh is not None, need[2], need[5], need[4] and gate is not None and gate.dim() == 1)
+        wanted = (need[3] and dh is not None, need[2], need[5], need[4] and ctx.refs[3] is not None)
         sums, add = [], []
         for p, want in zip(ctx.refs, wanted):
             running = want and _has_main_grad(p) and p.main_grad.dtype == torch.float32 and p.main_grad.is_contiguous()
             add.append(running)
-            sums.append(None if not want else p.main_grad if running else torch.empty_like(p, memory_format=torch.contiguous_format))
+            sums.append(None if not want else p.main_grad if running else torch.empty(p.shape, dtype=p.dtype, device=p.device))
         dx, df, dg = K.sandwich_bwd(rows(dy), rows(dh), x, f, stats, post, nxt, gate, scale, rms, sigmoid, sums, add)
         dnext, dpost, dscale, dgate = (None if a else s for s, a in zip(sums, add))
         if dg is not None:
@@ -437,9 +438,9 @@ def sandwich_norm(x, f, post=None, next=None, *, gate=None, sigmoid: bool = Fals
     sigmoid is taken with `sigmoid`. Norms are LayerNorm without bias, or RMSNorm."""
     if sigmoid and (gate is None or gate.dim() != 2):
         raise ValueError("sigmoid is for gates of tokens [T, C]")
-    K.check_sandwich(x, f, gate, post, next, scale, sigmoid)
-    if x.is_cuda and x.dtype in K.ROW_TYPES and x.shape[1] <= K.SANDWICH_MAX_C:
+    if x.is_cuda and x.dtype in K.ROW_TYPES and x.dim() == 2 and x.shape[1] <= K.SANDWICH_MAX_C:      # (checked there)
         return _call(_SandwichFn, x, f, post, next, gate, scale, eps, rms, sigmoid, with_next)
+    K.check_sandwich(x, f, gate, post, next, scale, sigmoid)
     n = norm(f.float(), post, eps, rms)
     if gate is not None:
         n = n * (torch.sigmoid(gate.float()) if sigmoid else gate.float())
@@ -566,8 +567,9 @@ class _RotaryFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, frequencies)
         ctx.how = (factor, interleaved, transposed)
-        unit = lambda t: t if t is None or t.stride(-1) == 1 else t.contiguous()
-        return K.rotary(unit(q), unit(k), positions, frequencies, factor, interleaved, transposed)
+        q = q if q.stride(-1) == 1 else q.contiguous()
+        k = k if k is None or k.stride(-1) == 1 else k.contiguous()
+        return K.rotary(q, k, positions, frequencies, factor, interleaved, transposed)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -587,10 +589,10 @@ def rotary(q, k=None, *, positions, frequencies, factor: float = 1.0, interleave
     (q', k'), or q' alone without k. positions: integers [T], [B, S] or [S]; frequencies (fp64) and factor from
     `rotary_frequencies`: their 2 n first channels rotate, as pairs (i, i + n) or, interleaved, (2 i, 2 i + 1). Angles are
     exact to fp32 for every 32-bit position: there is no table that ends."""
-    K.check_rotary(q, k, positions, frequencies)
-    if q.is_cuda and q.dtype in K.ROW_TYPES and q.shape[-1] <= K.ROTARY_MAX_WIDTH:
+    if q.is_cuda and q.dtype in K.ROW_TYPES and q.shape[-1] <= K.ROTARY_MAX_WIDTH:      # (checked there)
         out = _call(_RotaryFn, q, k, positions, frequencies, factor, interleaved, False)
         return out[0] if k is None else out
+    K.check_rotary(q, k, positions, frequencies)
     out = _rotate_plain(q, positions, frequencies, factor, interleaved)
     return out if k is None else (out, _rotate_plain(k, positions, frequencies, factor, interleaved))
 

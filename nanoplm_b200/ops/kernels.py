@@ -6,8 +6,9 @@ stream and returns output tensors. ``nanoplm_b200.ops.functional`` builds differ
 from __future__ import annotations
 
 from contextlib import nullcontext
-from ctypes import c_float, c_int, c_longlong, c_ubyte, c_void_p
+from ctypes import c_float, c_int, c_longlong
 from functools import lru_cache
+from struct import Struct
 
 import torch
 
@@ -34,6 +35,11 @@ def _dp(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def _address(t: torch.Tensor | None) -> int:
+    """Device address for a packed call; 0 for None."""
+    return 0 if t is None else t.data_ptr()
+
+
 def _is_tracing() -> bool:
     return torch._C._is_tracing()
 
@@ -46,10 +52,11 @@ def _device_of(first: torch.Tensor, *rest):
     """A context in which the first tensor's device is the current one; ValueError where another tensor is elsewhere."""
     if not first.is_cuda:
         raise ValueError("the tensors must be on a CUDA device")
+    index = first.get_device()
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
-    return _NULL if first.device.index == torch._C._cuda_getDevice() else torch.cuda.device(first.device)
+    return _NULL if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _rowmajor(t: torch.Tensor, name: str) -> int:
@@ -345,6 +352,7 @@ def norm_bwd(dy, x, w, mean, rstd, *, rms=False, dres=None, dw=None, ids=None, d
 
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_SIGMOID = 0, 1, 2, 3
 SANDWICH_MAX_C = 4096
+_SANDWICH = Struct("=15q4q6q9if")       # SandwichCall of csrc/sandwich_norm.cu
 
 
 def check_sandwich(x, f, gate, post, nxt, scale, sigmoid) -> tuple[int, bool]:
@@ -391,17 +399,17 @@ def sandwich_fwd(x, f, post, nxt, gate=None, scale=None, eps: float = 1e-5, rms:
     or all fp32. stats: fp32 [T, 4] for `sandwich_bwd`."""
     mode, param32 = check_sandwich(x, f, gate, post, nxt, scale, sigmoid)
     _sandwich_rows(x, f, gate)
-    (T, C), kind = x.shape, ROW_TYPES[x.dtype]
+    T, C = x.shape
     with _device_of(x, f, gate, post, nxt, scale):
         y = torch.empty((T, C), dtype=x.dtype, device=x.device)
-        h = torch.empty_like(y) if with_next else None
+        h = torch.empty((T, C), dtype=x.dtype, device=x.device) if with_next else None
         st = torch.empty((T, 4), dtype=torch.float32, device=x.device) if stats else None
         if T:
-            strides = (c_longlong * 3)(x.stride(0), f.stride(0), gate.stride(0) if mode >= GATE_TOKEN else 0)
-            rc = typed("sandwich_norm", "nplm_sandwich_fwd", "pppppppppplifiiiip")(
-                x.data_ptr(), f.data_ptr(), _dp(gate), _dp(post), _dp(nxt), _dp(scale), strides, y.data_ptr(), _dp(h), _dp(st),
-                T, C, eps, rms, mode, kind, param32, raw_stream())
-            check_rc(rc, "sandwich_fwd")
+            call = _SANDWICH.pack(x.data_ptr(), f.data_ptr(), _address(gate), _address(post), _address(nxt), _address(scale), 0, 0,
+                                  y.data_ptr(), _address(h), 0, 0, 0, _address(st), 0, 0, 0, 0, 0, x.stride(0), f.stride(0),
+                                  gate.stride(0) if mode >= GATE_TOKEN else 0, 0, 0, T, 0, 0, 0, 0, C, rms, mode,
+                                  ROW_TYPES[x.dtype], param32, eps)
+            check_rc(typed("sandwich_norm", "nplm_sandwich_fwd", "pp")(call, raw_stream()), "sandwich_fwd")
             count_launch()
     return y, h, st
 
@@ -434,15 +442,16 @@ def sandwich_bwd(dy, dh, x, f, stats, post, nxt, gate=None, scale=None, rms: boo
                 raise ValueError(f"sums must be contiguous [{C}] tensors, fp32 where added to")
             kinds.append(0 if s is None else 4 if a else _SUM_KINDS[s.dtype])
         partial = None
-        if any(kinds):
-            blocks = typed("sandwich_norm", "nplm_sandwich_bwd_blocks", "li")(T, C) if T else 0
+        if any(kinds) and T:
+            blocks = typed("sandwich_norm", "nplm_sandwich_bwd_blocks", "li")(T, C)
             partial = torch.empty((4, blocks, C), dtype=torch.float32, device=x.device)
         rs = lambda t: 0 if t is None else t.stride(0)
-        strides = (c_longlong * 5)(x.stride(0), f.stride(0), gate.stride(0) if mode >= GATE_TOKEN else 0, rs(dy), rs(dh))
-        rc = typed("sandwich_norm", "nplm_sandwich_bwd", "pppppppppp" + "pppppp" + "liiiiip")(
-            _dp(dy), _dp(dh), x.data_ptr(), f.data_ptr(), _dp(gate), _dp(post), _dp(nxt), _dp(scale), _dp(stats), strides,
-            dx.data_ptr(), df.data_ptr(), _dp(dg), _dp(partial), (c_void_p * 4)(*[_dp(s) for s in sums]),
-            (c_int * 4)(*kinds), T, C, rms, mode, kind, param32, raw_stream())
+        call = _SANDWICH.pack(x.data_ptr(), f.data_ptr(), _address(gate), _address(post), _address(nxt), _address(scale),
+                              _address(dy), _address(dh), 0, 0, dx.data_ptr(), df.data_ptr(), _address(dg), stats.data_ptr(),
+                              _address(partial), *map(_address, sums), x.stride(0), f.stride(0),
+                              gate.stride(0) if mode >= GATE_TOKEN else 0, rs(dy), rs(dh), T, *kinds, C, rms, mode, kind, param32,
+                              0.0)
+        rc = typed("sandwich_norm", "nplm_sandwich_bwd", "pp")(call, raw_stream())
         check_rc(rc, "sandwich_bwd")
         count_launch((T > 0) + any(kinds))
     return dx, df, dg
@@ -463,43 +472,43 @@ def rope_(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Te
 
 
 ROTARY_MAX_WIDTH = 512
-
-
-def _heads_last(t: torch.Tensor, name: str):
-    """(batch, tokens, heads, width) and the strides of the first three of a [T, H, D] or [B, S, H, D] tensor."""
-    if t.dim() == 3:
-        return (1, *t.shape), (0, t.stride(0), t.stride(1))
-    if t.dim() == 4:
-        return tuple(t.shape), t.stride()[:3]
-    raise ValueError(f"{name} must be [tokens, heads, width] or [batch, tokens, heads, width], got {tuple(t.shape)}")
+_ROTARY = Struct("=4q12q3q3q8if4x")       # RotaryCall of csrc/rotary.cu
 
 
 def check_rotary(q, k, positions, frequencies):
-    """Checks the arguments of a rotation: (sizes of q, its strides, heads of k, its strides, strides of the positions, number
-    of channels that rotate)."""
-    (B, S, H, D), qs = _heads_last(q, "q")
+    """Checks the arguments of a rotation: (batch, tokens, heads, width, heads of k, number of channels that rotate), strides of the
+    batch, tokens and heads of q, of k, and of the batch and tokens of the positions."""
+    shape, st = q.shape, q.stride()
+    if len(shape) == 3:
+        (S, H, D), B, qs = shape, 1, (0, st[0], st[1])
+    elif len(shape) == 4:
+        (B, S, H, D), qs = shape, st[:3]
+    else:
+        raise ValueError(f"q must be [tokens, heads, width] or [batch, tokens, heads, width], got {tuple(shape)}")
     Hk, ks = 0, (0, 0, 0)
     if k is not None:
-        (Bk, Sk, Hk, Dk), ks = _heads_last(k, "k")
-        if k.dim() != q.dim() or (Bk, Sk, Dk) != (B, S, D):
-            raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in tokens or width")
+        kshape, kst = k.shape, k.stride()
+        if len(kshape) != len(shape) or kshape[:-2] != shape[:-2] or kshape[-1] != D:
+            raise ValueError(f"q {tuple(shape)} and k {tuple(kshape)} differ in tokens or width")
         if k.dtype != q.dtype:
             raise ValueError(f"k must be {q.dtype}, got {k.dtype}")
+        Hk, ks = kshape[-2], (0, kst[0], kst[1]) if len(shape) == 3 else kst[:3]
     if H < 1 or (k is not None and Hk < 1):
         raise ValueError(f"at least one head is needed: got {H} and {Hk}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-    if positions.dim() == 1 and positions.shape[0] == S:
+    pshape = positions.shape
+    if len(pshape) == 1 and pshape[0] == S:
         ps = (0, positions.stride(0))
-    elif q.dim() == 4 and tuple(positions.shape) == (B, S):
+    elif len(shape) == 4 and pshape == shape[:2]:
         ps = positions.stride()
     else:
-        raise ValueError(f"positions {tuple(positions.shape)} do not fit q {tuple(q.shape)}")
+        raise ValueError(f"positions {tuple(pshape)} do not fit q {tuple(shape)}")
     R = 2 * frequencies.numel()
     if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not 2 <= R <= D or not frequencies.is_contiguous():
         raise ValueError(f"frequencies must be a contiguous fp64 vector of 1 to {D // 2} pairs, got "
                          f"{tuple(frequencies.shape)} {frequencies.dtype}")
-    return (B, S, H, D), qs, Hk, ks, ps, R
+    return (B, S, H, D, Hk, R), qs, ks, ps
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, factor: float = 1.0,
@@ -511,8 +520,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     for all of a batch. frequencies: fp64 [R / 2], radians a position for each pair of the first R channels of a head; the
     others pass. Pairs are (i, i + R / 2), or (2 i, 2 i + 1) with `interleaved`. factor multiplies cos and sin. transposed:
     the gradient's rotation, backwards and with the same factor."""
-    (B, S, H, D), qs, Hk, ks, ps, R = check_rotary(q, k, positions, frequencies)
-    if q.dtype not in ROW_TYPES or D > ROTARY_MAX_WIDTH:
+    (B, S, H, D, Hk, R), qs, ks, ps = check_rotary(q, k, positions, frequencies)
+    kind = ROW_TYPES.get(q.dtype)
+    if kind is None or D > ROTARY_MAX_WIDTH:
         raise ValueError(f"q must be bf16, fp16 or fp32 with heads of up to {ROTARY_MAX_WIDTH} channels, got {q.dtype}, {D}")
     for t, name in ((q, "q"), (k, "k")):
         if t is not None and t.stride(-1) != 1 and t.numel():
@@ -521,18 +531,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
             raise ValueError(f"{name} is written in place but has elements that share memory")
     with _device_of(q, k, positions, frequencies):
         if inplace:
-            qo, ko = q, k
+            qo, ko, qos, kos = q, k, qs, ks
         else:
-            qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        qos = _heads_last(qo, "q")[1]
-        kos = (0, 0, 0) if ko is None else _heads_last(ko, "k")[1]
+            qo, qos = torch.empty(q.shape, dtype=q.dtype, device=q.device), (S * H * D, H * D, D)
+            ko, kos = (None, (0, 0, 0)) if k is None else (torch.empty(k.shape, dtype=k.dtype, device=k.device), (S * Hk * D, Hk * D, D))
         if B * S:
-            rc = typed("rotary", "nplm_rotary_qk", "pppppiipillpfilliiiip")(
-                q.data_ptr(), qo.data_ptr(), _dp(k), _dp(ko), (c_longlong * 12)(*qs, *qos, *ks, *kos), H, Hk,
-                positions.data_ptr(), positions.dtype == torch.int64, *ps, frequencies.data_ptr(), factor, transposed, B, S,
-                D, R, ROW_TYPES[q.dtype], interleaved, raw_stream())
-            check_rc(rc, "rotary")
+            call = _ROTARY.pack(q.data_ptr(), qo.data_ptr(), _address(k), _address(ko), *qs, *qos, *ks, *kos,
+                                positions.data_ptr(), *ps, frequencies.data_ptr(), B, S, H, Hk,
+                                positions.dtype == torch.int64, transposed, D, R, kind, interleaved, factor)
+            check_rc(typed("rotary", "nplm_rotary_qk", "pp")(call, raw_stream()), "rotary")
             count_launch()
     return qo, ko
 
@@ -750,6 +757,7 @@ def adamw_slots_(p, m, v, g, p_bf16, offsets, numels, decay, max_numel: int, sum
     count_launch()
 
 
+_STEP_TYPES = (torch.float32, torch.bfloat16)
 MOMENT_BLOCK = 256      # elements of a tensor that share the offset of their 8-bit moments
 
 
@@ -776,37 +784,39 @@ def check_moments(m: torch.Tensor, v: torch.Tensor, scales: torch.Tensor | None)
 def check_step(params, grads, copies, decay, m, v, scales, hyper, rng, sumsq) -> tuple[int, int, list[int]]:
     """Checks the arguments of an AdamW step over tensors; (bits, blocks, sizes)."""
     bits, blocks = check_moments(m, v, scales)
-    n = len(params)
+    n, tensor = len(params), torch.Tensor
     if len(grads) != n or (copies is not None and len(copies) != n) or (decay is not None and len(decay) != n):
         raise ValueError("params, grads, copies and decay must be equally long")
-    sizes = [p.numel() for p in params]
-    if sizes != [g.numel() for g in grads] or (copies is not None and sizes != [c.numel() for c in copies]):
+    sizes = list(map(tensor.numel, params))
+    if sizes != list(map(tensor.numel, grads)) or (copies is not None and sizes != list(map(tensor.numel, copies))):
         raise ValueError("params, grads and copies must have the same sizes")
     if moment_blocks(sizes) > blocks:
         raise ValueError(f"the moments hold {blocks} blocks of {MOMENT_BLOCK}, the tensors take {moment_blocks(sizes)}")
-    for name, ts, allowed in (("params", params, (torch.float32, _BF16)), ("grads", grads, (torch.float32, _BF16)),
-                              ("copies", copies, (_BF16,))):
+    home = m.get_device()
+    for name, ts, allowed in (("params", params, _STEP_TYPES), ("grads", grads, _STEP_TYPES), ("copies", copies, (_BF16,))):
         if ts:
             kinds = {t.dtype for t in ts}
-            if len(kinds) != 1 or not kinds <= set(allowed):
+            if len(kinds) != 1 or not kinds.issubset(allowed):
                 raise ValueError(f"{name} must all be one of {allowed}, got {sorted(map(str, kinds))}")
-            if not all([t.is_contiguous() for t in ts]):
+            if not all(map(tensor.is_contiguous, ts)):
                 raise ValueError(f"{name} must be contiguous")
+            if set(map(tensor.get_device, ts)) != {home}:
+                raise ValueError(f"{name} and the moments are on different devices")
     if copies is not None and n and params[0].dtype != torch.float32:
         raise ValueError("bf16 copies are of fp32 params")
-    starts = [p.data_ptr() for p, k in zip(params, sizes) if k]
-    if len(set(starts)) != len(starts):
-        raise ValueError("a tensor is listed twice")
+    if len(set(map(tensor.data_ptr, params))) != n:       # (tensors without elements have none)
+        starts = [p.data_ptr() for p, k in zip(params, sizes) if k]
+        if len(set(starts)) != len(starts):
+            raise ValueError("a tensor is listed twice")
     if hyper.dtype != torch.float32 or hyper.numel() != 9 or not hyper.is_contiguous():
         raise ValueError("hyper must be 9 contiguous fp32 numbers")
     if sumsq is not None and (sumsq.dtype != torch.float32 or sumsq.numel() != 1):
         raise ValueError("sumsq must be one fp32 number")
     if bits == 8 and (rng is None or rng.dtype != torch.int64 or rng.numel() != 1):
         raise ValueError("8-bit moments need rng, one int64 number")
-    devices = {t.device for ts in (params, grads, copies or ()) for t in ts}
-    devices |= {t.device for t in (m, v, scales, hyper, rng, sumsq) if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"tensors on different devices: {sorted(map(str, devices))}")
+    for t in (v, scales, hyper, rng, sumsq):
+        if t is not None and t.get_device() != home:
+            raise ValueError(f"tensors on different devices: {m.device} and {t.device}")
     return bits, blocks, sizes
 
 
@@ -820,9 +830,9 @@ def adamw_tensors_(params, grads, exp_avg, exp_avg_sq, hyper, *, scales=None, rn
     an int64 number that must be another one each step: codes are rounded stochastically.
     hyper: fp32 [9] lr, beta1, beta2, eps, weight decay, bias corrections 1 and 2, gradient scale, largest norm; with sumsq, the
     sum of the gradients' squares, gradients are clipped to the largest norm. hyper, rng and sumsq are read on the
-    device, by a captured step at each replay."""
+    device, by a captured step at each replay. The codes of moments that are not finite are unspecified."""
     bits, blocks, sizes = check_step(params, grads, copies, decay, exp_avg, exp_avg_sq, scales, hyper, rng, sumsq)
-    n = len(params)
+    n, pointer = len(params), torch.Tensor.data_ptr
     if not n:
         return
     if exp_avg.data_ptr() % 16 or exp_avg_sq.data_ptr() % 16:
@@ -831,17 +841,16 @@ def adamw_tensors_(params, grads, exp_avg, exp_avg_sq, hyper, *, scales=None, rn
     for k in sizes:
         first.append(at)
         at += -(-k // MOMENT_BLOCK)
-    ptrs = c_void_p * n
-    kind = lambda t: 2 if t.dtype == torch.float32 else 0
+    table = Struct(f"={n}q")
     with _device_of(exp_avg):
         rc = typed("adamw_tensors", "nplm_adamw_tensors", "ppppppiiiippplpppp")(
-            ptrs(*[p.data_ptr() for p in params]), ptrs(*[g.data_ptr() for g in grads]),
-            None if copies is None else ptrs(*[c.data_ptr() for c in copies]), (c_longlong * n)(*sizes),
-            (c_longlong * n)(*first), (c_ubyte * n)(*([1] * n if decay is None else map(bool, decay))), n, kind(params[0]),
-            kind(grads[0]), bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), _dp(scales), blocks, hyper.data_ptr(), _dp(sumsq),
-            _dp(rng), raw_stream())
+            table.pack(*map(pointer, params)), table.pack(*map(pointer, grads)),
+            None if copies is None else table.pack(*map(pointer, copies)), table.pack(*sizes), table.pack(*first),
+            bytes([1] * n) if decay is None else bytes(map(bool, decay)), n, 2 if params[0].dtype == torch.float32 else 0,
+            2 if grads[0].dtype == torch.float32 else 0, bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), _dp(scales), blocks,
+            hyper.data_ptr(), _dp(sumsq), _dp(rng), raw_stream())
         check_rc(rc, "adamw_tensors")
-    count_launch(-(-sum(k > 0 for k in sizes) // 128))
+    count_launch(-(-(n - sizes.count(0)) // 128))
 
 
 def moment_values(exp_avg, exp_avg_sq, scales, dtype=torch.float32):
