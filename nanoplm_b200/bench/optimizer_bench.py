@@ -28,6 +28,7 @@ def main():
                     help="library collectives instead of the peer-memory kernels (multi-GPU A/B)")
     ap.add_argument("--per-matrix", action="store_true",
                     help="Muon: orthogonalise matrix by matrix on every rank (no stacking, no split over ranks)")
+    ap.add_argument("--state-bits", type=int, default=32, choices=(8, 32), help="AdamW: bits of the moments")
     args = ap.parse_args()
 
     from nanoplm_b200.config.schema import ModelConfig, PretrainingConfig
@@ -46,7 +47,7 @@ def main():
         hyper = AdamWHyper(lr=1e-3, max_grad_norm=1.0)
         if name == "adamw":
             eng = ShardedEngine(model, hyper, device, compute_dtype=torch.bfloat16,
-                                fused_comm=world > 1 and not args.no_fused_comm)
+                                fused_comm=world > 1 and not args.no_fused_comm, state_bits=args.state_bits)
         else:
             eng = MuonEngine(model, hyper, PretrainingConfig(dataset_dir="x", optimizer=name), device,
                              fused_comm=world > 1 and not args.no_fused_comm)
@@ -77,7 +78,7 @@ def main():
         _lib.check_status()
         if rank == 0:
             print(json.dumps({"bench": "optimizer_step", "optimizer": name + (" (matrix by matrix, replicated)" if args.per_matrix and name != "adamw" else ""),
-                              "n_gpus": world, "peer_memory_comm": getattr(eng, "fused", None) is not None,
+                              "state_bits": getattr(eng, "state_bits", 32), "n_gpus": world, "peer_memory_comm": getattr(eng, "fused", None) is not None,
                               "parameters": eng.num_parameters(), "ms_per_step": round(float(t), 3),
                               "own_kernel_launches_per_step": (_lib.launches() - n0) // args.steps,
                               "note": "includes filling the gradient buffer with random numbers"}), flush=True)

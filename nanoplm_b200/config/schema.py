@@ -70,6 +70,16 @@ class ModelConfig:
     conv_bias: bool = False
     mhc_streams: int = 1                 # 1 = plain residual, 4 = hyper-connections
     mhc_sinkhorn_iters: int = 5
+    # rotary positions beyond the reference's: {"type": linear | ntk | yarn, "factor": s, "original_max_position": n} for a
+    # context s times the trained one; the part of a head's channels that rotates; pairs of neighbours instead of halves
+    rope_scaling: Optional[dict] = None
+    rotary_fraction: float = 1.0
+    rope_interleaved: bool = False
+    # a norm after each block as well, with a gate (none | channel: a weight | token: sigmoid of a projection of the block's
+    # input) and, with residual_scale, a learned scale per channel on the residual stream
+    sandwich_norm: bool = False
+    residual_gate: str = "none"
+    residual_scale: bool = False
     moe: MoEConfig = field(default_factory=MoEConfig)
 
     def __post_init__(self) -> None:
@@ -90,6 +100,13 @@ class ModelConfig:
             raise ValueError("conv_kernel_size must be 0 (off) or an odd size <= 9")
         if self.mhc_streams < 1:
             raise ValueError("mhc_streams must be >= 1")
+        self._check_rotary()
+        if self.residual_gate not in ("none", "channel", "token"):
+            raise ValueError(f"residual_gate must be none, channel or token, got {self.residual_gate}")
+        if (self.residual_gate != "none" or self.residual_scale) and not self.sandwich_norm:
+            raise ValueError("residual_gate and residual_scale need sandwich_norm")
+        if self.sandwich_norm and (self.mhc_streams > 1 or self.norm_bias):
+            raise ValueError("sandwich_norm does not go with hyper-connections (mhc_streams) or norm_bias")
         for name in ("mlp_dropout", "attention_dropout", "embedding_dropout"):
             v = float(getattr(self, name))
             if not 0.0 <= v < 1.0:
@@ -103,9 +120,36 @@ class ModelConfig:
                              "dropout on attention probabilities; set attention_dropout: 0.0 "
                              "(mlp_dropout and embedding_dropout are supported)")
 
+    def _check_rotary(self) -> None:
+        if self.rope_scaling is not None:
+            sc = dict(self.rope_scaling)
+            kind = sc.get("type", "none")
+            if kind not in ("none", "linear", "ntk", "yarn"):
+                raise ValueError(f"rope_scaling.type must be none, linear, ntk or yarn, got {kind}")
+            if kind != "none" and not float(sc.get("factor", 0.0)) >= 1.0:
+                raise ValueError(f"rope_scaling.factor must be at least 1, got {sc.get('factor')}")
+            if kind == "yarn" and not int(sc.get("original_max_position", 0)) > 0:
+                raise ValueError("rope_scaling of type yarn needs original_max_position")
+            unknown = sorted(set(sc) - {"type", "factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor"})
+            if unknown:
+                raise ValueError(f"Unexpected rope_scaling keys: {', '.join(unknown)}")
+            self.rope_scaling = None if kind == "none" else sc
+        if not 0.0 < self.rotary_fraction <= 1.0 or self.rotary_channels < 2:
+            raise ValueError(f"rotary_fraction must leave 2 to {self.head_dim} rotating channels a head, got {self.rotary_fraction}")
+
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_attention_heads
+
+    @property
+    def rotary_channels(self) -> int:
+        """Channels of a head that rotate: an even number."""
+        return int(self.head_dim * self.rotary_fraction) // 2 * 2
+
+    @property
+    def rotary_general(self) -> bool:
+        """Whether rotation takes more than half-layout tables over whole heads."""
+        return self.rope_interleaved or self.rotary_channels != self.head_dim
 
     @property
     def sliding_window(self) -> int:
@@ -182,6 +226,7 @@ class PretrainingConfig:
     shard_params: bool = False           # keep 1/N of every layer's weights per rank, gather inside the GEMMs
     nvtx_ranges: bool = False            # NVTX ranges around data / forward / backward / optimizer (for profilers)
     deterministic_attention: bool = False  # attention backward (~1.4x its time) and linear weight gradients: the same bits every run
+    optimizer_state_bits: int = 32       # 8: AdamW moments as stochastically rounded 8-bit codes, 2 bytes a parameter instead of 8
     hf_checkpoint_files: bool = False    # also write model.safetensors + trainer_state.json (HF-Trainer layout)
 
 

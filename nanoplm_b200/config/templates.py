@@ -29,6 +29,12 @@ model:
   # conv_bias: false
   # mhc_streams: 1                # 4 = manifold-constrained hyper-connections
   # mhc_sinkhorn_iters: 5
+  # rope_scaling: {type: "yarn", factor: 4.0, original_max_position: 1024}   # longer contexts: linear | ntk | yarn
+  # rotary_fraction: 1.0          # part of each head's channels that rotates
+  # rope_interleaved: false       # rotate pairs of neighbours instead of halves
+  # sandwich_norm: false          # a norm after each block as well
+  # residual_gate: "none"         # with sandwich_norm: "channel" (weights) or "token" (learned from the block's input)
+  # residual_scale: false         # with sandwich_norm: a learned scale per channel on the residual stream
   # moe:
   #   num_experts: 0              # e.g. 64
   #   top_k: 2
@@ -102,6 +108,7 @@ pretraining:
   # shard_params: false           # shard the layers' weights over the ranks (all-gather fused into the GEMMs)
   # nvtx_ranges: false            # NVTX ranges around forward / backward / optimizer step
   # deterministic_attention: false  # attention backward and linear weight gradients bitwise reproducible (slower)
+  # optimizer_state_bits: 32      # 8: AdamW moments in 8 bits (2 bytes a parameter instead of 8)
   # hf_checkpoint_files: false    # also write model.safetensors + trainer_state.json with every checkpoint
 
 # The native pipeline (own CUDA kernels, sharded data parallelism). `use_compile` is accepted for

@@ -10,7 +10,9 @@ names equal the reference's, so `pytorch_model.bin` files are interchangeable.
 
 Differences by design: activations are always flat `(T, C)` with `cu_seqlens` (padded input is
 unpadded on entry); the MLM head runs only on positions that carry a label, which leaves the loss
-unchanged; optional varlen depthwise conv, hyper-connections (mHC) and MoE blocks.
+unchanged; optional varlen depthwise conv, hyper-connections (mHC) and MoE blocks, norms after the blocks with a
+gate and a scale on the residual stream, and rotary positions scaled for longer contexts, on part of a head, or
+interleaved.
 """
 from __future__ import annotations
 
@@ -71,6 +73,13 @@ class Embeddings(nn.Module):
         return x
 
 
+class RotaryPlan:
+    """Rotary positions that are not half-layout tables over whole heads: what `ops.rotary_qkv` takes."""
+
+    def __init__(self, frequencies: torch.Tensor, factor: float, interleaved: bool):
+        self.frequencies, self.factor, self.interleaved = frequencies, factor, interleaved
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: ModelConfig):
         super().__init__()
@@ -79,8 +88,12 @@ class Attention(nn.Module):
         self.Wqkv = Linear(cfg.hidden_size, 3 * cfg.hidden_size, cfg.attention_bias)
         self.Wo = Linear(cfg.hidden_size, cfg.hidden_size, cfg.attention_bias)
 
-    def forward(self, x, ctx: "BatchContext", window: int, rope: tuple, residual=None):
+    def forward(self, x, ctx: "BatchContext", window: int, rope, residual=None):
         H, D = self.num_heads, self.head_dim
+        if type(rope) is RotaryPlan:
+            qkv = ops.rotary_qkv(self.Wqkv(x), H, D, positions=ctx.position_ids, frequencies=rope.frequencies,
+                                 factor=rope.factor, interleaved=rope.interleaved)
+            return self.Wo(ops.attention_varlen(qkv, ctx.seq_start, ctx.seq_end, H, D, window, self.scale), residual=residual)
         fused = (x.is_cuda and x.dtype == torch.bfloat16 and D == 64 and self.Wqkv.bias is None
                  and x.dim() == 2 and self.Wqkv.in_features % 8 == 0 and not ops.fp8_enabled())
         if fused:   # RoPE in the QKV GEMM epilogue, its transpose inside the attention backward
@@ -138,6 +151,28 @@ class MLP(nn.Module):
         return self.Wo(h, residual=residual)
 
 
+class BlockJoin(nn.Module):
+    """Where a block ends: norm of its output, gate, scale of the residual stream, sum, and the norm of the next block, in one
+    operator (`ops.sandwich_norm`). The reference has pre-norm blocks only."""
+
+    def __init__(self, cfg: ModelConfig):
+        super().__init__()
+        C = cfg.hidden_size
+        self.eps, self.rms = cfg.norm_eps, cfg.norm_type == "rmsnorm"
+        self.norm_weight = nn.Parameter(torch.ones(C))
+        self.gate = nn.Parameter(torch.ones(C)) if cfg.residual_gate == "channel" else None
+        self.gate_proj = Linear(C, C) if cfg.residual_gate == "token" else None
+        self.scale = nn.Parameter(torch.ones(C)) if cfg.residual_scale else None
+
+    def forward(self, x, y, block_input, next_norm: Optional[Norm]):
+        """(x after the block with output y, next_norm of it or None without one); block_input: what the block was given."""
+        gate, token = self.gate, self.gate_proj is not None
+        if token:
+            gate = self.gate_proj(block_input)
+        return ops.sandwich_norm(x, y, self.norm_weight, None if next_norm is None else next_norm.weight, gate=gate, sigmoid=token,
+                                 scale=self.scale, eps=self.eps, rms=self.rms, with_next=next_norm is not None)
+
+
 class BatchContext:
     """Per-batch device metadata shared by all layers. bounds: (first key, one past the last key) of every token, int32 [T]
     each, where the caller has them; else the sequence of `cu_seqlens` that the token lies in."""
@@ -168,6 +203,10 @@ class EncoderLayer(nn.Module):
         if cfg.conv_kernel_size > 0:
             from .conv import VarlenDepthwiseConv
             self.conv = VarlenDepthwiseConv(cfg.hidden_size, cfg.conv_kernel_size, cfg.conv_bias)
+        self.rotary_general = cfg.rotary_general
+        self.attn_join = self.mlp_join = None
+        if cfg.sandwich_norm:
+            self.attn_join, self.mlp_join = BlockJoin(cfg), BlockJoin(cfg)
         self.mhc_attn = self.mhc_mlp = None
         if cfg.mhc_streams > 1:
             from .mhc import HyperConnection
@@ -189,6 +228,8 @@ class EncoderLayer(nn.Module):
         """The parts are the ones this class was built with, and none of the optional blocks is there."""
         p = self._modules       # (a look-up by attribute walks through the module's __getattr__: 0.5 us each)
         a, m = p["attn"], p["mlp"]
+        if self.rotary_general or self.attn_join is not None:
+            return False
         if not (self.conv is None and type(a) is Attention and type(m) is MLP and type(p["mlp_norm"]) is Norm
                 and type(p["attn_norm"]) is (nn.Identity if self.layer_idx == 0 else Norm)):
             return False
@@ -201,8 +242,22 @@ class EncoderLayer(nn.Module):
         return (type(self.mlp) is MoEMLP and type(self.mlp_norm) is Norm
                 and native_layer.unobserved((self.mlp, self.mlp_norm)))
 
-    def forward(self, x, ctx: BatchContext, window: int, rope: tuple):
+    def _joined(self, x, ctx, window, rope, h=None, next_norm: Optional[Norm] = None):
+        """The layer with norms after its blocks: (x, aux, next_norm of x or None). h: this layer's first norm of x, where the
+        layer before has formed it."""
+        if h is None:
+            h = self.attn_norm(x)
+        own = _joinable(self.mlp_norm)
+        x, n = self.attn_join(x, self._attn_branch(h, ctx, window, rope, residual=None, normed=True), h, self.mlp_norm if own else None)
+        h = n if own else self.mlp_norm(x)
+        y, aux = self.mlp(h) if self.is_moe else (self.mlp(h), None)
+        x, h = self.mlp_join(x, y, h, next_norm)
+        return x, aux, h
+
+    def forward(self, x, ctx: BatchContext, window: int, rope):
         aux = None
+        if self.attn_join is not None:
+            return self._joined(x, ctx, window, rope)[:2]
         if self.mhc_attn is None:
             if x.is_cuda and self._plain():
                 y = native_layer.run(self.attn, self.mlp, self.attn_norm, self.mlp_norm, x, ctx, window, rope)
@@ -241,6 +296,11 @@ class EncoderLayer(nn.Module):
         return x, aux, (h, state)
 
 
+def _joinable(norm) -> bool:
+    """A norm of this package that the operator before it may form: nobody watches its call."""
+    return type(norm) is Norm and native_layer.unobserved((norm,))
+
+
 _LAYER_FORWARD = EncoderLayer.forward
 
 
@@ -270,10 +330,21 @@ class EncoderModel(nn.Module):
         if key not in self._rope_cache:
             c = self.config
             self._rope_cache[key] = {
-                "full_attention": ops.rope_tables(c.max_position_embeddings, c.head_dim, c.global_rope_theta, device),
-                "sliding_attention": ops.rope_tables(c.max_position_embeddings, c.head_dim, c.local_rope_theta, device),
+                "full_attention": self._rope_of(c.global_rope_theta, device),
+                "sliding_attention": self._rope_of(c.local_rope_theta, device),
             }
         return self._rope_cache[key]
+
+    def _rope_of(self, theta: float, device):
+        """Tables (cos, sin) for halves of whole heads, which the QKV product's epilogue takes, else a plan."""
+        c = self.config
+        if not c.rotary_general and c.rope_scaling is None:
+            return ops.rope_tables(c.max_position_embeddings, c.head_dim, theta, device)
+        w, factor = ops.rotary_frequencies(c.rotary_channels, theta, c.rope_scaling, device)
+        if c.rotary_general:
+            return RotaryPlan(w, factor, c.rope_interleaved)
+        a = torch.outer(torch.arange(c.max_position_embeddings, dtype=torch.float64, device=device), w)
+        return (factor * a.cos()).float().contiguous(), (factor * a.sin()).float().contiguous()
 
     def forward_hidden(self, input_ids, ctx: BatchContext):
         """Returns the residual stream after the last layer (before final_norm) and MoE aux loss."""
@@ -285,7 +356,7 @@ class EncoderModel(nn.Module):
             x = x.unsqueeze(1).expand(-1, n, -1).contiguous()
         aux_total = None
         layers = list(self.layers)
-        if n <= 1 and x.is_cuda:    # several layers to a native call, as far as they are plain
+        if n <= 1 and x.is_cuda and not cfg.rotary_general:    # several layers to a native call, as far as they are plain
             types = [layer.attention_type for layer in layers]
             x, done = native_layer.run_stack(layers, _stackable, x, ctx,
                                              [-1 if t == "full_attention" else cfg.sliding_window for t in types],
@@ -294,10 +365,17 @@ class EncoderModel(nn.Module):
         # on streams, a layer's last write and the next one's first read are one where nobody watches the layers' calls
         own = [n > 1 and x.is_cuda and _own_forward(layer) and native_layer.unobserved((layer,)) for layer in layers]
         entry = None
+        # a layer's last norm and the next one's first are one where nobody watches the layers' and the norm's calls
+        joined = [cfg.sandwich_norm and _own_forward(layer) and native_layer.unobserved((layer,)) for layer in layers]
         for i, layer in enumerate(layers):
             lt = layer.attention_type
             window = -1 if lt == "full_attention" else cfg.sliding_window
-            if own[i]:
+            if joined[i]:
+                after = layers[i + 1].attn_norm if i + 1 < len(layers) and joined[i + 1] else None
+                if after is not None and not _joinable(after):
+                    after = None
+                x, aux, entry = layer._joined(x, ctx, window, rope[lt], entry, after)
+            elif own[i]:
                 nxt = layers[i + 1].mhc_attn if i + 1 < len(layers) and own[i + 1] else None
                 x, aux, entry = layer._streams(x, ctx, window, rope[lt], entry, nxt)
             else:
@@ -375,6 +453,15 @@ class ProtEncoderMLM(nn.Module):
             for lin in lins:
                 if lin.bias is not None:
                     nn.init.zeros_(lin.bias)
+            for join, out in ((layer.attn_join, layer.attn.Wo), (layer.mlp_join, getattr(layer.mlp, "Wo", None))):
+                if join is not None:
+                    # a norm behind zeros multiplies the first gradients by 1 / sqrt(eps): the projection starts like the
+                    # others, and the branches add up to a stream of twice the input's variance through the norm's weight
+                    nn.init.constant_(join.norm_weight, (2 * cfg.num_hidden_layers) ** -0.5)
+                    if out is not None:
+                        nn.init.uniform_(out.weight, -bound, bound)
+                    if join.gate_proj is not None:
+                        nn.init.zeros_(join.gate_proj.weight)
         nn.init.uniform_(self.head.dense.weight, -bound, bound)
         if self.head.dense.bias is not None:
             nn.init.zeros_(self.head.dense.bias)

@@ -597,6 +597,40 @@ def rotary(q, k=None, *, positions, frequencies, factor: float = 1.0, interleave
     return out if k is None else (out, _rotate_plain(k, positions, frequencies, factor, interleaved))
 
 
+def _qk_heads(qkv, H: int, D: int):
+    x = qkv.view(qkv.shape[0], 3, H, D)
+    return x[:, 0], x[:, 1]
+
+
+class _RotaryQkvFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, positions, frequencies, factor, interleaved, H, D):
+        ctx.save_for_backward(positions, frequencies)
+        ctx.how = (factor, interleaved, H, D)
+        K.rotary(*_qk_heads(qkv, H, D), positions, frequencies, factor, interleaved, inplace=True)
+        ctx.mark_dirty(qkv)
+        return qkv
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d):
+        positions, frequencies = ctx.saved_tensors
+        factor, interleaved, H, D = ctx.how
+        d = d.contiguous()
+        out = torch.empty_like(d)
+        K.rotary(*_qk_heads(d, H, D), positions, frequencies, factor, interleaved, transposed=True, out=_qk_heads(out, H, D))
+        out[:, 2 * H * D:] = d[:, 2 * H * D:]
+        return out, None, None, None, None, None, None
+
+
+def rotary_qkv(qkv, H: int, D: int, *, positions, frequencies, factor: float = 1.0, interleaved: bool = False):
+    """`rotary` on the q and k parts of a packed projection [T, 3 * H * D], in place on a GPU."""
+    if qkv.is_cuda and qkv.dtype in K.ROW_TYPES and D <= K.ROTARY_MAX_WIDTH and qkv.is_contiguous():
+        return _RotaryQkvFn.apply(qkv, positions, frequencies, factor, interleaved, H, D)
+    q, k = rotary(*_qk_heads(qkv, H, D), positions=positions, frequencies=frequencies, factor=factor, interleaved=interleaved)
+    return torch.cat((q.flatten(1), k.flatten(1), qkv[:, 2 * H * D:]), dim=1)
+
+
 # ------------------------------------------------------------------------------------- attention
 class _AttnFn(torch.autograd.Function):
     @staticmethod

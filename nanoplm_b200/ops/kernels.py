@@ -512,9 +512,9 @@ def check_rotary(q, k, positions, frequencies):
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, factor: float = 1.0,
-           interleaved: bool = False, transposed: bool = False, inplace: bool = False):
+           interleaved: bool = False, transposed: bool = False, inplace: bool = False, out: tuple | None = None):
     """Rotary positions on q [T, H, D] or [B, S, H, D] and, in the same launch, k with as many tokens, any number of heads and
-    the same width: (q', k'), contiguous, or with `inplace` q and k themselves.
+    the same width: (q', k'), contiguous, or `out` (tensors like q and k, of any strides), or with `inplace` q and k themselves.
 
     bf16, fp16 or fp32; the last dimension contiguous, the others of any stride. positions: int32 or int64, [T], [B, S], or [S]
     for all of a batch. frequencies: fp64 [R / 2], radians a position for each pair of the first R channels of a head; the
@@ -524,14 +524,22 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     kind = ROW_TYPES.get(q.dtype)
     if kind is None or D > ROTARY_MAX_WIDTH:
         raise ValueError(f"q must be bf16, fp16 or fp32 with heads of up to {ROTARY_MAX_WIDTH} channels, got {q.dtype}, {D}")
-    for t, name in ((q, "q"), (k, "k")):
+    if inplace:
+        out = (q, k)
+    qo, ko = out or (None, None)
+    if out is not None and ((ko is None) != (k is None) or qo.shape != q.shape or qo.dtype != q.dtype
+                            or (k is not None and (ko.shape != k.shape or ko.dtype != k.dtype))):
+        raise ValueError("out must be like q and k")
+    for t, name in ((q, "q"), (k, "k"), (qo, "out"), (ko, "out")):
         if t is not None and t.stride(-1) != 1 and t.numel():
             raise ValueError(f"{name} must have a contiguous last dim")
-        if inplace and t is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
-            raise ValueError(f"{name} is written in place but has elements that share memory")
-    with _device_of(q, k, positions, frequencies):
-        if inplace:
-            qo, ko, qos, kos = q, k, qs, ks
+    for t in (qo, ko):
+        if t is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            raise ValueError("what is written has elements that share memory")
+    with _device_of(q, k, positions, frequencies, qo, ko):
+        if out is not None:
+            heads = lambda t: (0, 0, 0) if t is None else (0, *t.stride()[:2]) if t.dim() == 3 else t.stride()[:3]
+            qos, kos = heads(qo), heads(ko)
         else:
             qo, qos = torch.empty(q.shape, dtype=q.dtype, device=q.device), (S * H * D, H * D, D)
             ko, kos = (None, (0, 0, 0)) if k is None else (torch.empty(k.shape, dtype=k.dtype, device=k.device), (S * Hk * D, Hk * D, D))

@@ -73,7 +73,13 @@ def _invalidate_fp8_weights() -> None:
 class ShardedEngine:
     def __init__(self, model: nn.Module, hyper: AdamWHyper, device: torch.device,
                  process_group=None, compute_dtype: torch.dtype = torch.bfloat16,
-                 fused_comm: bool = False, exclude: Iterable[str] = (), decay_all: bool = False):
+                 fused_comm: bool = False, exclude: Iterable[str] = (), decay_all: bool = False, state_bits: int = 32):
+        """state_bits 8: the moments as 8-bit codes (`ops.moments`), 2 bytes an element instead of 8; the step is then one kernel
+        over all tensors, and between ranks the library's collectives move gradients and parameters."""
+        if state_bits not in (8, 32):
+            raise ValueError(f"optimizer states have 8 or 32 bits, got {state_bits}")
+        self.state_bits = state_bits
+        fused_comm = fused_comm and state_bits == 32
         self.model = model
         self.hyper = hyper
         self.device = torch.device(device)
@@ -130,8 +136,17 @@ class ShardedEngine:
             self.flat_params = torch.zeros(self.total, dtype=self.compute_dtype, device=dev)
             self.main_grad = torch.zeros(self.total, dtype=torch.float32, device=dev)
         self.master = torch.zeros(self.shard, dtype=torch.float32, device=dev)
-        self.exp_avg = torch.zeros(self.shard, dtype=torch.float32, device=dev)
-        self.exp_avg_sq = torch.zeros(self.shard, dtype=torch.float32, device=dev)
+        if state_bits == 8:
+            from nanoplm_b200.ops.moments import TensorMoments
+            # this rank's part of every tensor, as (from, to) in its slice
+            self._parts = [(max(s.offset, self.lo) - self.lo, min(s.offset + s.numel, self.hi) - self.lo, s.decay) for s in self.slots
+                           if s.offset < self.hi and s.offset + s.numel > self.lo]
+            self.moments = TensorMoments([b - a for a, b, _ in self._parts], dev, 8)
+            self._rng = torch.zeros(1, dtype=torch.int64, device=dev)
+        else:
+            self.moments = None
+            self.exp_avg = torch.zeros(self.shard, dtype=torch.float32, device=dev)
+            self.exp_avg_sq = torch.zeros(self.shard, dtype=torch.float32, device=dev)
         self._sumsq = torch.zeros(1, dtype=torch.float32, device=dev)
         self._hyper_dev = torch.zeros(2, 9, dtype=torch.float32, device=dev)
         self._hyper_host = torch.zeros(2, 9, dtype=torch.float32,
@@ -266,7 +281,9 @@ class ShardedEngine:
         grad_norm = self._sumsq.sqrt() * grad_scale
         # 3. clip + AdamW on the owned slice, decay part then no-decay part
         new_shard = self.flat_params[self.lo:self.hi]
-        for i, (a, b) in enumerate(((0, self.decay_end), (self.decay_end, self.total))):
+        if self.moments is not None:
+            self._step_8bit(shard_grad, new_shard)
+        for i, (a, b) in enumerate(((0, self.decay_end), (self.decay_end, self.total)) if self.moments is None else ()):
             a, b = max(a, self.lo), min(b, self.hi)
             if b <= a:
                 continue
@@ -282,6 +299,34 @@ class ShardedEngine:
             dist.all_gather_into_tensor(self.flat_params, new_shard.clone(), group=self.pg)
         self.main_grad.zero_()
         return grad_norm
+
+    def _step_8bit(self, grad, out) -> None:
+        """Clip + AdamW on the owned slice, tensor by tensor in one launch. The rounding's random numbers follow from the step
+        and the rank: a resumed run rounds as the uninterrupted one would."""
+        cut = lambda flat: [flat[a:b] for a, b, _ in self._parts]
+        self._rng.fill_((self.step_count << 20) + self.rank)
+        copies = cut(out) if self.compute_dtype == torch.bfloat16 else None
+        self.moments.step(cut(self.master), cut(grad), self._hyper_dev[0], rng=self._rng, copies=copies,
+                          decay=[d for _, _, d in self._parts], sumsq=self._sumsq)
+        if copies is None:
+            out.copy_(self.master)
+
+    def _moments_flat(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """fp32 first and second moments of this rank's slice."""
+        if self.moments is None:
+            return self.exp_avg, self.exp_avg_sq
+        both = torch.zeros(2, self.shard, dtype=torch.float32, device=self.device)
+        for flat, parts in zip(both, self.moments.values()):
+            for (a, b, _), t in zip(self._parts, parts):
+                flat[a:b] = t
+        return both[0], both[1]
+
+    def _set_moments(self, m: torch.Tensor, v: torch.Tensor) -> None:
+        if self.moments is None:
+            self.exp_avg.copy_(m)
+            self.exp_avg_sq.copy_(v)
+        else:
+            self.moments.load([m[a:b] for a, b, _ in self._parts], [v[a:b] for a, b, _ in self._parts])
 
     def _adamw_reference(self, sl, grad, out, group, lr, grad_scale) -> None:
         self._adamw_cpu(self.master[sl], self.exp_avg[sl], self.exp_avg_sq[sl], grad[sl], out[sl], group, lr,
@@ -357,8 +402,7 @@ class ShardedEngine:
     def optimizer_state_dict(self) -> dict:
         """torch.optim.AdamW-compatible state dict (full tensors; collective on every rank).
         Parameter order = decay group then no-decay group (reference: pure_pipeline.py:127-130)."""
-        m = self._gather_full(self.exp_avg).cpu()
-        v = self._gather_full(self.exp_avg_sq).cpu()
+        m, v = (self._gather_full(t).cpu() for t in self._moments_flat())
         h = self.hyper
         state, groups = {}, []
         idx = 0
@@ -384,8 +428,7 @@ class ShardedEngine:
         return {"state": state, "param_groups": groups}
 
     def load_optimizer_state_dict(self, sd: dict) -> None:
-        m = self._gather_full(self.exp_avg).clone()
-        v = self._gather_full(self.exp_avg_sq).clone()
+        m, v = (self._gather_full(t).clone() for t in self._moments_flat())
         ordered = [s for s in self.slots if s.decay] + [s for s in self.slots if not s.decay]
         step = 0
         for idx, s in enumerate(ordered):
@@ -395,22 +438,20 @@ class ShardedEngine:
             m[s.offset:s.offset + s.numel] = st["exp_avg"].to(m.device, torch.float32).reshape(-1)
             v[s.offset:s.offset + s.numel] = st["exp_avg_sq"].to(v.device, torch.float32).reshape(-1)
             step = max(step, int(float(st["step"])))
-        self.exp_avg.copy_(self._take_local(m))
-        self.exp_avg_sq.copy_(self._take_local(v))
+        self._set_moments(self._take_local(m), self._take_local(v))
         self.step_count = step
 
     def shard_state(self) -> dict:
         """This rank's slice only (sharded checkpoint fast path)."""
+        m, v = self._moments_flat()
         return {"rank": self.rank, "world": self.world, "total": self.total, "step": self.step_count,
-                "master": self.master.cpu(), "exp_avg": self.exp_avg.cpu(),
-                "exp_avg_sq": self.exp_avg_sq.cpu()}
+                "master": self.master.cpu(), "exp_avg": m.cpu(), "exp_avg_sq": v.cpu()}
 
     def load_shard_state(self, st: dict) -> None:
         if st["world"] != self.world or st["total"] != self.total:
             raise ValueError("sharded checkpoint was written with a different world size / layout")
         self.master.copy_(st["master"])
-        self.exp_avg.copy_(st["exp_avg"])
-        self.exp_avg_sq.copy_(st["exp_avg_sq"])
+        self._set_moments(st["exp_avg"], st["exp_avg_sq"])
         self.step_count = int(st["step"])
         full = self._gather_full(self.master)
         self.flat_params.copy_(full.to(self.compute_dtype))

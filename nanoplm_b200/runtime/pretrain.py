@@ -163,6 +163,18 @@ def build_collators(tokenizer, cfg: PretrainingConfig, pt: PureTorchConfig, max_
     return train, ProtDataCollatorForLM(tokenizer, **kw, seed=seed + 1)
 
 
+def check_state_bits(cfg: PretrainingConfig, distributed: bool) -> int:
+    """`optimizer_state_bits`, where the other settings allow it."""
+    bits = int(getattr(cfg, "optimizer_state_bits", 32) or 32)
+    if bits not in (8, 32):
+        raise ValueError(f"optimizer_state_bits must be 8 or 32, got {bits}")
+    if bits == 8 and (str(cfg.optimizer).lower() not in ("adamw", "stable_adamw") or int(getattr(cfg, "expert_parallel_size", 1) or 1) > 1
+                      or (bool(getattr(cfg, "shard_params", False)) and distributed)):
+        raise ValueError("optimizer_state_bits: 8 is implemented for the AdamW engine without expert parallelism and "
+                         "without shard_params")
+    return bits
+
+
 def run_pretraining(model: ProtEncoderMLM, pretrain_config: PretrainingConfig,
                     pure_torch_config: Optional[PureTorchConfig] = None,
                     resume_config: Optional[ResumeConfig] = None, max_steps: Optional[int] = None,
@@ -214,6 +226,7 @@ def run_pretraining(model: ProtEncoderMLM, pretrain_config: PretrainingConfig,
                        weight_decay=float(cfg.adam_weight_decay), max_grad_norm=float(cfg.max_grad_norm))
     opt_name = str(cfg.optimizer).lower()
     ep_size = int(getattr(cfg, "expert_parallel_size", 1) or 1)
+    state_bits = check_state_bits(cfg, distributed)
     if ep_size > 1:
         # experts split over the data-parallel ranks (peer-memory dispatch / combine on CUDA)
         if ep_size > world or world % ep_size:
@@ -241,7 +254,7 @@ def run_pretraining(model: ProtEncoderMLM, pretrain_config: PretrainingConfig,
             engine_cls = ParamShardedEngine
         engine = engine_cls(model, hyper, device,
                             compute_dtype=torch.bfloat16 if use_bf16 else torch.float32,
-                            fused_comm=bool(cfg.fused_comm))
+                            fused_comm=bool(cfg.fused_comm), **({"state_bits": 8} if state_bits == 8 else {}))
     else:
         raise ValueError(f"Invalid optimizer: {cfg.optimizer}. Supported: [adamw, stable_adamw, muon, normuon]")
     model.train()
