@@ -256,9 +256,10 @@ __device__ __forceinline__ void at_moments(const float (&g)[8], float (&m)[8], f
     v[e + 1] = __fadd_rn(v0.y, v1.y);
   }
 }
-template <typename P, typename G>
-__device__ __forceinline__ void at_weights(const P (&old)[8], const float (&m)[8], const float (&v)[8], const AtPlace<P, G>& at,
-                                           const AdamScalars& s, int lane) {
+// p, copy: the block's first element; copy may be null. s.decay: the tensor's.
+template <typename P>
+__device__ __forceinline__ void at_weights(const P (&old)[8], const float (&m)[8], const float (&v)[8], P* p, __nv_bfloat16* copy,
+                                           int n, bool vec, const AdamScalars& s, int lane) {
   P pv[8];
   __nv_bfloat16 half[8];
   float root[8];
@@ -269,17 +270,16 @@ __device__ __forceinline__ void at_weights(const P (&old)[8], const float (&m)[8
 #pragma unroll
     for (int e = 0; e < 8; ++e) asm("sqrt.approx.f32 %0, %1;" : "=f"(root[e]) : "f"(v[e]));
   }
-  const float decay = at.decays ? s.decay : 1.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root[e], s.inv_bc2, s.eps)));
-    const float pn = fmaf(-s.step, m[e] * inv, __fmul_rn(at_get<P>(old[e]), decay));
+    const float pn = fmaf(-s.step, m[e] * inv, __fmul_rn(at_get<P>(old[e]), s.decay));
     pv[e] = at_put<P>(pn);
     half[e] = at_put<__nv_bfloat16>(pn);
   }
-  at_store(at.p, lane, at.n(), at.vec(), pv);
-  if (at.copy != nullptr) at_store(at.copy, lane, at.n(), at.vec(), half);
+  at_store(p, lane, n, vec, pv);
+  if (copy != nullptr) at_store(copy, lane, n, vec, half);
 }
 
 // A block with fp32 moments.
@@ -296,15 +296,61 @@ __device__ __forceinline__ void at_block(const AtPlace<P, G>& at, float* m_all, 
 #pragma unroll
   for (int e = 0; e < 8; ++e) g[e] = at_get<G>(gv[e]);
   at_moments(g, m, v, s);       // (behind the tensor m, v and g are zero, and stay so)
-  at_weights(pv, m, v, at, s, lane);
+  at_weights(pv, m, v, at.p, at.copy, at.n(), at.vec(), s, lane);
   at_store(mp, lane, AT_BLOCK, true, m);
   at_store(vp, lane, AT_BLOCK, true, v);
 }
 
-// A block with 8-bit moments, its inputs in shared memory; em, ev: its exponents, and then the new ones.
+// Codes of a lane's eight moments in a block of exponent e; x: their 32 random bits, of which the first moment takes the lowest 20
+// and the second the highest. low: the smallest magnitude.
+template <bool SIGNED>
+__device__ __forceinline__ void at_pack(const float (&v)[8], float low, uint32_t e, const uint32_t (&x)[8], uint32_t (&code)[2]) {
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = SIGNED ? x[i] & 0xfffffu : x[i] >> 12;
+  if (!at_plain<SIGNED>(e)) {
+    const uint32_t bottom = at_base<SIGNED>(e) << 20;
+    code[0] = at_codes<SIGNED>(v, r, bottom);
+    code[1] = at_codes<SIGNED>(v + 4, r + 4, bottom);
+    return;
+  }
+  const float lift = at_lift<SIGNED>(e);
+  float a[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = v[i] * lift;
+  if (!(low * lift >= AT_LEAST)) {
+    // Some are below code 1: they become the value of code 1, or that of a code 0, by the rule of at_codes, and are not rounded.
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float size = fabsf(a[i]);
+      bool up = v[i] != 0.f;
+      if (SIGNED) {     // r 2^-20 code 1 < size; r as a number: its bits behind 2^23, less that
+        const float rf = __uint_as_float(0x4b000000u | r[i]) - 8388608.f;
+        up = __fmul_rn(rf, AT_LEAST * 9.5367431640625e-7f) < size || (r[i] == 0u && up);
+      }
+      const float to = up ? copysignf(AT_LEAST, a[i]) : AT_LEAST / 1.125f;
+      r[i] = size < AT_LEAST ? 0u : r[i];
+      a[i] = size < AT_LEAST ? to : a[i];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    uint32_t t[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t[i] = (__float_as_uint(a[4 * j + i]) + r[4 * j + i]) << 4;
+    code[j] = at_top_bytes(t[0], t[1], t[2], t[3]);
+    if (SIGNED)
+      code[j] |= 0x80808080u & at_top_bytes(__float_as_uint(a[4 * j]), __float_as_uint(a[4 * j + 1]), __float_as_uint(a[4 * j + 2]),
+                                            __float_as_uint(a[4 * j + 3]));
+  }
+}
+
+// A block with 8-bit moments, its inputs in shared memory. em, ev: its exponents, and then the new ones. p, copy: its first element.
+// mc, vc: the lane's codes. first, key: the place of its first element modulo 2^32, and what it is mixed with.
 template <typename P, typename G>
-__device__ __forceinline__ void at_block(const AtStage<P, G>& in, const AtPlace<P, G>& at, uint8_t* m_all, uint8_t* v_all,
-                                         uint32_t& em, uint32_t& ev, const AdamScalars& s, int lane) {
+__device__ __forceinline__ void at_block(const AtStage<P, G>& in, P* p, __nv_bfloat16* copy, int n, bool vec, uint32_t* mc,
+                                         uint32_t* vc, uint32_t first, uint32_t key, uint32_t& em, uint32_t& ev,
+                                         const AdamScalars& s, int lane) {
   float m[8], v[8];
   {
     G gv[8];
@@ -323,7 +369,7 @@ __device__ __forceinline__ void at_block(const AtStage<P, G>& in, const AtPlace<
   {
     P pv[8];
     at_load(in.p, lane, AT_BLOCK, true, pv);
-    at_weights(pv, m, v, at, s, lane);
+    at_weights(pv, m, v, p, copy, n, vec, s, lane);
   }
   float top_m = fabsf(m[0]), top_v = v[0], low_m = fabsf(m[0]), low_v = v[0];
 #pragma unroll
@@ -337,57 +383,21 @@ __device__ __forceinline__ void at_block(const AtStage<P, G>& in, const AtPlace<
   ev = at_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
   // The random bits are at_mix(place ^ key) of the element's place. Places of a block differ in their lowest 8 bits, so the
   // mix's first shift gives all of them the same.
-  const long long first = static_cast<long long>(at.block) * AT_BLOCK;
-  const uint32_t key = at_mix(s.key + static_cast<uint32_t>(first >> 32));
-  uint32_t mine = (static_cast<uint32_t>(first) + lane * 4) ^ key;
+  uint32_t mine = (first + lane * 4) ^ key;
   mine ^= mine >> 16;
-  uint32_t x[8];
+  uint32_t x[8], code[2];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     uint32_t h = (mine ^ ((e >> 2) * 128 + (e & 3))) * 0x7feb352du;
     h = (h ^ (h >> 15)) * 0x846ca68bu;
     x[e] = h ^ (h >> 16);
   }
-  uint32_t *mc = reinterpret_cast<uint32_t*>(m_all + first) + lane, *vc = reinterpret_cast<uint32_t*>(v_all + first) + lane;
-  const float lift_m = at_lift<true>(em), lift_v = at_lift<false>(ev);
-  uint32_t cm[2], cv[2];
-  if (at_plain<true>(em) && low_m * lift_m >= AT_LEAST) {
-#pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      uint32_t t[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = (__float_as_uint(m[j + e] * lift_m) + (x[j + e] & 0xfffffu)) << 4;
-      const uint32_t signs = at_top_bytes(__float_as_uint(m[j]), __float_as_uint(m[j + 1]), __float_as_uint(m[j + 2]), __float_as_uint(m[j + 3]));
-      cm[j / 4] = at_top_bytes(t[0], t[1], t[2], t[3]) | (signs & 0x80808080u);
-    }
-  } else {
-    uint32_t r[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = x[e] & 0xfffffu;
-    const uint32_t bm = at_base<true>(em) << 20;
-    cm[0] = at_codes<true>(m, r, bm);
-    cm[1] = at_codes<true>(m + 4, r + 4, bm);
-  }
-  if (at_plain<false>(ev) && low_v * lift_v >= AT_LEAST) {
-#pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      uint32_t t[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) t[e] = (__float_as_uint(v[j + e] * lift_v) + (x[j + e] >> 12)) << 4;
-      cv[j / 4] = at_top_bytes(t[0], t[1], t[2], t[3]);
-    }
-  } else {
-    uint32_t r[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = x[e] >> 12;
-    const uint32_t bv = at_base<false>(ev) << 20;
-    cv[0] = at_codes<false>(v, r, bv);
-    cv[1] = at_codes<false>(v + 4, r + 4, bv);
-  }
-  mc[0] = cm[0];
-  mc[32] = cm[1];
-  vc[0] = cv[0];
-  vc[32] = cv[1];
+  at_pack<true>(m, low_m, em, x, code);
+  mc[0] = code[0];
+  mc[32] = code[1];
+  at_pack<false>(v, low_v, ev, x, code);
+  vc[0] = code[0];
+  vc[32] = code[1];
 }
 
 // hyper: [lr, beta1, beta2, eps, weight_decay, bias_corr1, bias_corr2, grad_scale, max_norm]; rng: one 64-bit number, another one
@@ -425,9 +435,81 @@ adamw_tensors_kernel(const __grid_constant__ AdamTensors t, float* m, float* v, 
   AtPlace<P, G> at;
   at.find(t, blockIdx.x, warp_index());
   if (at.rest <= 0) return;
-  const AdamScalars s = at_scalars(hyper, sumsq, nullptr);
+  AdamScalars s = at_scalars(hyper, sumsq, nullptr);
+  if (!at.decays) s.decay = 1.f;
   do at_block(at, m, v, s, lane);
   while (at.next());
+}
+
+// The blocks of a chunk that are a warp's. WHOLE: all of them are, on 16 bytes; their addresses are then steps from lane to lane
+// and block to block, and nothing is asked of them.
+template <typename P, typename G, bool WHOLE>
+__device__ __forceinline__ void at_chunk(AtPlace<P, G> at, AtStage<P, G>* ring, uint8_t* m_all, uint8_t* v_all,
+                                         uint8_t (*exponents)[AT_CHUNK], int held, const float* hyper, const float* sumsq,
+                                         const long long* rng, int warp, int lane) {
+  constexpr int step = AT_WARPS * AT_BLOCK;
+  const long long first = static_cast<long long>(at.block) * AT_BLOCK;
+  const P* p_next = at.p;
+  const G* g_next = at.g;
+  const uint8_t* codes = (lane < 16 ? m_all : v_all) + first + (lane & 15) * 16;
+  int left = at.rest;         // elements from the block to fetch next on
+  auto fetch = [&](AtStage<P, G>& to) {
+    if (WHOLE || (at.aligned && left >= AT_BLOCK)) {
+      at_fetch(to.p, p_next, lane);
+      at_fetch(to.g, g_next, lane);
+    } else {      // (there for the warp after its next __syncwarp)
+      P pv[8];
+      G gv[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pv[e] = e * 32 + lane < left ? p_next[e * 32 + lane] : P(0.f);
+        gv[e] = e * 32 + lane < left ? g_next[e * 32 + lane] : G(0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        to.p[e * 32 + lane] = pv[e];
+        to.g[e * 32 + lane] = gv[e];
+      }
+    }
+    at_copy_16((lane < 16 ? to.m : to.v) + (lane & 15) * 16, codes);
+    p_next += step;
+    g_next += step;
+    codes += step;
+    left -= step;
+  };
+  if (warp < held) fetch(ring[0]);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  AdamScalars s = at_scalars(hyper, sumsq, rng);
+  if (!at.decays) s.decay = 1.f;
+  __syncthreads();            // the exponents are there
+  uint32_t high = static_cast<uint32_t>(first >> 32), low = static_cast<uint32_t>(first);
+  uint32_t key = at_mix(s.key + high);
+  uint32_t *mc = reinterpret_cast<uint32_t*>(m_all + first) + lane, *vc = reinterpret_cast<uint32_t*>(v_all + first) + lane;
+  P* p = at.p;
+  __nv_bfloat16* copy = at.copy;
+  int rest = at.rest, stage = 0;
+  for (int j = warp; j < held; j += AT_WARPS) {
+    __syncwarp();     // every lane has read the stage that is filled now
+    if (j + AT_WARPS < held) fetch(ring[stage ^ 1]);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    uint32_t em = exponents[0][j], ev = exponents[1][j];
+    const int n = WHOLE || rest >= AT_BLOCK ? AT_BLOCK : rest;
+    at_block(ring[stage], p, copy, n, WHOLE || (at.aligned && n == AT_BLOCK), mc, vc, low, key, em, ev, s, lane);
+    if (lane == 0) {
+      exponents[0][j] = static_cast<uint8_t>(em);
+      exponents[1][j] = static_cast<uint8_t>(ev);
+    }
+    p += step;
+    if (copy != nullptr) copy += step;
+    mc += step / 4;
+    vc += step / 4;
+    rest -= step;
+    low += step;
+    if (low < step) key = at_mix(s.key + ++high);
+    stage ^= 1;
+  }
 }
 
 // With 8-bit moments a warp's next block is on its way to shared memory while it works on one: there is about as much to
@@ -443,56 +525,15 @@ adamw_tensors_8bit_kernel(const __grid_constant__ AdamTensors t, uint8_t* m, uin
   grid_chain();
   const int lane = threadIdx.x & 31, warp = warp_index();
   AtStage<P, G>* ring = reinterpret_cast<AtStage<P, G>*>(at_smem) + warp * AT_STAGES;
-  auto fetch = [&](const AtPlace<P, G>& at, AtStage<P, G>& to) {
-    if (at.vec()) {
-      at_fetch(to.p, at.p, lane);
-      at_fetch(to.g, at.g, lane);
-    } else {      // (there for the warp after its next __syncwarp)
-      const int n = at.n();
-      P pv[8];
-      G gv[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        pv[e] = e * 32 + lane < n ? at.p[e * 32 + lane] : P(0.f);
-        gv[e] = e * 32 + lane < n ? at.g[e * 32 + lane] : G(0.f);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        to.p[e * 32 + lane] = pv[e];
-        to.g[e * 32 + lane] = gv[e];
-      }
-    }
-    const long long first = static_cast<long long>(at.block) * AT_BLOCK;
-    if (lane < 16) at_copy_16(to.m + lane * 16, m + first + lane * 16);
-    else at_copy_16(to.v + lane * 16 - AT_BLOCK, v + first + lane * 16 - AT_BLOCK);
-  };
   AtPlace<P, G> at;
   at.find(t, blockIdx.x, warp);
-  bool more = at.rest > 0;
-  const int of_chunk = at.block - warp;       // the chunk's first block, and how many it has
-  const int held = min(t.per_chunk, static_cast<int>(min((at.rest + warp * AT_BLOCK + AT_BLOCK - 1LL) / AT_BLOCK, 1LL * AT_CHUNK)));
-  if (more) fetch(at, ring[0]);
-  asm volatile("cp.async.commit_group;" ::: "memory");
+  const int of_chunk = at.block - warp, elements = at.rest + warp * AT_BLOCK;       // the chunk's first block, and its elements
+  const int held = (elements + AT_BLOCK - 1) / AT_BLOCK;
   if (warp < 2 && lane < held) exponents[warp][lane] = scales[warp * blocks + of_chunk + lane];
-  const AdamScalars s = at_scalars(hyper, sumsq, rng);
-  __syncthreads();
-  int stage = 0;
-  for (int j = warp; more; j += AT_WARPS) {
-    const AtPlace<P, G> now = at;
-    more = at.next();
-    __syncwarp();     // every lane has read the stage that is filled now
-    if (more) fetch(at, ring[stage ^ 1]);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    __syncwarp();
-    uint32_t em = exponents[0][j], ev = exponents[1][j];
-    at_block(ring[stage], now, m, v, em, ev, s, lane);
-    if (lane == 0) {
-      exponents[0][j] = static_cast<uint8_t>(em);
-      exponents[1][j] = static_cast<uint8_t>(ev);
-    }
-    stage ^= 1;
-  }
+  if (at.aligned && elements % AT_BLOCK == 0)
+    at_chunk<P, G, true>(at, ring, m, v, exponents, held, hyper, sumsq, rng, warp, lane);
+  else
+    at_chunk<P, G, false>(at, ring, m, v, exponents, held, hyper, sumsq, rng, warp, lane);
   __syncthreads();
   if (warp < 2 && lane < held) scales[warp * blocks + of_chunk + lane] = exponents[warp][lane];
 }

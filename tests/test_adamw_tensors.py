@@ -175,6 +175,24 @@ def test_kernel_has_the_bits_of_the_restatement(bits, p_type, g_type, shift, cud
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-30, 1e-22, 1e-15, 1.0, 1e12, 1e17])
+def test_codes_of_extreme_and_of_far_apart_gradients(size, cuda_status):
+    """Gradients over 40 octaves inside a block, so that most moments are below code 1, or zero, at sizes at which squares leave fp32's
+    normal range on either side."""
+    torch.manual_seed(3)
+    g = size * torch.randn(4096) * torch.exp2(-40 * torch.rand(4096))
+    g[::7] = 0.0
+    a, b = M.TensorMoments([4096], "cpu", 8), M.TensorMoments([4096], "cuda", 8)
+    p, q = torch.randn(4096), None
+    q = p.cuda()
+    for t in (1, 2, 3):
+        rng = torch.tensor([t * 12345678901])
+        a.step([p], [g], _hyper(t, gs=1.0, most=0.0), rng=rng)
+        b.step([q], [g.cuda()], _hyper(t, gs=1.0, most=0.0, device="cuda"), rng=rng.cuda())
+        assert torch.equal(a.scales, b.scales.cpu()) and torch.equal(a.m, b.m.cpu()) and torch.equal(a.v, b.v.cpu())
+
+
+@pytest.mark.gpu
 def test_more_tensors_than_a_launch_takes(cuda_status):
     shapes = [(1 + 37 * i % 900,) for i in range(301)]
     _same(*_both(shapes, F32, F32, 8, steps=1), F32)
