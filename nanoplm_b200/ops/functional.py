@@ -419,7 +419,7 @@ class _SandwichFn(torch.autograd.Function):
         for p, want in zip(ctx.refs, wanted):
             running = want and _has_main_grad(p) and p.main_grad.dtype == torch.float32 and p.main_grad.is_contiguous()
             add.append(running)
-            sums.append(None if not want else p.main_grad if running else torch.empty(p.shape, dtype=p.dtype, device=p.device))
+            sums.append(None if not want else p.main_grad if running else K._like(p))
         dx, df, dg = K.sandwich_bwd(rows(dy), rows(dh), x, f, stats, post, nxt, gate, scale, rms, sigmoid, sums, add)
         dnext, dpost, dscale, dgate = (None if a else s for s, a in zip(sums, add))
         if dg is not None:
