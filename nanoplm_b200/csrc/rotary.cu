@@ -16,6 +16,7 @@
 namespace nplm {
 
 constexpr int ROT_THREADS = 256;
+constexpr int ROT_STAGED = 32 * 1024;   // shared memory of a block that turns pairs there
 constexpr int ROT_PAIRS = 2048;     // cos and sin of a block's tokens: 16 KB
 // Items that a thread has in flight.
 __host__ __device__ constexpr int rot_unroll(int bytes) { return bytes >= 16 ? 2 : 4; }
@@ -92,6 +93,28 @@ struct RotVec {
   }
 };
 
+// cos and sin (times factor and sign) of the block's tokens: [tokens][half].
+__device__ __forceinline__ void rotary_angles(const RotaryArgs& a, long long t0, int tokens, int half, float* sm_cos, float* sm_sin) {
+  for (int j = threadIdx.x; j < tokens * half; j += ROT_THREADS) {
+    const int tk = j / half, p2 = j - tk * half;
+    const long long t = t0 + tk;
+    long long b = 0, s = t;
+    if (a.seq != a.tokens) {
+      b = t / a.seq;
+      s = t - b * a.seq;
+    }
+    const long long from = b * a.pb + s * a.pt;
+    const double p = a.pos64 ? static_cast<double>(static_cast<const long long*>(a.pos)[from])
+                             : static_cast<double>(static_cast<const int*>(a.pos)[from]);
+    const double turns = p * (a.freq[p2] * 0.15915494309189535);   // 1 / (2 pi)
+    const float rest = static_cast<float>(turns - rint(turns));
+    float sn, cs;
+    sincospif(2.f * rest, &sn, &cs);
+    sm_cos[j] = a.factor * cs;
+    sm_sin[j] = a.factor * a.sign * sn;
+  }
+}
+
 // VE: elements an access, a divisor of R / 2, of D - R and of all strides, with the addresses on its multiples. A thread's
 // item is VE pairs of a head (two accesses) or up to 2 VE channels behind the rotated ones. Its place in the head stays the
 // same, so that only token and head advance from item to item.
@@ -154,24 +177,7 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     }
   };
   load();     // on its way while cos and sin are formed
-  for (int j = threadIdx.x; j < tokens * half; j += ROT_THREADS) {
-    const int tk = j / half, p2 = j - tk * half;
-    const long long t = t0 + tk;
-    long long b = 0, s = t;
-    if (a.seq != a.tokens) {
-      b = t / a.seq;
-      s = t - b * a.seq;
-    }
-    const long long from = b * a.pb + s * a.pt;
-    const double p = a.pos64 ? static_cast<double>(static_cast<const long long*>(a.pos)[from])
-                             : static_cast<double>(static_cast<const int*>(a.pos)[from]);
-    const double turns = p * (a.freq[p2] * 0.15915494309189535);   // 1 / (2 pi)
-    const float rest = static_cast<float>(turns - rint(turns));
-    float sn, cs;
-    sincospif(2.f * rest, &sn, &cs);
-    sm_cos[j] = a.factor * cs;
-    sm_sin[j] = a.factor * a.sign * sn;
-  }
+  rotary_angles(a, t0, tokens, half, sm_cos, sm_sin);
   __syncthreads();
   while (true) {
 #pragma unroll
@@ -224,6 +230,72 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     if (row >= rows) break;
     load();
   }
+}
+
+// The same for pairs that lie on no 16 bytes while whole heads do: a head moves in pieces of 16 bytes through shared memory, and
+// the pairs are turned there. Accesses of 2 or 4 bytes to global memory leave too little in flight. Forward and backward in us, so /
+// staged: bf16, 100 000 tokens x 8 heads of 64, 50 turn 264 / 171 (floor 64); 30 000 x 16 of 128, 30 turn, interleaved 289 / 125 (76);
+// fp32, 30 000 x 16 of 80, 42 turn 247 / 153 (95). With accesses of 8 bytes it does not pay: bf16, 60 000 x 16 of 80, 40 turn 147 / 199.
+// Shared memory: [rows][D] values, then cos and sin.
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(ROT_THREADS, 4)
+rotary_staged_kernel(const __grid_constant__ RotaryArgs a) {
+  extern __shared__ __align__(16) uint8_t rot_smem[];
+  grid_chain();
+  const int half = a.R >> 1, heads = a.heads[0] + a.heads[1];
+  const long long t0 = static_cast<long long>(blockIdx.x) * a.tile;
+  const int tokens = static_cast<int>(min(static_cast<long long>(a.tile), a.tokens - t0));
+  const int rows = tokens * heads, pieces = a.D * static_cast<int>(sizeof(T)) / 16;
+  T* values = reinterpret_cast<T*>(rot_smem);
+  float* sm_cos = reinterpret_cast<float*>(rot_smem + static_cast<size_t>(a.tile) * heads * a.D * sizeof(T));
+  float* sm_sin = sm_cos + a.tile * half;
+  const int stride = ROT_THREADS / pieces, first = threadIdx.x / pieces, piece = threadIdx.x - first * pieces;
+  auto place = [&](int row, const long long (&sb)[2], const long long (&st)[2], const long long (&sh)[2], const void* const* base) {
+    const int tok = row / heads, h = row - tok * heads, k = h >= a.heads[0];
+    const long long t = t0 + tok;
+    long long b = 0, s = t;
+    if (a.seq != a.tokens) {
+      b = t / a.seq;
+      s = t - b * a.seq;
+    }
+    return static_cast<const T*>(base[k]) + b * sb[k] + s * st[k] + (h - (k ? a.heads[0] : 0)) * sh[k];
+  };
+  if (first < stride) {
+    for (int row = first; row < rows; row += stride) {
+      const T* from = place(row, a.xb, a.xt, a.xh, a.x);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(values + row * a.D) + piece * 16),
+                   "l"(reinterpret_cast<const char*>(from) + piece * 16)
+                   : "memory");
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  rotary_angles(a, t0, tokens, half, sm_cos, sm_sin);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  // all pairs of all rows: pair after pair of a row, row after row
+  for (int j = threadIdx.x; j < rows * half; j += ROT_THREADS) {
+    const int row = j / half, i = j - row * half, at = row / heads * half + i;
+    T* x = values + row * a.D;
+    const int j0 = INTER ? 2 * i : i, j1 = INTER ? 2 * i + 1 : i + half;
+    const float x1 = static_cast<float>(x[j0]), x2 = static_cast<float>(x[j1]), co = sm_cos[at], sn = sm_sin[at];
+    x[j0] = static_cast<T>(x1 * co - x2 * sn);      // (to the nearest)
+    x[j1] = static_cast<T>(x2 * co + x1 * sn);
+  }
+  __syncthreads();
+  if (first < stride) {
+    for (int row = first; row < rows; row += stride) {
+      T* to = const_cast<T*>(place(row, a.yb, a.yt, a.yh, a.y));
+      *reinterpret_cast<uint4*>(reinterpret_cast<char*>(to) + piece * 16) =
+          *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(values + row * a.D) + piece * 16);
+    }
+  }
+}
+
+template <typename T>
+static cudaError_t launch_staged(const RotaryArgs& a, int interleaved, unsigned blocks, size_t smem, cudaStream_t st) {
+  const bool chained = a.tokens * (a.heads[0] + a.heads[1]) * a.D <= CHAIN_ELEMENTS;
+  return interleaved ? launch_when(chained, rotary_staged_kernel<T, true>, blocks, ROT_THREADS, smem, st, a)
+                     : launch_when(chained, rotary_staged_kernel<T, false>, blocks, ROT_THREADS, smem, st, a);
 }
 
 template <typename T, int VE>
@@ -295,11 +367,30 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
     return true;
   };
   while (ve > 1 && !fits(ve)) ve /= 2;
-  const int half = R / 2;
-  const int per_token = (q_heads + k_heads) * (half / ve + (a.in_place ? 0 : (D - R + 2 * ve - 1) / (2 * ve)));
+  const int half = R / 2, heads = q_heads + k_heads;
+  bool whole = D * size % 16 == 0;       // heads on 16 bytes
+  for (int j = 0; j < (k_heads ? 2 : 1); ++j) {
+    const long long all = a.xb[j] | a.xt[j] | a.xh[j] | a.yb[j] | a.yt[j] | a.yh[j];
+    whole &= all * size % 16 == 0 && reinterpret_cast<uintptr_t>(a.x[j]) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y[j]) % 16 == 0;
+  }
+  const int token_bytes = heads * D * size + 2 * half * 4;       // values, cos and sin
+  if (ve * size <= 4 && whole && token_bytes <= ROT_STAGED) {
+    const long long even = (a.tokens + 147) / 148;      // (few tokens: over all multiprocessors)
+    a.tile = ROT_STAGED / token_bytes;
+    if (a.tile > even) a.tile = static_cast<int>(even);
+    const long long blocks = (a.tokens + a.tile - 1) / a.tile;
+    if (blocks > 0x7fffffffLL) return -2;
+    const size_t smem = static_cast<size_t>(a.tile) * token_bytes;
+    const unsigned n = static_cast<unsigned>(blocks);
+    const cudaError_t e = dtype == 0   ? launch_staged<__nv_bfloat16>(a, c.interleaved, n, smem, st)
+                          : dtype == 1 ? launch_staged<__half>(a, c.interleaved, n, smem, st)
+                                       : launch_staged<float>(a, c.interleaved, n, smem, st);
+    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+  }
+  const int per_token = heads * (half / ve + (a.in_place ? 0 : (D - R + 2 * ve - 1) / (2 * ve)));
   // as many tokens as the unrolled items of all threads, at least one, as long as their cos and sin fit
-  const int per_head = per_token / (q_heads + k_heads);
-  int tile = ROT_THREADS / per_head * rot_unroll(ve * size) / (q_heads + k_heads);
+  const int per_head = per_token / heads;
+  int tile = ROT_THREADS / per_head * rot_unroll(ve * size) / heads;
   if (tile > ROT_PAIRS / half) tile = ROT_PAIRS / half;
   if (tile < 1) tile = 1;
   a.tile = tile;

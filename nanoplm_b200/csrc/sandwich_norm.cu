@@ -91,9 +91,10 @@ __device__ __forceinline__ uint32_t sw_pack(float2 v, __half) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// How a row lies in a group's threads. STRIDED: any width, addresses and strides, a thread has every tpr-th channel. ALIGNED: widths
-// and addresses on 16 bytes, a thread has eight neighbouring channels, or none. FULL: the same, and no thread has none.
-enum : int { STRIDED = 0, ALIGNED = 1, FULL = 2 };
+// How a row lies in a group's threads, eight channels a thread. STRIDED: any width, addresses and strides, single channels tpr apart.
+// PAIRED: 16-bit rows on 4 bytes, neighbouring pairs tpr apart. ALIGNED: widths and addresses on 16 bytes, eight neighbours, or
+// none. FULL: the same, and no thread has none.
+enum : int { STRIDED = 0, ALIGNED = 1, FULL = 2, PAIRED = 3 };
 
 template <typename T, int MODE>
 struct Place {
@@ -104,58 +105,66 @@ struct Place {
     lane = threadIdx.x - group * tpr;
     any = MODE == FULL || channel(0) < C;
   }
-  __device__ __forceinline__ int channel(int e) const { return MODE != STRIDED ? lane * 8 + e : e * tpr + lane; }
-  __device__ __forceinline__ bool on(int e) const { return MODE == FULL ? true : MODE == ALIGNED ? any : channel(e) < C; }
+  __device__ __forceinline__ int channel(int e) const {
+    return MODE == STRIDED ? e * tpr + lane : MODE == PAIRED ? 2 * ((e >> 1) * tpr + lane) + (e & 1) : lane * 8 + e;
+  }
+  __device__ __forceinline__ bool on(int e) const {
+    return MODE == FULL ? true : MODE == ALIGNED ? any : channel(e) < C;
+  }
   // the slot of a [C] table in shared memory: two halves of four channels a thread, so that a warp's 16-byte reads are
   // consecutive
   __device__ __forceinline__ int slot(int e) const { return (e >> 2) * tpr * 4 + lane * 4 + (e & 3); }
   // The thread's channels of a row; `mine` is where its first one lies.
   __device__ __forceinline__ Eight load(const T* mine) const {
     Eight v;
-    if (MODE != STRIDED) {
-      if (MODE == FULL || any) {
-        if constexpr (sizeof(T) == 2) {
-          const uint4 u = *reinterpret_cast<const uint4*>(mine);
-          v.p[0] = sw_unpack(u.x, T());
-          v.p[1] = sw_unpack(u.y, T());
-          v.p[2] = sw_unpack(u.z, T());
-          v.p[3] = sw_unpack(u.w, T());
-        } else {
-          const float4 a = *reinterpret_cast<const float4*>(mine), b = *reinterpret_cast<const float4*>(mine + 4);
-          v.p[0] = make_float2(a.x, a.y);
-          v.p[1] = make_float2(a.z, a.w);
-          v.p[2] = make_float2(b.x, b.y);
-          v.p[3] = make_float2(b.z, b.w);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v.p[k] = sw_both(0.f);
-      }
-    } else {
+    if constexpr (MODE == STRIDED) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         v.p[k].x = on(2 * k) ? Io<T>::get(mine[2 * k * tpr]) : 0.f;
         v.p[k].y = on(2 * k + 1) ? Io<T>::get(mine[(2 * k + 1) * tpr]) : 0.f;
       }
+    } else if constexpr (MODE == PAIRED) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v.p[k] = on(2 * k) ? sw_unpack(*reinterpret_cast<const uint32_t*>(mine + 2 * k * tpr), T()) : sw_both(0.f);
+    } else if (MODE == FULL || any) {
+      if constexpr (sizeof(T) == 2) {
+        const uint4 u = *reinterpret_cast<const uint4*>(mine);
+        v.p[0] = sw_unpack(u.x, T());
+        v.p[1] = sw_unpack(u.y, T());
+        v.p[2] = sw_unpack(u.z, T());
+        v.p[3] = sw_unpack(u.w, T());
+      } else {
+        const float4 a = *reinterpret_cast<const float4*>(mine), b = *reinterpret_cast<const float4*>(mine + 4);
+        v.p[0] = make_float2(a.x, a.y);
+        v.p[1] = make_float2(a.z, a.w);
+        v.p[2] = make_float2(b.x, b.y);
+        v.p[3] = make_float2(b.z, b.w);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v.p[k] = sw_both(0.f);
     }
     return v;
   }
   __device__ __forceinline__ void store(T* mine, const Eight& v) const {
-    if (MODE != STRIDED) {
-      if (MODE == FULL || any) {
-        if constexpr (sizeof(T) == 2) {
-          *reinterpret_cast<uint4*>(mine) =
-              make_uint4(sw_pack(v.p[0], T()), sw_pack(v.p[1], T()), sw_pack(v.p[2], T()), sw_pack(v.p[3], T()));
-        } else {
-          *reinterpret_cast<float4*>(mine) = make_float4(v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y);
-          *reinterpret_cast<float4*>(mine + 4) = make_float4(v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y);
-        }
-      }
-    } else {
+    if constexpr (MODE == STRIDED) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (on(2 * k)) mine[2 * k * tpr] = Io<T>::put(v.p[k].x);
         if (on(2 * k + 1)) mine[(2 * k + 1) * tpr] = Io<T>::put(v.p[k].y);
+      }
+    } else if constexpr (MODE == PAIRED) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (on(2 * k)) *reinterpret_cast<uint32_t*>(mine + 2 * k * tpr) = sw_pack(v.p[k], T());
+    } else if (MODE == FULL || any) {
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(mine) =
+            make_uint4(sw_pack(v.p[0], T()), sw_pack(v.p[1], T()), sw_pack(v.p[2], T()), sw_pack(v.p[3], T()));
+      } else {
+        *reinterpret_cast<float4*>(mine) = make_float4(v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y);
+        *reinterpret_cast<float4*>(mine + 4) = make_float4(v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y);
       }
     }
   }
@@ -170,8 +179,8 @@ struct Place {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       r.p[k] = add2(v.p[k], m);
-      if (MODE == STRIDED && !on(2 * k)) r.p[k].x = 0.f;
-      if (MODE == STRIDED && !on(2 * k + 1)) r.p[k].y = 0.f;
+      if ((MODE == STRIDED || MODE == PAIRED) && !on(2 * k)) r.p[k].x = 0.f;
+      if ((MODE == STRIDED || MODE == PAIRED) && !on(2 * k + 1)) r.p[k].y = 0.f;
     }
     return r;
   }
@@ -183,13 +192,17 @@ constexpr bool SW_RING = MODE != STRIDED || sizeof(T) == 4;
 
 template <typename T, int MODE>
 __device__ __forceinline__ void sw_fetch(const Place<T, MODE>& at, uint8_t* to, const T* from) {
-  if (MODE != STRIDED) {
-#pragma unroll
-    for (int j = 0; j < static_cast<int>(8 * sizeof(T)); j += 16) sw_cp_async_16(to + j, reinterpret_cast<const uint8_t*>(from) + j);
-  } else {
+  if constexpr (MODE == STRIDED) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (at.on(e)) sw_cp_async_4(to + e * at.tpr * sizeof(T), from + e * at.tpr);
+  } else if constexpr (MODE == PAIRED) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at.on(2 * k)) sw_cp_async_4(to + 4 * k * at.tpr, from + 2 * k * at.tpr);
+  } else {
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(8 * sizeof(T)); j += 16) sw_cp_async_16(to + j, reinterpret_cast<const uint8_t*>(from) + j);
   }
 }
 
@@ -197,10 +210,20 @@ __device__ __forceinline__ void sw_fetch(const Place<T, MODE>& at, uint8_t* to, 
 // either number to half of the lanes, which then add it up in four; the warps' sums meet in slots: [2][2][16] of the group,
 // the ones behind the last warp zero. The barrier of one sum keeps the slots of the one before it from being
 // overwritten too early, so two sets are enough.
+//
+// SUB: several groups a warp, threads (a power of two) lanes each; all of the warp's lanes take part.
+template <bool SUB>
 struct GroupSum {
   float* slots;
   int warps, warp, bar, threads, phase;
   __device__ __forceinline__ void two(float& a, float& b) {
+    if (SUB) {
+      for (int o = threads >> 1; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+      }
+      return;
+    }
     const int lane = threadIdx.x & 31;
     const bool high = lane & 16;
     const float keep = high ? b : a, give = high ? a : b;
@@ -233,7 +256,9 @@ __device__ __forceinline__ float sw_param(const void* p, int c, int param32) {
   return param32 ? static_cast<const float*>(p)[c] : Io<T>::get(static_cast<const T*>(p)[c]);
 }
 
-// Shared memory: tables post, next, scale, gate [4][tpr * 8] fp32 | sums [groups][2][2][16] | ring [groups][stages][rows][parts][C]
+// Shared memory: tables post, next, scale, gate [4][tpr * 8] fp32 | sums [groups][2][2][16] where a row has several warps | ring [groups][stages][rows][parts][C]
+__host__ __device__ constexpr int sw_sums(int tpr, int groups) { return tpr > 32 ? groups * 64 : 0; }
+
 template <typename T, int MODE>
 __device__ __forceinline__ void sw_tables(const SandwichArgs& a, const Place<T, MODE>& at, float* tables, float* sums) {
   const int wide = a.tpr * 8;
@@ -247,7 +272,7 @@ __device__ __forceinline__ void sw_tables(const SandwichArgs& a, const Place<T, 
       tables[k * wide + at.slot(e)] = c < a.C ? sw_param<T>(of[k], c, a.param32) : 0.f;
     }
   }
-  for (int i = threadIdx.x; i < a.groups * 64; i += blockDim.x) sums[i] = 0.f;
+  for (int i = threadIdx.x; i < sw_sums(a.tpr, a.groups); i += blockDim.x) sums[i] = 0.f;
   __syncthreads();
 }
 
@@ -294,7 +319,7 @@ __device__ __forceinline__ Eight sw_add(const Eight& a, const Eight& b) {
 constexpr int GATE_ANY = -1;
 
 // Two rows at a time: their sums share the exchanges and barriers, and the tables are read once for both.
-template <typename T, int MODE, int GATE>
+template <typename T, int MODE, int GATE, bool SUB>
 __global__ void __maxnreg__(MODE == STRIDED ? 128 : 80)
 sandwich_fwd_kernel(const __grid_constant__ SandwichArgs a) {
   extern __shared__ __align__(128) uint8_t sw_smem[];
@@ -302,12 +327,12 @@ sandwich_fwd_kernel(const __grid_constant__ SandwichArgs a) {
   float* tables = reinterpret_cast<float*>(sw_smem);
   const int wide = a.tpr * 8;
   float* sums = tables + 4 * wide;
-  GroupSum sum{sums + at.group * 64, a.tpr >> 5, at.lane >> 5, 1 + at.group, a.tpr, 0};
+  GroupSum<SUB> sum{sums + (SUB ? 0 : at.group * 64), a.tpr >> 5, at.lane >> 5, 1 + at.group, a.tpr, 0};
   const int gate_mode = GATE == GATE_ANY ? a.gate_mode : GATE == GATE_NONE ? (a.gate_mode ? GATE_CHANNEL : GATE_NONE) : GATE;
   const bool token_gate = GATE == GATE_ANY ? gate_mode >= GATE_TOKEN : GATE >= GATE_TOKEN;
   const uint32_t row_bytes = static_cast<uint32_t>(a.C) * sizeof(T), parts = token_gate ? 3 : 2;
   const uint32_t step_bytes = 2 * parts * row_bytes;      // two rows of all parts
-  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + a.groups * 64) + at.group * a.stages * step_bytes + at.channel(0) * sizeof(T);
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + sw_sums(a.tpr, a.groups)) + at.group * a.stages * step_bytes + at.channel(0) * sizeof(T);
   grid_chain();
   const long long row0 = static_cast<long long>(blockIdx.x) * a.groups + at.group;
   const long long stride = static_cast<long long>(gridDim.x) * a.groups;
@@ -341,8 +366,10 @@ sandwich_fwd_kernel(const __grid_constant__ SandwichArgs a) {
   sw_tables<T, MODE>(a, at, tables, sums);
   const float inv_c = 1.f / a.C;
   uint32_t stage = 0;
-  for (long long row = row0; row < a.T; row += 2 * stride) {
-    const bool two = row + stride < a.T;     // (a second row that is not there holds what the memory did, and is not stored)
+  const int behind = SUB ? (threadIdx.x & 31) / a.tpr : 0;      // groups of the warp before this one, whose rows come first
+  for (long long row = row0; row - behind < a.T; row += 2 * stride) {
+    // (a row that is not there holds what the memory did, and is not stored)
+    const bool live = !SUB || row < a.T, two = row + stride < a.T;
     const T *px[2], *pf[2], *pg[2];
     if (SW_RING<T, MODE>) {
       const uint8_t* s = ring + stage * step_bytes;
@@ -355,12 +382,12 @@ sandwich_fwd_kernel(const __grid_constant__ SandwichArgs a) {
       if (a.stages > 1) sw_cp_wait<1>();
       else sw_cp_wait<0>();
     } else {
-      px[0] = x;
-      pf[0] = f;
-      pg[0] = gate;
-      px[1] = two ? x + dx : x;
-      pf[1] = two ? f + df : f;
-      pg[1] = two ? gate + dg : gate;
+      px[0] = live ? x : static_cast<const T*>(a.x) + at.channel(0);
+      pf[0] = live ? f : static_cast<const T*>(a.f) + at.channel(0);
+      pg[0] = live || !token_gate ? gate : static_cast<const T*>(a.gate) + at.channel(0);
+      px[1] = two ? x + dx : px[0];
+      pf[1] = two ? f + df : pf[0];
+      pg[1] = two ? gate + dg : pg[0];
     }
     // norm of the block's output
     Eight v[2];
@@ -408,7 +435,7 @@ sandwich_fwd_kernel(const __grid_constant__ SandwichArgs a) {
       v[0] = sw_add(at.load(px[0]), v[0]);
       v[1] = sw_add(at.load(px[1]), v[1]);
     }
-    at.store(y, v[0]);
+    if (live) at.store(y, v[0]);
     if (two) at.store(y + dy, v[1]);
     y += 2 * dy;
     if (SW_RING<T, MODE>) {
@@ -440,18 +467,18 @@ sandwich_fwd_kernel(const __grid_constant__ SandwichArgs a) {
         rstd_y[k] = rsqrtf(fmaf(rstd_y[k], inv_c, a.eps));
         v[k] = sw_mul(sw_scaled(v[k], rstd_y[k]), w);
       }
-      at.store(h, v[0]);
+      if (live) at.store(h, v[0]);
       if (two) at.store(h + dy, v[1]);
       h += 2 * dy;
     }
-    if (a.stats != nullptr && at.lane == 0) {
+    if (a.stats != nullptr && at.lane == 0 && live) {
       a.stats[row] = make_float4(mean_f[0], rstd_f[0], mean_y[0], rstd_y[0]);
       if (two) a.stats[row + stride] = make_float4(mean_f[1], rstd_f[1], mean_y[1], rstd_y[1]);
     }
   }
 }
 
-template <typename T, int MODE, int GATE>
+template <typename T, int MODE, int GATE, bool SUB>
 __global__ void __launch_bounds__(512)
 sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
   extern __shared__ __align__(128) uint8_t sw_smem[];
@@ -459,14 +486,14 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
   float* tables = reinterpret_cast<float*>(sw_smem);
   const int wide = a.tpr * 8;
   float* sums = tables + 4 * wide;
-  GroupSum sum{sums + at.group * 64, a.tpr >> 5, at.lane >> 5, 1 + at.group, a.tpr, 0};
+  GroupSum<SUB> sum{sums + (SUB ? 0 : at.group * 64), a.tpr >> 5, at.lane >> 5, 1 + at.group, a.tpr, 0};
   const int gate_mode = GATE == GATE_ANY ? a.gate_mode : GATE;      // (none and a weight are the same: the table has the ones)
   const bool token_gate = gate_mode >= GATE_TOKEN;
   const bool has_dy = a.dy != nullptr, has_dh = a.dh != nullptr;
   const uint32_t row_bytes = static_cast<uint32_t>(a.C) * sizeof(T);
   const uint32_t o_dy = 2 * row_bytes, o_dh = o_dy + has_dy * row_bytes, o_g = o_dh + has_dh * row_bytes;
   const uint32_t step_bytes = o_g + token_gate * row_bytes;
-  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + a.groups * 64) + at.group * a.stages * step_bytes + at.channel(0) * sizeof(T);
+  uint8_t* ring = reinterpret_cast<uint8_t*>(sums + sw_sums(a.tpr, a.groups)) + at.group * a.stages * step_bytes + at.channel(0) * sizeof(T);
   grid_chain();
   const long long row0 = static_cast<long long>(blockIdx.x) * a.groups + at.group;
   const long long stride = static_cast<long long>(gridDim.x) * a.groups;
@@ -512,7 +539,9 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
   uint32_t stage = 0;
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);      // statistics of the next row
   if (row0 < a.T) st = a.stats[row0];
-  for (long long row = row0; row < a.T; row += stride) {
+  const int behind = SUB ? (threadIdx.x & 31) / a.tpr : 0;
+  for (long long row = row0; row - behind < a.T; row += stride) {
+    const bool live = !SUB || row < a.T;
     const float mean_f = st.x, rstd_f = st.y, mean_y = st.z, rstd_y = st.w;
     if (row + stride < a.T) st = a.stats[row + stride];
     const T *px, *pf, *pdy, *pdh, *pg;
@@ -526,11 +555,11 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
       if (a.stages > 1) sw_cp_wait<1>();
       else sw_cp_wait<0>();
     } else {
-      px = x;
-      pf = f;
-      pdy = dy;
-      pdh = dh;
-      pg = gate;
+      px = live ? x : static_cast<const T*>(a.x) + c0;
+      pf = live ? f : static_cast<const T*>(a.f) + c0;
+      pdy = live || !has_dy ? dy : static_cast<const T*>(a.dy) + c0;
+      pdh = live || !has_dh ? dh : static_cast<const T*>(a.dh) + c0;
+      pg = live || !token_gate ? gate : static_cast<const T*>(a.gate) + c0;
     }
     const Eight uf = sw_scaled(at.centred(at.load(pf), mean_f), rstd_f);       // u(f)
     Eight g, t;
@@ -545,7 +574,7 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
       uy = sw_fma(at.table(tables + 2 * wide), at.load(px), uy);
       uy = sw_scaled(at.centred(uy, mean_y), rstd_y);
       const Eight d = at.load(pdh);
-      acc[0] = sw_fma(d, uy, acc[0]);
+      if (live) acc[0] = sw_fma(d, uy, acc[0]);
       t = sw_mul(d, at.table(tables + wide));
       float s1 = sw_total(t), s2 = sw_dot(t, uy);
       sum.two(s1, s2);
@@ -558,8 +587,8 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
       t = at.load(pdy);
     }
     {   // dx, and the sum for the residual scale
-      acc[2] = sw_fma(t, at.load(px), acc[2]);
-      at.store(static_cast<T*>(a.dx) + out, sw_mul(t, at.table(tables + 2 * wide)));
+      if (live) acc[2] = sw_fma(t, at.load(px), acc[2]);
+      if (live) at.store(static_cast<T*>(a.dx) + out, sw_mul(t, at.table(tables + 2 * wide)));
     }
     const Eight w = at.table(tables);
     const Eight tn = sw_mul(t, sw_mul(uf, w));      // t n
@@ -571,15 +600,15 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
           const float2 slope = fma2(make_float2(-g.p[k].x, -g.p[k].y), g.p[k], g.p[k]);
           o.p[k] = mul2(tn.p[k], slope);
         }
-        at.store(static_cast<T*>(a.dg) + out, o);
+        if (live) at.store(static_cast<T*>(a.dg) + out, o);
       } else {
-        at.store(static_cast<T*>(a.dg) + out, tn);
+        if (live) at.store(static_cast<T*>(a.dg) + out, tn);
       }
     } else {
-      acc[3] = sw_add(acc[3], tn);
+      if (live) acc[3] = sw_add(acc[3], tn);
     }
     t = sw_mul(t, g);
-    acc[1] = sw_fma(t, uf, acc[1]);
+    if (live) acc[1] = sw_fma(t, uf, acc[1]);
     t = sw_mul(t, w);
     float s1 = sw_total(t), s2 = sw_dot(t, uf);
     sum.two(s1, s2);
@@ -587,7 +616,7 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
     s2 *= -inv_c * rstd_f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) t.p[k] = fma2(uf.p[k], sw_both(s2), fma2(t.p[k], sw_both(rstd_f), sw_both(s1)));
-    at.store(static_cast<T*>(a.df) + out, t);
+    if (live) at.store(static_cast<T*>(a.df) + out, t);
     out += nout;
     if (SW_RING<T, MODE>) {
       fetch(stage);
@@ -603,9 +632,20 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
   for (int k = 0; k < 4; ++k) {
     if (!(a.want >> k & 1)) continue;
     float* out = a.partial + (static_cast<size_t>(k) * gridDim.x + blockIdx.x) * a.C;
-    for (int j = 0; j < a.groups; ++j) {
+    if (SUB) {        // a warp's groups first
+      for (int o = a.tpr; o < 32; o <<= 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[k].p[e].x += __shfl_xor_sync(0xffffffffu, acc[k].p[e].x, o);
+          acc[k].p[e].y += __shfl_xor_sync(0xffffffffu, acc[k].p[e].y, o);
+        }
+      }
+    }
+    const int members = SUB ? static_cast<int>(blockDim.x) >> 5 : a.groups;
+    const int me = SUB ? (behind == 0 ? static_cast<int>(threadIdx.x) >> 5 : -1) : at.group;
+    for (int j = 0; j < members; ++j) {
       __syncthreads();
-      if (at.group == j) {
+      if (me == j) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int q = at.slot(e);
@@ -663,12 +703,15 @@ sandwich_columns_kernel(const float* __restrict__ partial, const __grid_constant
 // are spread over all multiprocessors.
 static int sw_shape(SandwichArgs& a, bool backward, int mode, unsigned* blocks) {
   if (a.C < 1 || a.C > SW_MAX_C) return -3;
-  a.tpr = ((a.C + 7) / 8 + 31) / 32 * 32;
+  const int threads = (a.C + 7) / 8;
+  a.tpr = (threads + 31) / 32 * 32;
+  while (a.tpr / 2 >= threads && a.tpr <= 32 && a.tpr > 1) a.tpr /= 2;      // up to 128 channels: several rows a warp
   const bool wide = !backward && mode != STRIDED;
   const int most = wide ? 384 : 512;
   a.groups = a.tpr > most ? 1 : most / a.tpr;
   const long long spread = (a.T + 147) / 148;
   if (a.groups > spread) a.groups = static_cast<int>(spread < 1 ? 1 : spread);
+  if (a.tpr < 32) a.groups = (a.groups + 32 / a.tpr - 1) / (32 / a.tpr) * (32 / a.tpr);      // whole warps
   int per_sm = (wide ? 768 : 512) / (a.tpr * a.groups);
   if (per_sm < 1) per_sm = 1;
   const long long all = (a.T + a.groups - 1) / a.groups, room = 148LL * per_sm;
@@ -677,13 +720,13 @@ static int sw_shape(SandwichArgs& a, bool backward, int mode, unsigned* blocks) 
 }
 
 static size_t sw_smem_bytes(const SandwichArgs& a, int rows, int parts, int size, bool ring) {
-  return static_cast<size_t>(a.tpr) * 8 * 4 * 4 + static_cast<size_t>(a.groups) * 64 * 4 +
+  return static_cast<size_t>(a.tpr) * 8 * 4 * 4 + static_cast<size_t>(sw_sums(a.tpr, a.groups)) * 4 +
          (ring ? static_cast<size_t>(a.groups) * a.stages * rows * parts * a.C * size : 0);
 }
 
-template <typename T, int MODE, int GATE>
+template <typename T, int MODE, int GATE, bool SUB>
 static int sw_launch(const SandwichArgs& a, bool backward, unsigned blocks, size_t smem, cudaStream_t st) {
-  auto kern = backward ? sandwich_bwd_kernel<T, MODE, GATE> : sandwich_fwd_kernel<T, MODE, GATE>;
+  auto kern = backward ? sandwich_bwd_kernel<T, MODE, GATE, SUB> : sandwich_fwd_kernel<T, MODE, GATE, SUB>;
   static bool configured_on[2][MAX_DEVICES];
   const int dev = current_device_slot();
   if (dev < 0) return -4;
@@ -696,27 +739,42 @@ static int sw_launch(const SandwichArgs& a, bool backward, unsigned blocks, size
   return static_cast<int>(cudaGetLastError());
 }
 
+template <typename T, int MODE>
+static int sw_launch(const SandwichArgs& a, bool backward, unsigned blocks, size_t smem, cudaStream_t st) {
+  return a.tpr < 32 ? sw_launch<T, MODE, GATE_ANY, true>(a, backward, blocks, smem, st)
+                    : sw_launch<T, MODE, GATE_ANY, false>(a, backward, blocks, smem, st);
+}
+
 template <typename T>
 static int sw_launch(const SandwichArgs& a, bool backward, int mode, unsigned blocks, size_t smem, cudaStream_t st) {
-  if (mode == STRIDED) return sw_launch<T, STRIDED, GATE_ANY>(a, backward, blocks, smem, st);
-  if (mode == ALIGNED) return sw_launch<T, ALIGNED, GATE_ANY>(a, backward, blocks, smem, st);
-  if (a.gate_mode == GATE_SIGMOID) return sw_launch<T, FULL, GATE_SIGMOID>(a, backward, blocks, smem, st);
-  if (a.gate_mode == GATE_TOKEN) return sw_launch<T, FULL, GATE_TOKEN>(a, backward, blocks, smem, st);
-  return sw_launch<T, FULL, GATE_NONE>(a, backward, blocks, smem, st);
+  if (mode == STRIDED) return sw_launch<T, STRIDED>(a, backward, blocks, smem, st);
+  if (mode == ALIGNED) return sw_launch<T, ALIGNED>(a, backward, blocks, smem, st);
+  if constexpr (sizeof(T) == 2) {
+    if (mode == PAIRED) return sw_launch<T, PAIRED>(a, backward, blocks, smem, st);
+  }
+  if (a.gate_mode == GATE_SIGMOID) return sw_launch<T, FULL, GATE_SIGMOID, false>(a, backward, blocks, smem, st);
+  if (a.gate_mode == GATE_TOKEN) return sw_launch<T, FULL, GATE_TOKEN, false>(a, backward, blocks, smem, st);
+  return sw_launch<T, FULL, GATE_NONE, false>(a, backward, blocks, smem, st);
 }
 
 static int sw_run(SandwichArgs& a, bool backward, int dtype, unsigned* blocks, cudaStream_t st) {
   const int size = dtype == 2 ? 4 : 2;
   const void* rows[] = {a.x, a.f, a.gate_mode >= GATE_TOKEN ? a.gate : nullptr, a.dy, a.dh, a.y, a.h, a.dx, a.df, a.dg};
   const long long strides[] = {a.xs, a.fs, a.gate_mode >= GATE_TOKEN ? a.gs : 0, a.dys, a.dhs};
-  bool aligned = a.C % 8 == 0;
-  for (const void* p : rows) aligned &= reinterpret_cast<uintptr_t>(p) % 16 == 0;
-  for (long long s : strides) aligned &= s * size % 16 == 0;
-  const int mode = !aligned ? STRIDED : a.C % 256 == 0 ? FULL : ALIGNED;
+  bool aligned = a.C % 8 == 0, paired = size == 2 && a.C % 2 == 0;
+  for (const void* p : rows) {
+    aligned &= reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    paired &= reinterpret_cast<uintptr_t>(p) % 4 == 0;
+  }
+  for (long long s : strides) {
+    aligned &= s * size % 16 == 0;
+    paired &= s % 2 == 0;
+  }
+  const int mode = aligned ? (a.C % 256 == 0 ? FULL : ALIGNED) : paired ? PAIRED : STRIDED;
   const int rc = sw_shape(a, backward, mode, blocks);
   if (rc) return rc;
   const int parts = 2 + (a.gate_mode >= GATE_TOKEN) + (a.dy != nullptr) + (a.dh != nullptr);
-  const bool ring = aligned || size == 4;
+  const bool ring = mode != STRIDED || size == 4;
   a.stages = SW_STAGES;
   size_t smem = sw_smem_bytes(a, backward ? 1 : 2, parts, size, ring);
   if (smem > SW_MAX_SMEM) {      // (fp32 rows of more than 3 500 channels with a gate)

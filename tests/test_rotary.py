@@ -25,12 +25,14 @@ def _exact(x, pos, w, factor=1.0, interleaved=False, sign=1.0):
 
 
 def _close(got, x, pos, w, **how):
-    """Within half a step of the type, and the fp32 errors before it: of an angle in turns, 2^-26 from the cast of the part behind
+    """Within half a step of the type, which below its smallest normal number is that number's (fp16: 2^-14 eps / 2 = 2^-25, half of the
+    subnormal numbers' distance 2^-24), and the fp32 errors before it: of an angle in turns, 2^-26 from the cast of the part behind
     the comma and 2^-50 of the turns before it (products of rounded fp64 numbers, here and in the 64-bit form), i.e.
     2 pi times that; of sincospi and factor 2^-22, of the two products and their sum 2^-23."""
     want, size = _exact(x, pos, w, **how)
     turns = float(pos.abs().max()) * float(w.max()) / (2 * math.pi) if pos.numel() else 0.0
-    tol = torch.finfo(got.dtype).eps / 2 * want.abs() + size * (2 * math.pi * (2.0 ** -26 + turns * 2.0 ** -50) + 2.0 ** -21)
+    info = torch.finfo(got.dtype)
+    tol = info.eps / 2 * want.abs().clamp(min=info.smallest_normal) + size * (2 * math.pi * (2.0 ** -26 + turns * 2.0 ** -50) + 2.0 ** -21)
     n = len(w)
     assert torch.equal(got[..., 2 * n:], x[..., 2 * n:])
     assert ((got.double() - want).abs() <= tol + 1e-30).all(), ((got.double() - want).abs() - tol).max()
@@ -103,6 +105,7 @@ def test_refusals():
 SHAPES = [  # tokens, query heads, key heads, width, pairs
     (1, 1, 1, 2, 1), (1, 8, 8, 64, 32), (3, 5, 0, 70, 17), (129, 4, 1, 128, 16), (77, 3, 3, 80, 40), (250, 12, 2, 64, 31),
     (33, 2, 1, 512, 256), (19, 70, 3, 6, 1), (11, 1, 1, 511, 255), (4097, 2, 2, 32, 12),
+    (300, 6, 2, 64, 25), (1, 4, 4, 128, 1), (900, 5, 0, 80, 21), (40, 48, 12, 96, 47), (64, 3, 2, 8, 3),
 ]
 
 

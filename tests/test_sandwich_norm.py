@@ -111,7 +111,8 @@ def test_refusals():
 
 # ------------------------------------------------------------------------------------------- GPU
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,C", [(1, 1), (1, 8), (3, 250), (37, 256), (5, 264), (700, 512), (130, 768), (9, 1111), (1300, 1024),
+@pytest.mark.parametrize("T,C", [(1, 1), (1, 8), (2, 3), (33, 7), (150, 16), (1, 24), (301, 17), (700, 32), (37, 66), (500, 100), (149, 128),
+                                 (3, 250), (37, 256), (5, 264), (700, 512), (130, 768), (9, 1111), (1300, 1024),
                                  (33, 2048), (3, 3001), (5, 4096)])
 @pytest.mark.parametrize("dtype", [BF, F16, F32])
 @pytest.mark.parametrize("gate,sigmoid,scaled", [("none", False, False), ("channel", False, True), ("token", False, False),
