@@ -622,7 +622,7 @@ static int at_launch(const AdamTensors& t, int bits, long long elements, void* m
 
 using namespace nplm;
 
-// n tensors: p, g, copy (a null entry, or copy itself null: none), numel, first block in the moments, decay. p_type, g_type: 0
+// n tensors: p, g, copy (null: none), numel, first block in the moments, decay. p_type, g_type: 0
 // bf16, 2 fp32; copies are bf16. bits 8: m, v uint8 [blocks][256], scales uint8 [2][blocks]; 32: m, v fp32 [blocks][256].
 extern "C" int nplm_adamw_tensors(void* const* p, const void* const* g, void* const* copy, const long long* numel,
                                   const long long* block, const unsigned char* decay, int n, int p_type, int g_type, int bits,

@@ -338,7 +338,7 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
   const RotaryCall& c = *call;
   const int q_heads = c.q_heads, k_heads = c.k_heads, D = c.D, R = c.R, dtype = c.dtype;
   const long long batch = c.batch, seq = c.seq;
-  if (batch < 0 || seq < 0 || q_heads < 1 || k_heads < 0 || D < 2 || D > 512 || R < 2 || R > D || R % 2 || dtype < 0 ||
+  if (batch < 0 || seq < 0 || q_heads < 1 || k_heads < 0 || q_heads > 65536 || k_heads > 65536 || D < 2 || D > 512 || R < 2 || R > D || R % 2 || dtype < 0 ||
       dtype > 2)
     return -1;
   if (batch == 0 || seq == 0) return 0;
@@ -353,7 +353,9 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
   a.pos = c.pos; a.pos64 = c.pos64; a.pb = c.pb; a.pt = c.pt; a.freq = c.freq; a.factor = c.factor;
   a.sign = c.transposed ? -1.f : 1.f;
   a.tokens = batch * seq; a.seq = seq; a.D = D; a.R = R;
-  a.in_place = c.q == c.q_out && (k_heads == 0 || c.k == c.k_out);
+  a.in_place = 1;
+  for (int j = 0; j < (k_heads ? 2 : 1); ++j)
+    a.in_place &= a.x[j] == a.y[j] && a.xb[j] == a.yb[j] && a.xt[j] == a.yt[j] && a.xh[j] == a.yh[j];
   // the widest access, up to 16 bytes, that sizes, strides and addresses allow
   const int size = dtype == 2 ? 4 : 2;
   int ve = 16 / size;
@@ -373,10 +375,10 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
     const long long all = a.xb[j] | a.xt[j] | a.xh[j] | a.yb[j] | a.yt[j] | a.yh[j];
     whole &= all * size % 16 == 0 && reinterpret_cast<uintptr_t>(a.x[j]) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y[j]) % 16 == 0;
   }
-  const int token_bytes = heads * D * size + 2 * half * 4;       // values, cos and sin
+  const long long token_bytes = static_cast<long long>(heads) * D * size + 2 * half * 4;       // values, cos and sin
   if (ve * size <= 4 && whole && token_bytes <= ROT_STAGED) {
     const long long even = (a.tokens + 147) / 148;      // (few tokens: over all multiprocessors)
-    a.tile = ROT_STAGED / token_bytes;
+    a.tile = static_cast<int>(ROT_STAGED / token_bytes);
     if (a.tile > even) a.tile = static_cast<int>(even);
     const long long blocks = (a.tokens + a.tile - 1) / a.tile;
     if (blocks > 0x7fffffffLL) return -2;

@@ -524,8 +524,8 @@ def rotary_frequencies(rotated: int, theta: float, scaling: dict | None = None, 
     scaling {"type": ..., "factor": s > 1} stretches the positions that a model was trained on (`original_max_position`)
     s-fold: "linear" divides every frequency by s; "ntk" raises theta so that the slowest pair turns s times slower and
     the fastest as before; "yarn" (Peng et al., 2023) divides the frequencies of pairs that turn at most `beta_slow` (1) times in
-    the original context, keeps those above `beta_fast` (32) turns, blends between, and multiplies cos and sin by
-    0.1 ln s + 1 (or `attention_factor`)."""
+    the original context, keeps those above `beta_fast` (32) turns, blends between them linearly in the logarithm of the
+    turns, that is in the pair's index, and multiplies cos and sin by 0.1 ln s + 1 (or `attention_factor`)."""
     if rotated < 2 or rotated % 2:
         raise ValueError(f"an even number of channels rotates, got {rotated}")
     at = torch.arange(0, rotated, 2, dtype=torch.float64, device=device) / rotated

@@ -498,8 +498,8 @@ def check_rotary(q, k, positions, frequencies):
         if k.dtype != q.dtype:
             raise ValueError(f"k must be {q.dtype}, got {k.dtype}")
         Hk, ks = kshape[-2], (0, kst[0], kst[1]) if len(shape) == 3 else kst[:3]
-    if H < 1 or (k is not None and Hk < 1):
-        raise ValueError(f"at least one head is needed: got {H} and {Hk}")
+    if not 1 <= H <= 65536 or (k is not None and not 1 <= Hk <= 65536):
+        raise ValueError(f"1 to 65536 heads are taken: got {H} and {Hk}")
     if positions.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
     pshape = positions.shape
@@ -519,7 +519,8 @@ def check_rotary(q, k, positions, frequencies):
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor, factor: float = 1.0,
            interleaved: bool = False, transposed: bool = False, inplace: bool = False, out: tuple | None = None):
     """Rotary positions on q [T, H, D] or [B, S, H, D] and, in the same launch, k with as many tokens, any number of heads and
-    the same width: (q', k'), contiguous, or `out` (tensors like q and k, of any strides), or with `inplace` q and k themselves.
+    the same width: (q', k'), contiguous, or `out` (tensors like q and k, of any strides, that share no memory with each other,
+    nor with q and k unless they are those), or with `inplace` q and k themselves.
 
     bf16, fp16 or fp32; the last dimension contiguous, the others of any stride. positions: int32 or int64, [T], [B, S], or [S]
     for all of a batch. frequencies: fp64 [R / 2], radians a position for each pair of the first R channels of a head; the
@@ -541,6 +542,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     for t in (qo, ko):
         if t is not None and any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
             raise ValueError("what is written has elements that share memory")
+    if qo is not None and ko is not None and qo.data_ptr() == ko.data_ptr() and qo.numel() and ko.numel():
+        raise ValueError("q and k are written to the same memory")
     with _device_of(q, k, positions, frequencies, qo, ko):
         if out is not None:
             heads = lambda t: (0, 0, 0) if t is None else (0, *t.stride()[:2]) if t.dim() == 3 else t.stride()[:3]

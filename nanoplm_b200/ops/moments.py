@@ -124,7 +124,8 @@ class TensorMoments:
                 _step_cpu(params, grads, self.m, self.v, hyper, self.scales, rng, copies, decay, sumsq)
 
     def values(self) -> tuple[list[torch.Tensor], list[torch.Tensor]]:
-        """fp32 first and second moments of every tensor, flat (for checkpoints)."""
+        """fp32 first and second moments of every tensor, flat (for checkpoints). Those of 32 bits are the moments themselves,
+        which the next step changes."""
         if self.bits == 32:
             m, v = self.m, self.v
         elif self.device.type == "cuda":

@@ -134,7 +134,10 @@ def _write_hf_config(ckp: Path, cfg) -> None:
         "global_attn_every_n_layers": cfg.global_attn_every_n_layers, "global_rope_theta": cfg.global_rope_theta,
         "local_rope_theta": cfg.local_rope_theta, "torch_dtype": "float32",
         # what HF's config has no field for (the MLP variant matters to a loader)
-        "nanoplm": {"mlp_activation": cfg.mlp_activation, "norm_type": cfg.norm_type},
+        "nanoplm": {"mlp_activation": cfg.mlp_activation, "norm_type": cfg.norm_type,
+                    **{k: getattr(cfg, k) for k, default in (("rope_scaling", None), ("rotary_fraction", 1.0), ("rope_interleaved", False),
+                                                             ("sandwich_norm", False), ("residual_gate", "none"), ("residual_scale", False))
+                       if getattr(cfg, k, default) != default}},
     }
     (ckp / "config.json").write_text(json.dumps(data, indent=2), encoding="utf-8")
 

@@ -252,6 +252,36 @@ def test_values_and_codes(cuda_status):
 
 
 @pytest.mark.gpu
+def test_tensor_past_32_bit_places(cuda_status):
+    """2^32 + 700 elements: the blocks on both sides of place 2^32 and the last ones against a restatement of theirs alone, the random
+    numbers of their places among it."""
+    n, tail = 2 ** 32 + 700, 256 * 6
+    p, g = torch.zeros(n, dtype=BF, device="cuda"), torch.zeros(n, dtype=BF, device="cuda")
+    st = M.TensorMoments([n], "cuda", 8)
+    first = 2 ** 32 - 256 * 3
+    gen = torch.Generator().manual_seed(1)
+    p[first:] = torch.randn(n - first, generator=gen).to(BF).cuda()
+    g[first:] = torch.randn(n - first, generator=gen).to(BF).cuda()
+    want_p, grad = p[first:].cpu(), g[first:].cpu()
+    rng = torch.tensor([77])
+    st.step([p], [g], _hyper(1, most=0.0, device="cuda"), rng=rng.cuda())
+    m = torch.zeros(tail)
+    m[:n - first] = grad.float() * 0.5 * (1 - _hyper(1)[1])
+    v = torch.zeros(tail)
+    v[:n - first] = (grad.float() * 0.5) ** 2 * (1 - _hyper(1)[2])
+    key = M._mix((rng & M._LOW32) ^ M._mix(rng >> 32))
+    at = torch.arange(first, first + tail)
+    r = M._mix((at & M._LOW32) ^ M._mix((key + (at >> 32)) & M._LOW32))
+    for codes, row, values, bits, signed in ((st.m, 0, m, r & 0xfffff, True), (st.v, 1, v, r >> 12, False)):
+        c, e = M.encode(values, bits, signed)
+        assert torch.equal(codes[first:first + tail].cpu(), c)
+        assert torch.equal(st.scales[row, first // 256:first // 256 + 6].cpu(), e)
+        assert not codes[:first].any()
+    new = want_p.float() * (1 - 0.01 * 0.1) - 0.01 * torch.sign(grad.float())
+    assert ((p[first:].cpu().float() - new).abs() <= 2 ** -8 * new.abs() + 1e-4).all()
+
+
+@pytest.mark.gpu
 def test_no_tensors(cuda_status):
     M.TensorMoments([], "cuda", 8).step([], [], _hyper(1, device="cuda"), rng=torch.tensor([1], device="cuda"))
     m, v = K.moment_values(*(torch.zeros(0, dtype=torch.uint8, device="cuda") for _ in range(2)), torch.zeros(2, 0, dtype=torch.uint8, device="cuda"))

@@ -99,6 +99,11 @@ def test_refusals():
         K.rotary(q[:, :1].expand(5, 2, 8), None, pos, w, inplace=True)
     with pytest.raises(ValueError):
         K.rotary(q.transpose(1, 2), None, pos, w)
+    for out in ((q,), (q[:4], k), (q.double(), k), (q, None)):
+        with pytest.raises(ValueError):
+            K.rotary(q, k, pos, w, out=out if len(out) == 2 else (out[0], k[:, :, :6]))
+    with pytest.raises(ValueError):         # one memory for both
+        K.rotary(q, q, pos, w, inplace=True)
 
 
 # ------------------------------------------------------------------------------------------- GPU
@@ -169,6 +174,27 @@ def test_in_place_leaves_the_rest(cuda_status):
     for got, x in zip(parts(packed), parts(before)):
         _close(got, x, pos, w)
     assert torch.equal(packed[:, (H + Hk) * D:], before[:, (H + Hk) * D:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [24, 25])
+def test_given_outputs_of_other_strides(n, cuda_status):
+    """Outputs inside wider rows, and one that starts where the input does but with other strides."""
+    T, H, D = 70, 3, 64
+    pos, w = torch.arange(T, device="cuda"), _w(n, "cuda")
+    q, k = torch.randn(T, H, D, device="cuda"), torch.randn(T, 1, D, device="cuda")
+    wide = torch.full((T, (H + 2) * D), 7.0, device="cuda")
+    a, b = wide[:, :H * D].view(T, H, D), wide[:, H * D:(H + 1) * D].view(T, 1, D)
+    got = K.rotary(q, k, pos, w, out=(a, b))
+    assert got[0] is a and got[1] is b
+    _close(a, q, pos, w)
+    _close(b, k, pos, w)
+    assert (wide[:, (H + 1) * D:] == 7.0).all()
+    one = torch.randn(1, 2 * D, device="cuda")
+    x, y = one.view(1, 2, D)[:, :1], one.as_strided((1, 1, D), (D, 5 * D, 1))        # one token, one head: the same elements
+    before = x.clone()
+    K.rotary(x, None, pos[:1] + 3, w, out=(y, None))
+    _close(y, before, pos[:1] + 3, w)
 
 
 @pytest.mark.gpu

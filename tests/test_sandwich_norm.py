@@ -248,6 +248,23 @@ def test_captured_passes_do_not_share_their_scratch(cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [256, 40, 33])
+def test_rows_past_32_bit_offsets(C, cuda_status):
+    """Rows 2^30 elements apart in one buffer, outputs and gradients against those of the same rows put together."""
+    big = torch.zeros(3 * 2 ** 30 + C, dtype=BF, device="cuda")
+    far = big.as_strided((4, C), (2 ** 30, 1))
+    far.copy_(torch.randn(4, C))
+    near = far.contiguous()
+    f, dy = torch.randn(4, C, device="cuda").to(BF), torch.randn(4, C, device="cuda").to(BF)
+    a = K.sandwich_fwd(far, f, None, None, gate=far, sigmoid=True)
+    b = K.sandwich_fwd(near, f, None, None, gate=near, sigmoid=True)
+    x = K.sandwich_bwd(far, dy, far, f, a[2], None, None, gate=far, sigmoid=True)
+    y = K.sandwich_bwd(near, dy, near, f, b[2], None, None, gate=near, sigmoid=True)
+    for s, t in zip(a + x, b + y):
+        assert torch.allclose(s.float(), t.float(), rtol=2 ** -7, atol=1e-6)
+
+
+@pytest.mark.gpu
 def test_rows_without_variance_and_large_means(cuda_status):
     """Constant rows are zeros behind a LayerNorm, and a mean a thousand times the deviation costs no more than the cast did."""
     T, C = 6, 384
