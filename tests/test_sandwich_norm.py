@@ -248,6 +248,23 @@ def test_captured_passes_do_not_share_their_scratch(cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,C,width,first", [
+    (BF, 1001, 1005, 2), (F16, 1001, 1005, 1), (BF, 1001, 1004, 0), (BF, 1002, 1006, 2), (F16, 1002, 1007, 0), (BF, 129, 131, 4),
+    (BF, 4095, 4097, 0), (F32, 1001, 1003, 1), (F32, 130, 133, 3), (F32, 17, 21, 1), (F32, 4001, 4003, 2), (BF, 6, 14, 2), (BF, 66, 70, 0)])
+@pytest.mark.parametrize("gate,sigmoid", [("channel", False), ("token", True)])
+def test_rows_beside_numbers_that_are_none(dtype, C, width, first, gate, sigmoid, cuda_status):
+    """Rows of any width, stride and place in wider ones whose other channels are NaN: nothing of them shows in any result. Enough
+    rows that blocks have several groups and groups several steps, an odd number of them."""
+    T = 1501
+    p = _inputs(T, C, dtype, gate, True, True, "cuda")
+    for name in ("x", "f") + (("gate",) if gate == "token" else ()):
+        around = torch.full((T + 2, width), float("nan"), device="cuda", dtype=dtype)
+        rows = around.view(-1)[first:first + T * width].view(T, width)[:, :C]
+        p[name] = rows.copy_(p[name].detach()).requires_grad_(True)
+    _check(p, sigmoid, rms=C % 2 == 0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C", [256, 40, 33])
 def test_rows_past_32_bit_offsets(C, cuda_status):
     """Rows 2^30 elements apart in one buffer, outputs and gradients against those of the same rows put together."""
