@@ -21,6 +21,16 @@ constexpr int ROT_PAIRS = 2048;     // cos and sin of a block's tokens: 16 KB
 // Items that a thread has in flight.
 __host__ __device__ constexpr int rot_unroll(int bytes) { return bytes >= 16 ? 2 : 4; }
 
+// Division of numbers below 2^32 / d by d: a product with 2^32 / d, rounded up, whose excess stays below a 1 / d.
+struct RotDiv {
+  uint32_t m, one;
+  RotDiv() = default;
+  explicit RotDiv(uint32_t d) : m(d > 1 ? static_cast<uint32_t>((0x100000000ull + d - 1) / d) : 0u), one(d == 1) {}
+  __device__ __forceinline__ int of(int j) const {
+    return static_cast<int>(__umulhi(static_cast<uint32_t>(j), m) + static_cast<uint32_t>(j) * one);
+  }
+};
+
 struct RotaryArgs {
   const void* x[2];                 // queries, keys (keys may have no heads)
   void* y[2];
@@ -35,6 +45,10 @@ struct RotaryArgs {
   long long seq;
   int D, R, tile;                   // tile: tokens a block
   int in_place;                     // the channels from R on are there already
+  int near;                         // batches follow one another, and a tile's offsets in a tensor fit in 31 bits
+  int xt32[2], xh32[2], yt32[2], yh32[2];
+  RotDiv by_half, by_heads, by_run; // by_run: pieces of a token
+  int run;                          // bytes of a piece of a run; 0: heads are no runs
 };
 
 // An access as it is moved, and its VE values.
@@ -93,16 +107,51 @@ struct RotVec {
   }
 };
 
+__device__ __forceinline__ void rot_split(const RotaryArgs& a, long long t, long long& b, long long& s) {
+  b = 0;
+  s = t;
+  if (a.seq != a.tokens) {
+    b = a.tokens >> 32 ? t / a.seq : static_cast<uint32_t>(t) / static_cast<uint32_t>(a.seq);
+    s = t - b * a.seq;
+  }
+}
+
+// Where a head of the block's token `tok` lies: by 32-bit offsets from the block's first token where they reach (64-bit products
+// for each of both places were half of the instructions of narrow accesses).
+template <typename T>
+struct RotPlace {
+  const T *x0, *x1;
+  T *y0, *y1;
+  __device__ __forceinline__ RotPlace(const RotaryArgs& a, long long t0) {
+    x0 = static_cast<const T*>(a.x[0]) + t0 * a.xt[0];
+    x1 = static_cast<const T*>(a.x[1]) + t0 * a.xt[1];
+    y0 = static_cast<T*>(a.y[0]) + t0 * a.yt[0];
+    y1 = static_cast<T*>(a.y[1]) + t0 * a.yt[1];
+  }
+  __device__ __forceinline__ const T* from(const RotaryArgs& a, long long t0, int tok, int h) const {
+    const bool k = h >= a.heads[0];
+    const int hh = h - (k ? a.heads[0] : 0);
+    if (a.near) return (k ? x1 : x0) + (tok * (k ? a.xt32[1] : a.xt32[0]) + hh * (k ? a.xh32[1] : a.xh32[0]));
+    long long b, s;
+    rot_split(a, t0 + tok, b, s);
+    return static_cast<const T*>(a.x[k]) + b * a.xb[k] + s * a.xt[k] + hh * a.xh[k];
+  }
+  __device__ __forceinline__ T* to(const RotaryArgs& a, long long t0, int tok, int h) const {
+    const bool k = h >= a.heads[0];
+    const int hh = h - (k ? a.heads[0] : 0);
+    if (a.near) return (k ? y1 : y0) + (tok * (k ? a.yt32[1] : a.yt32[0]) + hh * (k ? a.yh32[1] : a.yh32[0]));
+    long long b, s;
+    rot_split(a, t0 + tok, b, s);
+    return static_cast<T*>(a.y[k]) + b * a.yb[k] + s * a.yt[k] + hh * a.yh[k];
+  }
+};
+
 // cos and sin (times factor and sign) of the block's tokens: [tokens][half].
 __device__ __forceinline__ void rotary_angles(const RotaryArgs& a, long long t0, int tokens, int half, float* sm_cos, float* sm_sin) {
   for (int j = threadIdx.x; j < tokens * half; j += ROT_THREADS) {
-    const int tk = j / half, p2 = j - tk * half;
-    const long long t = t0 + tk;
-    long long b = 0, s = t;
-    if (a.seq != a.tokens) {
-      b = t / a.seq;
-      s = t - b * a.seq;
-    }
+    const int tk = a.by_half.of(j), p2 = j - tk * half;
+    long long b, s;
+    rot_split(a, t0 + tk, b, s);
     const long long from = b * a.pb + s * a.pt;
     const double p = a.pos64 ? static_cast<double>(static_cast<const long long*>(a.pos)[from])
                              : static_cast<double>(static_cast<const int*>(a.pos)[from]);
@@ -113,6 +162,49 @@ __device__ __forceinline__ void rotary_angles(const RotaryArgs& a, long long t0,
     sm_cos[j] = a.factor * cs;
     sm_sin[j] = a.factor * a.sign * sn;
   }
+}
+
+// Two accesses' worth of a head, VE pairs, turned by their cos and sin.
+template <typename T, int VE, bool INTER>
+__device__ __forceinline__ void rot_turn(RotVec<T, VE>& v0, RotVec<T, VE>& v1, const float* cos, const float* sin) {
+  float cs[VE], sn[VE];
+  if constexpr (VE >= 4) {
+#pragma unroll
+    for (int e = 0; e < VE; e += 4) {
+      const float4 cc = *reinterpret_cast<const float4*>(cos + e);
+      const float4 ss = *reinterpret_cast<const float4*>(sin + e);
+      cs[e] = cc.x; cs[e + 1] = cc.y; cs[e + 2] = cc.z; cs[e + 3] = cc.w;
+      sn[e] = ss.x; sn[e + 1] = ss.y; sn[e + 2] = ss.z; sn[e + 3] = ss.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      cs[e] = cos[e];
+      sn[e] = sin[e];
+    }
+  }
+  float x[2 * VE], lo[VE], hi[VE];
+  v0.get(lo);
+  v1.get(hi);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    x[e] = lo[e];
+    x[VE + e] = hi[e];
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {      // the two members of pair e of this item
+    const int j0 = INTER ? 2 * e : e, j1 = INTER ? 2 * e + 1 : VE + e;
+    const float x1 = x[j0], x2 = x[j1];
+    x[j0] = x1 * cs[e] - x2 * sn[e];
+    x[j1] = x2 * cs[e] + x1 * sn[e];
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    lo[e] = x[e];
+    hi[e] = x[VE + e];
+  }
+  v0.set(lo);
+  v1.set(hi);
 }
 
 // VE: elements an access, a divisor of R / 2, of D - R and of all strides, with the addresses on its multiples. A thread's
@@ -157,12 +249,8 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
       if (row < rows) {
         const int k = h >= a.heads[0];
         const int hh = h - (k ? a.heads[0] : 0);
-        const long long t = t0 + tok;
-        long long b = 0, s = t;
-        if (a.seq != a.tokens) {
-          b = t / a.seq;
-          s = t - b * a.seq;
-        }
+        long long b, s;
+        rot_split(a, t0 + tok, b, s);
         const T* from = static_cast<const T*>(a.x[k]) + b * a.xb[k] + s * a.xt[k] + hh * a.xh[k];
         to[u] = static_cast<T*>(a.y[k]) + b * a.yb[k] + s * a.yt[k] + hh * a.yh[k];
         at[u] = tok * half + i;
@@ -186,44 +274,7 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     for (int u = 0; u < ROT_UNROLL; ++u) {
       if (to[u] != nullptr) {
         if (pairs) {
-          float cs[VE], sn[VE];
-          if constexpr (VE >= 4) {
-#pragma unroll
-            for (int e = 0; e < VE; e += 4) {
-              const float4 cc = *reinterpret_cast<const float4*>(sm_cos + at[u] + e);
-              const float4 ss = *reinterpret_cast<const float4*>(sm_sin + at[u] + e);
-              cs[e] = cc.x; cs[e + 1] = cc.y; cs[e + 2] = cc.z; cs[e + 3] = cc.w;
-              sn[e] = ss.x; sn[e + 1] = ss.y; sn[e + 2] = ss.z; sn[e + 3] = ss.w;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              cs[e] = sm_cos[at[u] + e];
-              sn[e] = sm_sin[at[u] + e];
-            }
-          }
-          float x[2 * VE], lo[VE], hi[VE];
-          v0[u].get(lo);
-          v1[u].get(hi);
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            x[e] = lo[e];
-            x[VE + e] = hi[e];
-          }
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {      // the two members of pair e of this item
-            const int j0 = INTER ? 2 * e : e, j1 = INTER ? 2 * e + 1 : VE + e;
-            const float x1 = x[j0], x2 = x[j1];
-            x[j0] = x1 * cs[e] - x2 * sn[e];
-            x[j1] = x2 * cs[e] + x1 * sn[e];
-          }
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            lo[e] = x[e];
-            hi[e] = x[VE + e];
-          }
-          v0[u].set(lo);
-          v1[u].set(hi);
+          rot_turn<T, VE, INTER>(v0[u], v1[u], sm_cos + at[u], sm_sin + at[u]);
         }
         *reinterpret_cast<Raw*>(to[u] + o0) = v0[u].raw;
         if (second) *reinterpret_cast<Raw*>(to[u] + o1) = v1[u].raw;
@@ -234,12 +285,47 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
   }
 }
 
-// The same for pairs that lie on no 16 bytes while whole heads do: a head moves in pieces of 16 bytes through shared memory, and
-// the pairs are turned there. Accesses of 2 or 4 bytes to global memory leave too little in flight. Forward and backward in us, so /
-// staged: bf16, 100 000 tokens x 8 heads of 64, 50 turn 264 / 171 (floor 64); 30 000 x 16 of 128, 30 turn, interleaved 289 / 125 (76);
-// fp32, 30 000 x 16 of 80, 42 turn 247 / 153 (95). With accesses of 8 bytes it does not pay: bf16, 60 000 x 16 of 80, 40 turn 147 / 199.
-// Shared memory: [rows][D] values, then cos and sin.
-template <typename T, bool INTER>
+// The same for pairs that lie on no 16 bytes: values move through shared memory in pieces as wide as they can be, and the pairs are
+// turned there. Narrow accesses to global memory leave too little in flight and cost addresses (32 bits here where they reach).
+// Heads on 16 bytes are taken one by one (100 000 tokens x 8 of 64, 50 turn: 106 us, as runs 112); others where they lie side by
+// side, as one run of a token. Forward and backward in us, narrow accesses / staged (floor):
+//   bf16, 100 000 tokens x 8 heads of 64, 50 turn            264 / 107 (64)      30 000 x 16 of 80, 40 turn (8 bytes)   141 / 107 (95)
+//   bf16, 30 000 x 16 of 128, 30 turn, interleaved           289 / 84 (76)       fp32, 30 000 x 16 of 96, 36 turn       178 / 119 (114)
+//   bf16, 100 000 x 8 of 75, 50 turn, runs in 8 bytes        338 / 150 (74)      fp32, 50 000 x 16 of 33, 20 turn       160 / 86 (65)
+// With 16 bytes it does not pay: bf16, 60 000 x 16 of 96, all turn 142 / 153.
+// Shared memory: [tokens][heads][D] values, then cos and sin.
+template <int BYTES>
+__device__ __forceinline__ void rot_piece_in(void* to, const char* from) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(BYTES) : "memory");
+}
+
+// The runs of the block's tokens between memory and shared memory, in pieces of BYTES.
+template <typename T, int BYTES, bool OUT>
+__device__ __forceinline__ void rot_runs(const RotaryArgs& a, const RotPlace<T>& place, long long t0, int tokens, int heads, char* values) {
+  const int pieces = heads * a.D * static_cast<int>(sizeof(T)) / BYTES, of_q = a.heads[0] * a.D * static_cast<int>(sizeof(T)) / BYTES;
+#pragma unroll 4
+  for (int j = threadIdx.x; j < tokens * pieces; j += ROT_THREADS) {
+    const int tok = a.by_run.of(j), piece = j - tok * pieces;
+    const bool k = piece >= of_q;
+    const int h = k ? a.heads[0] : 0, at = (piece - (k ? of_q : 0)) * BYTES;
+    if constexpr (OUT) {
+      using Raw = typename RotRaw<BYTES>::type;
+      *reinterpret_cast<Raw*>(reinterpret_cast<char*>(place.to(a, t0, tok, h)) + at) = *reinterpret_cast<const Raw*>(values + j * BYTES);
+    } else {
+      rot_piece_in<BYTES>(values + j * BYTES, reinterpret_cast<const char*>(place.from(a, t0, tok, h)) + at);
+    }
+  }
+}
+template <typename T, bool OUT>
+__device__ __forceinline__ void rot_runs(const RotaryArgs& a, const RotPlace<T>& place, long long t0, int tokens, int heads, void* values) {
+  char* v = static_cast<char*>(values);
+  if (a.run == 16) rot_runs<T, 16, OUT>(a, place, t0, tokens, heads, v);
+  else if (a.run == 8) rot_runs<T, 8, OUT>(a, place, t0, tokens, heads, v);
+  else rot_runs<T, 4, OUT>(a, place, t0, tokens, heads, v);
+}
+
+template <typename T, int VE, bool INTER, bool RUNS>
 __global__ void __launch_bounds__(ROT_THREADS, 4)
 rotary_staged_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ __align__(16) uint8_t rot_smem[];
@@ -247,57 +333,72 @@ rotary_staged_kernel(const __grid_constant__ RotaryArgs a) {
   const int half = a.R >> 1, heads = a.heads[0] + a.heads[1];
   const long long t0 = static_cast<long long>(blockIdx.x) * a.tile;
   const int tokens = static_cast<int>(min(static_cast<long long>(a.tile), a.tokens - t0));
-  const int rows = tokens * heads, pieces = a.D * static_cast<int>(sizeof(T)) / 16;
+  const int rows = tokens * heads, pieces = RUNS ? 1 : a.D * static_cast<int>(sizeof(T)) / 16;
   T* values = reinterpret_cast<T*>(rot_smem);
-  float* sm_cos = reinterpret_cast<float*>(rot_smem + static_cast<size_t>(a.tile) * heads * a.D * sizeof(T));
+  float* sm_cos = reinterpret_cast<float*>(rot_smem + ((static_cast<size_t>(a.tile) * heads * a.D * sizeof(T) + 15) & ~size_t(15)));
   float* sm_sin = sm_cos + a.tile * half;
   const int stride = ROT_THREADS / pieces, first = threadIdx.x / pieces, piece = threadIdx.x - first * pieces;
-  auto place = [&](int row, const long long (&sb)[2], const long long (&st)[2], const long long (&sh)[2], const void* const* base) {
-    const int tok = row / heads, h = row - tok * heads, k = h >= a.heads[0];
-    const long long t = t0 + tok;
-    long long b = 0, s = t;
-    if (a.seq != a.tokens) {
-      b = t / a.seq;
-      s = t - b * a.seq;
-    }
-    return static_cast<const T*>(base[k]) + b * sb[k] + s * st[k] + (h - (k ? a.heads[0] : 0)) * sh[k];
-  };
-  if (first < stride) {
+  const RotPlace<T> place(a, t0);
+  if constexpr (RUNS) {
+    rot_runs<T, false>(a, place, t0, tokens, heads, values);
+  } else if (first < stride) {
     for (int row = first; row < rows; row += stride) {
-      const T* from = place(row, a.xb, a.xt, a.xh, a.x);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(values + row * a.D) + piece * 16),
-                   "l"(reinterpret_cast<const char*>(from) + piece * 16)
-                   : "memory");
+      const int tok = a.by_heads.of(row);
+      const T* from = place.from(a, t0, tok, row - tok * heads);
+      rot_piece_in<16>(reinterpret_cast<char*>(values + row * a.D) + piece * 16, reinterpret_cast<const char*>(from) + piece * 16);
     }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
   rotary_angles(a, t0, tokens, half, sm_cos, sm_sin);
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  // all pairs of all rows: pair after pair of a row, row after row
-  for (int j = threadIdx.x; j < rows * half; j += ROT_THREADS) {
-    const int row = j / half, i = j - row * half, at = row / heads * half + i;
-    T* x = values + row * a.D;
-    const int j0 = INTER ? 2 * i : i, j1 = INTER ? 2 * i + 1 : i + half;
-    const float x1 = static_cast<float>(x[j0]), x2 = static_cast<float>(x[j1]), co = sm_cos[at], sn = sm_sin[at];
-    x[j0] = static_cast<T>(x1 * co - x2 * sn);      // (to the nearest)
-    x[j1] = static_cast<T>(x2 * co + x1 * sn);
+  // a thread turns the same VE pairs of every so many-th head
+  const int items = half / VE, across = ROT_THREADS / items, from = threadIdx.x / items, i = (threadIdx.x - from * items) * VE;
+  if (from < across) {
+    for (int row = from; row < rows; row += across) {
+      const int at = a.by_heads.of(row) * half + i;
+      T* p0 = values + row * a.D + (INTER ? 2 * i : i);
+      T* p1 = p0 + (INTER ? VE : half);
+      RotVec<T, VE> v0, v1;
+      v0.raw = *reinterpret_cast<const typename RotVec<T, VE>::Raw*>(p0);
+      v1.raw = *reinterpret_cast<const typename RotVec<T, VE>::Raw*>(p1);
+      rot_turn<T, VE, INTER>(v0, v1, sm_cos + at, sm_sin + at);
+      *reinterpret_cast<typename RotVec<T, VE>::Raw*>(p0) = v0.raw;
+      *reinterpret_cast<typename RotVec<T, VE>::Raw*>(p1) = v1.raw;
+    }
   }
   __syncthreads();
-  if (first < stride) {
+  if constexpr (RUNS) {
+    rot_runs<T, true>(a, place, t0, tokens, heads, values);
+  } else if (first < stride) {
     for (int row = first; row < rows; row += stride) {
-      T* to = const_cast<T*>(place(row, a.yb, a.yt, a.yh, a.y));
+      const int tok = a.by_heads.of(row);
+      T* to = place.to(a, t0, tok, row - tok * heads);
       *reinterpret_cast<uint4*>(reinterpret_cast<char*>(to) + piece * 16) =
           *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(values + row * a.D) + piece * 16);
     }
   }
 }
 
+template <typename T, int VE, bool INTER>
+static cudaError_t launch_staged(const RotaryArgs& a, unsigned blocks, size_t smem, cudaStream_t st) {
+  const bool chained = a.tokens * (a.heads[0] + a.heads[1]) * a.D <= CHAIN_ELEMENTS;
+  return a.run ? launch_when(chained, rotary_staged_kernel<T, VE, INTER, true>, blocks, ROT_THREADS, smem, st, a)
+               : launch_when(chained, rotary_staged_kernel<T, VE, INTER, false>, blocks, ROT_THREADS, smem, st, a);
+}
+
+template <typename T, int VE>
+static cudaError_t launch_staged(const RotaryArgs& a, int interleaved, unsigned blocks, size_t smem, cudaStream_t st) {
+  return interleaved ? launch_staged<T, VE, true>(a, blocks, smem, st) : launch_staged<T, VE, false>(a, blocks, smem, st);
+}
+
+// (in accesses of 4 or 2 where pairs and heads are multiples of that)
 template <typename T>
 static cudaError_t launch_staged(const RotaryArgs& a, int interleaved, unsigned blocks, size_t smem, cudaStream_t st) {
-  const bool chained = a.tokens * (a.heads[0] + a.heads[1]) * a.D <= CHAIN_ELEMENTS;
-  return interleaved ? launch_when(chained, rotary_staged_kernel<T, true>, blocks, ROT_THREADS, smem, st, a)
-                     : launch_when(chained, rotary_staged_kernel<T, false>, blocks, ROT_THREADS, smem, st, a);
+  const int half = a.R / 2;
+  if (half % 4 == 0 && a.D % 4 == 0) return launch_staged<T, 4>(a, interleaved, blocks, smem, st);
+  if (half % 2 == 0 && a.D % 2 == 0) return launch_staged<T, 2>(a, interleaved, blocks, smem, st);
+  return launch_staged<T, 1>(a, interleaved, blocks, smem, st);
 }
 
 template <typename T, int VE>
@@ -372,19 +473,43 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
   };
   while (ve > 1 && !fits(ve)) ve /= 2;
   const int half = R / 2, heads = q_heads + k_heads;
-  bool whole = D * size % 16 == 0;       // heads on 16 bytes
+  // for narrow pairs: heads on 16 bytes, or heads side by side in pieces of 16, 8 or 4 bytes (of 2: bf16, 100 000 tokens x 10 heads of
+  // 37, 2 turn 340 us, by narrow accesses 202)
+  bool whole = D * size % 16 == 0;
+  int run = 16;
   for (int j = 0; j < (k_heads ? 2 : 1); ++j) {
-    const long long all = a.xb[j] | a.xt[j] | a.xh[j] | a.yb[j] | a.yt[j] | a.yh[j];
-    whole &= all * size % 16 == 0 && reinterpret_cast<uintptr_t>(a.x[j]) % 16 == 0 && reinterpret_cast<uintptr_t>(a.y[j]) % 16 == 0;
+    const long long tokens_at = a.xb[j] | a.xt[j] | a.yb[j] | a.yt[j], all = tokens_at | a.xh[j] | a.yh[j];
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.x[j]) | reinterpret_cast<uintptr_t>(a.y[j]);
+    whole &= all * size % 16 == 0 && at % 16 == 0;
+    if (a.heads[j] > 1 && (a.xh[j] != D || a.yh[j] != D)) run = 0;
+    while (run && (tokens_at * size % run || at % run || static_cast<long long>(a.heads[j]) * D * size % run)) run /= 2;
   }
+  if (whole || run < 4) run = 0;
+  a.by_half = RotDiv(half);
+  a.by_heads = RotDiv(heads);
+  auto reach = [&]() {      // (once the tile is known)
+    a.near = 1;
+    for (int j = 0; j < (k_heads ? 2 : 1); ++j) {
+      const long long t[] = {a.xt[j], a.yt[j]}, h[] = {a.xh[j], a.yh[j]}, b[] = {a.xb[j], a.yb[j]};
+      for (int w = 0; w < 2; ++w) {
+        const long long most = 0x7fffffffLL;
+        if ((batch > 1 && b[w] != seq * t[w]) || t[w] > most || h[w] > most || t[w] * a.tile + h[w] * a.heads[j] > most) a.near = 0;
+      }
+      a.xt32[j] = static_cast<int>(a.xt[j]); a.xh32[j] = static_cast<int>(a.xh[j]);
+      a.yt32[j] = static_cast<int>(a.yt[j]); a.yh32[j] = static_cast<int>(a.yh[j]);
+    }
+  };
   const long long token_bytes = static_cast<long long>(heads) * D * size + 2 * half * 4;       // values, cos and sin
-  if (ve * size <= 4 && whole && token_bytes <= ROT_STAGED) {
+  if (ve * size <= 8 && (whole || run) && token_bytes <= ROT_STAGED) {
+    a.run = run;
+    if (run) a.by_run = RotDiv(static_cast<uint32_t>(heads * D * size / run));
     const long long even = (a.tokens + 147) / 148;      // (few tokens: over all multiprocessors)
     a.tile = static_cast<int>(ROT_STAGED / token_bytes);
     if (a.tile > even) a.tile = static_cast<int>(even);
+    reach();
     const long long blocks = (a.tokens + a.tile - 1) / a.tile;
     if (blocks > 0x7fffffffLL) return -2;
-    const size_t smem = static_cast<size_t>(a.tile) * token_bytes;
+    const size_t smem = static_cast<size_t>(a.tile) * token_bytes + 16;      // (cos and sin start on 16 bytes)
     const unsigned n = static_cast<unsigned>(blocks);
     const cudaError_t e = dtype == 0   ? launch_staged<__nv_bfloat16>(a, c.interleaved, n, smem, st)
                           : dtype == 1 ? launch_staged<__half>(a, c.interleaved, n, smem, st)

@@ -177,6 +177,30 @@ def test_in_place_leaves_the_rest(cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,Hk,D,n,row,at", [(4, 4, 75, 25, 904, 0), (4, 2, 75, 37, 900, 4), (2, 4, 75, 3, 1000, 8), (8, 8, 33, 10, 1000, 0), (6, 2, 34, 1, 600, 2),
+                                            (3, 1, 64, 25, 520, 8), (2, 2, 80, 20, 480, 16), (1, 1, 10, 5, 24, 4), (16, 16, 128, 31, 6200, 8)])
+@pytest.mark.parametrize("dtype", [BF, torch.float16, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_heads_that_lie_side_by_side(H, Hk, D, n, row, at, dtype, interleaved, cuda_status):
+    """Pairs narrower than 16 bytes in heads that move in pieces of 4, 8 or 16 bytes, in rows of tokens with something before, between and
+    behind them, which stays as it is where the heads are turned in place."""
+    T = 211
+    first = torch.randn(T, row, device="cuda").to(dtype)
+    pos, w = torch.randint(0, 3000, (T,), device="cuda"), _w(n, "cuda")
+    cut = lambda t: (t[:, at:at + H * D].view(T, H, D), t[:, row - Hk * D:].view(T, Hk, D))
+    a, b = K.rotary(*cut(first), pos, w, factor=1.2, interleaved=interleaved)
+    for got, t in zip((a, b), cut(first)):
+        _close(got, t, pos, w, factor=1.2, interleaved=interleaved)
+    here = first.clone()
+    K.rotary(*cut(here), pos, w, factor=1.2, interleaved=interleaved, out=cut(here))
+    assert all(torch.equal(s, t) for s, t in zip(cut(here), (a, b)))
+    for t in (here, first):
+        for part in cut(t):
+            part.zero_()
+    assert torch.equal(here, first)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n", [24, 25])
 def test_given_outputs_of_other_strides(n, cuda_status):
     """Outputs inside wider rows, and one that starts where the input does but with other strides."""
