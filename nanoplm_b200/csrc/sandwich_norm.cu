@@ -919,7 +919,9 @@ static int sw_launch(const SandwichArgs& a, bool backward, unsigned blocks, size
 
 template <typename T, int MODE>
 static int sw_launch(const SandwichArgs& a, bool backward, unsigned blocks, size_t smem, cudaStream_t st) {
-  if (a.tpr < 32) return sw_launch<T, MODE, GATE_ANY, true>(a, backward, blocks, smem, st);
+  if constexpr (MODE != FULL) {      // (which has whole warps)
+    if (a.tpr < 32) return sw_launch<T, MODE, GATE_ANY, true>(a, backward, blocks, smem, st);
+  }
   if constexpr (MODE == FULL || MODE == WORDS) {
     if (a.gate_mode == GATE_SIGMOID) return sw_launch<T, MODE, GATE_SIGMOID, false>(a, backward, blocks, smem, st);
     if (a.gate_mode == GATE_TOKEN) return sw_launch<T, MODE, GATE_TOKEN, false>(a, backward, blocks, smem, st);
