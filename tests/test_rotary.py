@@ -275,3 +275,33 @@ def test_captured_and_on_another_stream(cuda_status):
     far = big.as_strided((4, 2, 64), (2 ** 30, 64, 1))
     far.copy_(torch.randn(4, 2, 64))
     _close(K.rotary(far, None, pos[:4], w)[0], far, pos[:4], w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,n", [(64, 25), (75, 25), (66, 10)])
+def test_narrow_pairs_past_32_bit_offsets(D, n, cuda_status):
+    """Tokens 2^30 elements apart, and tokens within 31 bits of one another."""
+    pos, w = torch.randint(0, 3000, (4,), device="cuda"), _w(n, "cuda")
+    big = torch.empty(3 * 2 ** 30 + 2 * D, dtype=BF, device="cuda")
+    for apart in (2 ** 30, 2 ** 28 + 2):
+        far = big.as_strided((4, 2, D), (apart, D, 1))
+        far.copy_(torch.randn(4, 2, D))
+        got = K.rotary(far, None, pos, w)[0]
+        _close(got, far, pos, w)
+        assert torch.equal(got, K.rotary(far.contiguous(), None, pos, w)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,n", [(64, 25), (75, 30), (34, 10)])
+def test_narrow_pairs_in_batches(D, n, cuda_status):
+    """[B, S, H, D]: batches behind one another, in another order, between others, and one for all; positions of their own or for all."""
+    B, S, H = 3, 53, 4
+    w = _w(n, "cuda")
+    full = torch.randn(2 * B, S, H, D, device="cuda").to(BF)
+    orders = (full[:B], full[::2], torch.randn(B, H, S, D, device="cuda").to(BF).transpose(1, 2), full[:1].expand(B, S, H, D),
+              torch.randn(S, B, H, D, device="cuda").to(BF).transpose(0, 1), full[:B, :, 1:3])
+    for q in orders:
+        for pos in (torch.randint(0, 999, (B, S), device="cuda"), torch.randint(0, 999, (S,), device="cuda")):
+            a, b = K.rotary(q, full[B:, :, :2], pos, w)
+            _close(a, q, pos.expand(B, S), w)
+            _close(b, full[B:, :, :2], pos.expand(B, S), w)

@@ -282,6 +282,23 @@ def test_rows_past_32_bit_offsets(C, cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,C,apart", [(BF, 1001, 2 ** 30 + 1), (F16, 1002, 2 ** 30 + 6), (F32, 131, 2 ** 29 + 3)])
+def test_rows_by_words_past_32_bit_offsets(dtype, C, apart, cuda_status):
+    """Rows that lie between words or 16 bytes, far from one another: the results of the same rows put together."""
+    big = torch.zeros(3 * apart + C, dtype=dtype, device="cuda")
+    far = big.as_strided((4, C), (apart, 1))
+    far.copy_(torch.randn(4, C))
+    near = far.contiguous()
+    f, dy = torch.randn(4, C, device="cuda").to(dtype), torch.randn(4, C, device="cuda").to(dtype)
+    a = K.sandwich_fwd(far, f, None, None, gate=far, sigmoid=True)
+    b = K.sandwich_fwd(near, f, None, None, gate=near, sigmoid=True)
+    x = K.sandwich_bwd(dy, far, far, f, a[2], None, None, gate=far, sigmoid=True)
+    y = K.sandwich_bwd(dy, near, near, f, b[2], None, None, gate=near, sigmoid=True)
+    for s, t in zip(a + x, b + y):
+        assert torch.equal(s, t)
+
+
+@pytest.mark.gpu
 def test_rows_without_variance_and_large_means(cuda_status):
     """Constant rows are zeros behind a LayerNorm, and a mean a thousand times the deviation costs no more than the cast did."""
     T, C = 6, 384
