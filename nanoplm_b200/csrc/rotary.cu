@@ -11,6 +11,8 @@
 // bits for every position that a 32-bit integer holds.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace nplm {
@@ -45,9 +47,11 @@ struct RotaryArgs {
   long long seq;
   int D, R, tile;                   // tile: tokens a block
   int in_place;                     // the channels from R on are there already
-  int near;                         // batches follow one another, and a tile's offsets in a tensor fit in 31 bits
+  int near;                         // batches follow one another, and tokens and strides are numbers of 31 bits
   int xt32[2], xh32[2], yt32[2], yh32[2];
   RotDiv by_half, by_heads, by_run; // by_run: pieces of a token
+  RotDiv by_items;                  // (items of a head; the heads that a block takes at a time, and whole tokens in them)
+  int across, step_t;
   int run;                          // bytes of a piece of a run; 0: heads are no runs
 };
 
@@ -116,8 +120,27 @@ __device__ __forceinline__ void rot_split(const RotaryArgs& a, long long t, long
   }
 }
 
-// Where a head of the block's token `tok` lies: by 32-bit offsets from the block's first token where they reach (64-bit products
-// for each of both places were half of the instructions of narrow accesses).
+// Where head h of token t is read and written. NEAR: by products of 32 bits where they reach: 55 424 tokens of 12 + 12 heads of 64,
+// bf16, both ways 124 -> 122 us, 32 768 of 16 + 4 heads of 128, fp16 119 -> 115; narrow accesses lose by it (100 000 of 10 heads of 37,
+// 2 turn: 181 -> 202).
+template <typename T, bool NEAR>
+__device__ __forceinline__ void rot_head(const RotaryArgs& a, long long t, int h, const T*& from, T*& to) {
+  const int k = h >= a.heads[0], hh = h - (k ? a.heads[0] : 0);
+  if (NEAR && a.near) {
+    const int at = static_cast<int>(t);
+    from = static_cast<const T*>(k ? a.x[1] : a.x[0]) + (static_cast<long long>(at) * (k ? a.xt32[1] : a.xt32[0]) +
+                                                         static_cast<long long>(hh) * (k ? a.xh32[1] : a.xh32[0]));
+    to = static_cast<T*>(k ? a.y[1] : a.y[0]) + (static_cast<long long>(at) * (k ? a.yt32[1] : a.yt32[0]) +
+                                                 static_cast<long long>(hh) * (k ? a.yh32[1] : a.yh32[0]));
+    return;
+  }
+  long long b, s;
+  rot_split(a, t, b, s);
+  from = static_cast<const T*>(a.x[k]) + b * a.xb[k] + s * a.xt[k] + hh * a.xh[k];
+  to = static_cast<T*>(a.y[k]) + b * a.yb[k] + s * a.yt[k] + hh * a.yh[k];
+}
+
+// The same for a kernel that has registers for the places of a block's first token: `tok` tokens on.
 template <typename T>
 struct RotPlace {
   const T *x0, *x1;
@@ -132,17 +155,19 @@ struct RotPlace {
     const bool k = h >= a.heads[0];
     const int hh = h - (k ? a.heads[0] : 0);
     if (a.near) return (k ? x1 : x0) + (tok * (k ? a.xt32[1] : a.xt32[0]) + hh * (k ? a.xh32[1] : a.xh32[0]));
-    long long b, s;
-    rot_split(a, t0 + tok, b, s);
-    return static_cast<const T*>(a.x[k]) + b * a.xb[k] + s * a.xt[k] + hh * a.xh[k];
+    const T* from;
+    T* to;
+    rot_head<T, false>(a, t0 + tok, h, from, to);
+    return from;
   }
   __device__ __forceinline__ T* to(const RotaryArgs& a, long long t0, int tok, int h) const {
     const bool k = h >= a.heads[0];
     const int hh = h - (k ? a.heads[0] : 0);
     if (a.near) return (k ? y1 : y0) + (tok * (k ? a.yt32[1] : a.yt32[0]) + hh * (k ? a.yh32[1] : a.yh32[0]));
-    long long b, s;
-    rot_split(a, t0 + tok, b, s);
-    return static_cast<T*>(a.y[k]) + b * a.yb[k] + s * a.yt[k] + hh * a.yh[k];
+    const T* from;
+    T* to;
+    rot_head<T, false>(a, t0 + tok, h, from, to);
+    return to;
   }
 };
 
@@ -210,8 +235,8 @@ __device__ __forceinline__ void rot_turn(RotVec<T, VE>& v0, RotVec<T, VE>& v1, c
 // VE: elements an access, a divisor of R / 2, of D - R and of all strides, with the addresses on its multiples. A thread's
 // item is VE pairs of a head (two accesses) or up to 2 VE channels behind the rotated ones. Its place in the head stays the
 // same, so that only token and head advance from item to item. Two items of 16 bytes in flight and four blocks a
-// multiprocessor, fetched before the cos and sin are formed: 55 424 tokens, 12 + 12 heads of 64, bf16, forward and backward 124 us (5.5
-// TB/s, 0.85 of the copy rate; loads behind the cos and sin 255); 32 768 tokens, 16 + 4 heads of 128 of which 32 turn, fp16, 119 us.
+// multiprocessor, fetched before the cos and sin are formed: 55 424 tokens, 12 + 12 heads of 64, bf16, forward and backward 122 us (5.6
+// TB/s, 0.86 of the copy rate; loads behind the cos and sin 255); 32 768 tokens, 16 + 4 heads of 128 of which 32 turn, fp16, 115 us.
 template <typename T, int VE, bool INTER>
 __global__ void __launch_bounds__(ROT_THREADS, 4)
 rotary_kernel(const __grid_constant__ RotaryArgs a) {
@@ -226,12 +251,12 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
   const int rot = half / VE;                                          // items a head: pairs,
   const int behind = a.in_place ? 0 : (a.D - a.R + 2 * VE - 1) / (2 * VE);   // and what is copied
   const int per_head = rot + behind;
-  const int stride = ROT_THREADS / per_head;                          // heads that the block takes at a time
-  const int first = threadIdx.x / per_head, c = threadIdx.x - first * per_head;
+  const int stride = a.across;                                        // heads that the block takes at a time
+  const int first = a.by_items.of(threadIdx.x), c = threadIdx.x - first * per_head;
   const int heads = a.heads[0] + a.heads[1];
   const int rows = first < stride ? tokens * heads : 0;
-  const int step_t = stride / heads, step_h = stride - step_t * heads;
-  int tok = first / heads, h = first - tok * heads, row = first;
+  const int step_t = a.step_t, step_h = stride - step_t * heads;
+  int tok = a.by_heads.of(first), h = first - tok * heads, row = first;
   const bool pairs = c < rot;
   // offsets of the two accesses in a head
   const int i = c * VE;
@@ -247,12 +272,9 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     for (int u = 0; u < ROT_UNROLL; ++u) {
       to[u] = nullptr;
       if (row < rows) {
-        const int k = h >= a.heads[0];
-        const int hh = h - (k ? a.heads[0] : 0);
-        long long b, s;
-        rot_split(a, t0 + tok, b, s);
-        const T* from = static_cast<const T*>(a.x[k]) + b * a.xb[k] + s * a.xt[k] + hh * a.xh[k];
-        to[u] = static_cast<T*>(a.y[k]) + b * a.yb[k] + s * a.yt[k] + hh * a.yh[k];
+        constexpr bool NEAR = sizeof(T) * VE >= 16;
+        const T* from;
+        rot_head<T, NEAR>(a, t0 + tok, h, from, to[u]);
         at[u] = tok * half + i;
         v0[u].raw = *reinterpret_cast<const Raw*>(from + o0);
         if (second) v1[u].raw = *reinterpret_cast<const Raw*>(from + o1);
@@ -474,7 +496,7 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
   while (ve > 1 && !fits(ve)) ve /= 2;
   const int half = R / 2, heads = q_heads + k_heads;
   // for narrow pairs: heads on 16 bytes, or heads side by side in pieces of 16, 8 or 4 bytes (of 2: bf16, 100 000 tokens x 10 heads of
-  // 37, 2 turn 340 us, by narrow accesses 202)
+  // 37, 2 turn 340 us, by narrow accesses 181)
   bool whole = D * size % 16 == 0;
   int run = 16;
   for (int j = 0; j < (k_heads ? 2 : 1); ++j) {
@@ -487,18 +509,13 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
   if (whole || run < 4) run = 0;
   a.by_half = RotDiv(half);
   a.by_heads = RotDiv(heads);
-  auto reach = [&]() {      // (once the tile is known)
-    a.near = 1;
-    for (int j = 0; j < (k_heads ? 2 : 1); ++j) {
-      const long long t[] = {a.xt[j], a.yt[j]}, h[] = {a.xh[j], a.yh[j]}, b[] = {a.xb[j], a.yb[j]};
-      for (int w = 0; w < 2; ++w) {
-        const long long most = 0x7fffffffLL;
-        if ((batch > 1 && b[w] != seq * t[w]) || t[w] > most || h[w] > most || t[w] * a.tile + h[w] * a.heads[j] > most) a.near = 0;
-      }
-      a.xt32[j] = static_cast<int>(a.xt[j]); a.xh32[j] = static_cast<int>(a.xh[j]);
-      a.yt32[j] = static_cast<int>(a.yt[j]); a.yh32[j] = static_cast<int>(a.yh[j]);
-    }
-  };
+  a.near = a.tokens <= 0x7fffffffLL;
+  for (int j = 0; j < (k_heads ? 2 : 1); ++j) {
+    const long long reach = a.xt[j] | a.yt[j] | a.xh[j] | a.yh[j];
+    a.near &= reach <= 0x7fffffffLL && (batch == 1 || (a.xb[j] == seq * a.xt[j] && a.yb[j] == seq * a.yt[j]));
+    a.xt32[j] = static_cast<int>(a.xt[j]); a.xh32[j] = static_cast<int>(a.xh[j]);
+    a.yt32[j] = static_cast<int>(a.yt[j]); a.yh32[j] = static_cast<int>(a.yh[j]);
+  }
   const long long token_bytes = static_cast<long long>(heads) * D * size + 2 * half * 4;       // values, cos and sin
   if (ve * size <= 8 && (whole || run) && token_bytes <= ROT_STAGED) {
     a.run = run;
@@ -507,7 +524,8 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
     const long long even = (a.tokens + 591) / 592;
     a.tile = static_cast<int>(ROT_STAGED / token_bytes);
     if (a.tile > even) a.tile = static_cast<int>(even);
-    reach();
+    for (int j = 0; j < (k_heads ? 2 : 1); ++j)      // (a tile's offsets are of 31 bits)
+      a.near &= std::max(a.xt[j], a.yt[j]) * a.tile + std::max(a.xh[j], a.yh[j]) * a.heads[j] <= 0x7fffffffLL;
     const long long blocks = (a.tokens + a.tile - 1) / a.tile;
     if (blocks > 0x7fffffffLL) return -2;
     const size_t smem = static_cast<size_t>(a.tile) * token_bytes + 16;      // (cos and sin start on 16 bytes)
@@ -524,6 +542,9 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
   if (tile > ROT_PAIRS / half) tile = ROT_PAIRS / half;
   if (tile < 1) tile = 1;
   a.tile = tile;
+  a.by_items = RotDiv(per_head);
+  a.across = ROT_THREADS / per_head;
+  a.step_t = a.across / heads;
   const long long blocks = (a.tokens + tile - 1) / tile;
   if (blocks > 0x7fffffffLL) return -2;
   const unsigned n = static_cast<unsigned>(blocks);
