@@ -320,21 +320,22 @@ __device__ __forceinline__ void at_pack(const float (&v)[8], float low, uint32_t
   }
   const float lift = at_lift<SIGNED>(e);
   float a[8];
+  uint32_t u[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = v[i] * lift;
+  for (int i = 0; i < 8; ++i) {
+    a[i] = v[i] * lift;
+    u[i] = __float_as_uint(a[i]) + r[i];
+  }
   if (!(low * lift >= AT_LEAST)) {
-    // Some are below code 1: they become the value of code 1, or that of a code 0, by the rule of at_codes, and are not rounded.
+    // Some are below code 1: they become code 1 or 0 by the rule of at_codes, without a rounding.
+    const float step = __fmul_rn(__uint_as_float((at_base<SIGNED>(e) + 1u) << 20), 9.5367431640625e-7f), far = step * -8388608.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float size = fabsf(a[i]);
-      bool up = v[i] != 0.f;
-      if (SIGNED) {     // r 2^-20 code 1 < size; r as a number: its bits behind 2^23, less that
-        const float rf = __uint_as_float(0x4b000000u | r[i]) - 8388608.f;
-        up = __fmul_rn(rf, AT_LEAST * 9.5367431640625e-7f) < size || (r[i] == 0u && up);
-      }
-      const float to = up ? copysignf(AT_LEAST, a[i]) : AT_LEAST / 1.125f;
-      r[i] = size < AT_LEAST ? 0u : r[i];
-      a[i] = size < AT_LEAST ? to : a[i];
+      // (r step with r as a number: its bits behind 2^23, less that, in one operation that rounds once)
+      const bool up = SIGNED ? __fmaf_rn(__uint_as_float(0x4b000000u | r[i]), step, far) < fabsf(v[i]) : v[i] != 0.f;
+      const uint32_t one = __float_as_uint(AT_LEAST) | (__float_as_uint(v[i]) & 0x80000000u);
+      const uint32_t to = up ? one : __float_as_uint(AT_LEAST / 1.125f);
+      u[i] = fabsf(a[i]) < AT_LEAST ? to : u[i];
     }
   }
 #pragma unroll
@@ -342,11 +343,9 @@ __device__ __forceinline__ void at_pack(const float (&v)[8], float low, uint32_t
     uint32_t t[4];
 #pragma unroll
     // (with a * 16 + r * 16 in this place nvcc 12.9 gives other top bytes than the sum has; the tests of the codes' bits show it)
-    for (int i = 0; i < 4; ++i) t[i] = (__float_as_uint(a[4 * j + i]) + r[4 * j + i]) << 4;
+    for (int i = 0; i < 4; ++i) t[i] = u[4 * j + i] << 4;
     code[j] = at_top_bytes(t[0], t[1], t[2], t[3]);
-    if (SIGNED)
-      code[j] |= 0x80808080u & at_top_bytes(__float_as_uint(a[4 * j]), __float_as_uint(a[4 * j + 1]), __float_as_uint(a[4 * j + 2]),
-                                            __float_as_uint(a[4 * j + 3]));
+    if (SIGNED) code[j] |= 0x80808080u & at_top_bytes(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
   }
 }
 
