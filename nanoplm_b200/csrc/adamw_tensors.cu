@@ -20,8 +20,8 @@
 // integer reduction a moment, and a lane has twice 4 consecutive elements, so that every access of a warp is contiguous. The
 // table of tensors travels in the launch's parameters: nothing is kept between calls, and a captured launch has its own.
 //
-// Measured: 114 M elements, fp32 gradients and a bf16 copy: 8-bit moments 419 us (6.0 TB/s, 0.93 of the copy rate, with an instruction issued in
-// 80 % of the cycles), fp32 moments 508 us (6.7 TB/s). 32 M bf16 weights and gradients at addresses off 16 bytes, 8-bit moments:
+// Measured: 114 M elements, fp32 gradients and a bf16 copy: 8-bit moments, read back afterwards, 419 us (6.0 TB/s, 0.93 of the copy
+// rate, with an instruction issued in 80 % of the cycles), fp32 moments 508 us (6.7 TB/s). 32 M bf16 weights and gradients at addresses off 16 bytes, 8-bit moments:
 // 140 us, 3.2 TB/s, bound by accesses of one element.
 #include "common.cuh"
 

@@ -463,8 +463,8 @@ extern "C" int nplm_rotary_qk(const RotaryCall* call, cudaStream_t st) {
   const RotaryCall& c = *call;
   const int q_heads = c.q_heads, k_heads = c.k_heads, D = c.D, R = c.R, dtype = c.dtype;
   const long long batch = c.batch, seq = c.seq;
-  if (batch < 0 || seq < 0 || q_heads < 1 || k_heads < 0 || q_heads > 65536 || k_heads > 65536 || D < 2 || D > 512 || R < 2 || R > D || R % 2 || dtype < 0 ||
-      dtype > 2)
+  if (batch < 0 || seq < 0 || q_heads < 1 || k_heads < 0 || q_heads > 65536 || k_heads > 65536 || D < 2 || D > 512 || R < 2 ||
+      R > D || R % 2 || dtype < 0 || dtype > 2)
     return -1;
   if (batch == 0 || seq == 0) return 0;
   RotaryArgs a;

@@ -300,7 +300,8 @@ __device__ __forceinline__ void sw_ready(uint32_t stages, int warps) {
 // the last one, may start between words; its slot is read all the same.)
 template <typename T>
 __device__ __forceinline__ const T* sw_within(const T* p, const T* ahead, long long step, uint32_t steps) {
-  const uint32_t row = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ahead)) - steps * static_cast<uint32_t>(step) * static_cast<uint32_t>(sizeof(T));
+  const uint32_t row = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ahead)) -
+                       steps * static_cast<uint32_t>(step) * static_cast<uint32_t>(sizeof(T));
   return reinterpret_cast<const T*>(reinterpret_cast<const uint8_t*>(p) + (row & 12u));
 }
 
@@ -354,7 +355,8 @@ __device__ __forceinline__ float sw_param(const void* p, int c, int param32) {
   return param32 ? static_cast<const float*>(p)[c] : Io<T>::get(static_cast<const T*>(p)[c]);
 }
 
-// Shared memory: tables post, next, scale, gate [4][tpr * 8] fp32 (where shifts differ: of even and of odd groups) | sums [groups][2][2][16] where a row has several warps | ring [groups][stages][rows][parts][C]
+// Shared memory: tables post, next, scale, gate [4][tpr * 8] fp32 (where shifts differ: of even and of odd groups) | sums
+// [groups][2][2][16] where a row has several warps | ring [groups][stages][rows][parts][C]
 __host__ __device__ constexpr int sw_sums(int tpr, int groups) { return tpr > 32 ? groups * 64 : 0; }
 __host__ __device__ constexpr int sw_sets(int mode, int C, int size, int groups) {
   return mode == WORDS && size == 2 && C % 2 && groups > 1 ? 2 : 1;
@@ -872,7 +874,8 @@ sandwich_columns_kernel(const float* __restrict__ partial, const __grid_constant
 }
 
 // Threads a row, rows a block and blocks of a pass. An SM holds 512 threads of 128 registers (backward, and rows that are read
-// channel by channel or word by word), in one block where that can be: fewer partial sums, tables and prologues. Forward 768 of 80: two blocks of 384
+// channel by channel or word by word), in one block where that can be: fewer partial sums, tables and prologues. Forward 768
+// of 80: two blocks of 384
 // (55 424 x 1024 with a gate of tokens, forward and backward: 282 us with 512 a multiprocessor forward, 263 with 768). Few rows
 // are spread over all multiprocessors.
 static int sw_shape(SandwichArgs& a, bool backward, int mode, unsigned* blocks) {
