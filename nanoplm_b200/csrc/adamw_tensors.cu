@@ -22,7 +22,8 @@
 //
 // Measured: 114 M elements, fp32 gradients and a bf16 copy: 8-bit moments, read back afterwards, 419 us (6.0 TB/s, 0.93 of the copy
 // rate, with an instruction issued in 80 % of the cycles), fp32 moments 508 us (6.7 TB/s). 32 M bf16 weights and gradients at addresses off 16 bytes, 8-bit moments:
-// 140 us, 3.2 TB/s, bound by accesses of one element.
+// 132 us, 3.4 TB/s, bound by instructions: as many an element as fp32 weights take, beside 14 instead of 22 bytes. (By single elements
+// from and to memory 139.)
 #include "common.cuh"
 
 namespace nplm {
@@ -197,11 +198,46 @@ __device__ __forceinline__ void at_fetch(T* to, const T* from, int lane) {      
       at_copy_16(reinterpret_cast<char*>(to) + j + lane * 16, reinterpret_cast<const char*>(from) + j + lane * 16);
 }
 
-// A block of a tensor with 8-bit moments in shared memory.
+// Whether a 16-bit tensor starts in the middle of a word: shared memory then holds its blocks one element on, so that words of either
+// side are words of the other.
+template <typename T>
+__device__ __forceinline__ int at_shift(const T* p) {
+  return sizeof(T) == 2 ? static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1) & 1 : 0;
+}
+// A whole block in words; with a shift the first one holds the element before the block, too, and the last one is read by half.
+template <typename T>
+__device__ __forceinline__ void at_fetch_words(T* to, const T* from, int shift, int lane) {
+  constexpr int words = AT_BLOCK * static_cast<int>(sizeof(T)) / 4;
+  const char* src = reinterpret_cast<const char*>(from - shift);
+  char* dst = reinterpret_cast<char*>(to);
+#pragma unroll
+  for (int i = 0; i < words; i += 32)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst + 4 * (i + lane))), "l"(src + 4 * (i + lane)) : "memory");
+  if (shift && lane == 0)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, 2;" ::"r"(smem_u32(dst + 4 * words)), "l"(src + 4 * words) : "memory");
+}
+// n elements of a block from shared memory (`from`, with the shift of `to`) to where they belong, lane beside lane.
+template <typename T>
+__device__ __forceinline__ void at_spread(T* to, const T* from, int shift, int n, int lane) {
+  if (sizeof(T) == 2 && n == AT_BLOCK) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(to - shift);
+    const uint32_t* r = reinterpret_cast<const uint32_t*>(from);
+#pragma unroll
+    for (int i = 0; i < AT_BLOCK / 2; i += 32)
+      if (i + lane >= shift) w[i + lane] = r[i + lane];
+    if (shift && lane < 2) to[lane * (AT_BLOCK - 1)] = from[shift + lane * (AT_BLOCK - 1)];
+  } else {
+#pragma unroll
+    for (int i = 0; i < AT_BLOCK; i += 32)
+      if (i + lane < n) to[i + lane] = from[shift + i + lane];
+  }
+}
+
+// A block of a tensor with 8-bit moments in shared memory, with room for a shift.
 template <typename P, typename G>
 struct alignas(16) AtStage {
-  P p[AT_BLOCK];
-  G g[AT_BLOCK];
+  P p[AT_BLOCK + 8];
+  G g[AT_BLOCK + 8];
   uint8_t m[AT_BLOCK], v[AT_BLOCK];
 };
 
@@ -213,7 +249,7 @@ struct AtPlace {
   __nv_bfloat16* copy;        // or null
   int rest;                   // elements from here to the end of the thread block's chunk, or of the tensor where that comes first
   int block;                  // in the moments
-  bool aligned, decays;
+  bool aligned, decays, begins;      // begins: the tensor's first block
   __device__ __forceinline__ int n() const { return rest < AT_BLOCK ? rest : AT_BLOCK; }
   __device__ __forceinline__ bool vec() const { return aligned && rest >= AT_BLOCK; }
   __device__ __forceinline__ void find(const AdamTensors& t, int chunk, int warp) {
@@ -234,6 +270,7 @@ struct AtPlace {
     if (copy != nullptr) copy += at;
     decays = t.flags[lo] & 1;
     aligned = t.flags[lo] & 2;
+    begins = off == 0;
   }
   // The warp's next block of the chunk; false behind the last.
   __device__ __forceinline__ bool next() {
@@ -260,12 +297,9 @@ __device__ __forceinline__ void at_moments(const float (&g)[8], float (&m)[8], f
     v[e + 1] = __fadd_rn(v0.y, v1.y);
   }
 }
-// p, copy: the block's first element; copy may be null. s.decay: the tensor's.
+// pv: the weights, old and then new; half: their copies. s.decay: the tensor's.
 template <typename P>
-__device__ __forceinline__ void at_weights(const P (&old)[8], const float (&m)[8], const float (&v)[8], P* p, __nv_bfloat16* copy,
-                                           int n, bool vec, const AdamScalars& s, int lane) {
-  P pv[8];
-  __nv_bfloat16 half[8];
+__device__ __forceinline__ void at_weights(P (&pv)[8], const float (&m)[8], const float (&v)[8], __nv_bfloat16 (&half)[8], const AdamScalars& s) {
   float root[8];
   if (s.eps >= 1e-15f) {      // (a second moment below fp32's normal range does not matter beside eps)
 #pragma unroll
@@ -278,12 +312,10 @@ __device__ __forceinline__ void at_weights(const P (&old)[8], const float (&m)[8
   for (int e = 0; e < 8; ++e) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root[e], s.inv_bc2, s.eps)));
-    const float pn = fmaf(-s.step, m[e] * inv, __fmul_rn(at_get<P>(old[e]), s.decay));
+    const float pn = fmaf(-s.step, m[e] * inv, __fmul_rn(at_get<P>(pv[e]), s.decay));
     pv[e] = at_put<P>(pn);
     half[e] = at_put<__nv_bfloat16>(pn);
   }
-  at_store(p, lane, n, vec, pv);
-  if (copy != nullptr) at_store(copy, lane, n, vec, half);
 }
 
 // A block with fp32 moments.
@@ -300,7 +332,10 @@ __device__ __forceinline__ void at_block(const AtPlace<P, G>& at, float* m_all, 
 #pragma unroll
   for (int e = 0; e < 8; ++e) g[e] = at_get<G>(gv[e]);
   at_moments(g, m, v, s);       // (behind the tensor m, v and g are zero, and stay so)
-  at_weights(pv, m, v, at.p, at.copy, at.n(), at.vec(), s, lane);
+  __nv_bfloat16 half[8];
+  at_weights(pv, m, v, half, s);
+  at_store(at.p, lane, at.n(), at.vec(), pv);
+  if (at.copy != nullptr) at_store(at.copy, lane, at.n(), at.vec(), half);
   at_store(mp, lane, AT_BLOCK, true, m);
   at_store(vp, lane, AT_BLOCK, true, v);
 }
@@ -350,16 +385,16 @@ __device__ __forceinline__ void at_pack(const float (&v)[8], float low, uint32_t
 }
 
 // A block with 8-bit moments, its inputs in shared memory. em, ev: its exponents, and then the new ones. p, copy: its first element.
-// mc, vc: the lane's codes. first, key: the place of its first element modulo 2^32, and what it is mixed with.
+// ps, gs: shifts of weights and gradients there. mc, vc: the lane's codes. first, key: the place of its first element modulo 2^32, and what it is mixed with.
 template <typename P, typename G>
-__device__ __forceinline__ void at_block(const AtStage<P, G>& in, P* p, __nv_bfloat16* copy, int n, bool vec, uint32_t* mc,
+__device__ __forceinline__ void at_block(AtStage<P, G>& in, int ps, int gs, P* p, __nv_bfloat16* copy, int n, bool vec, uint32_t* mc,
                                          uint32_t* vc, uint32_t first, uint32_t key, uint32_t& em, uint32_t& ev,
                                          const AdamScalars& s, int lane) {
   float m[8], v[8];
   {
     G gv[8];
     float g[8];
-    at_load(in.g, lane, AT_BLOCK, true, gv);
+    at_load(in.g + gs, lane, AT_BLOCK, gs == 0, gv);
 #pragma unroll
     for (int e = 0; e < 8; ++e) g[e] = at_get<G>(gv[e]);
     const uint32_t *sm = reinterpret_cast<const uint32_t*>(in.m) + lane, *sv = reinterpret_cast<const uint32_t*>(in.v) + lane;
@@ -372,8 +407,22 @@ __device__ __forceinline__ void at_block(const AtStage<P, G>& in, P* p, __nv_bfl
   }
   {
     P pv[8];
-    at_load(in.p, lane, AT_BLOCK, true, pv);
-    at_weights(pv, m, v, p, copy, n, vec, s, lane);
+    __nv_bfloat16 half[8];
+    at_load(in.p + ps, lane, AT_BLOCK, ps == 0, pv);
+    at_weights(pv, m, v, half, s);
+    if (vec) {
+      at_store(p, lane, n, true, pv);
+      if (copy != nullptr) at_store(copy, lane, n, true, half);
+    } else {      // through shared memory, the copies in the place of the gradients, and from there lane beside lane
+      const int cs = copy != nullptr ? at_shift(copy) : 0;
+      __nv_bfloat16* copies = reinterpret_cast<__nv_bfloat16*>(in.g);
+      __syncwarp();      // all have their gradients
+      at_store(in.p + ps, lane, AT_BLOCK, ps == 0, pv);
+      if (copy != nullptr) at_store(copies + cs, lane, AT_BLOCK, cs == 0, half);
+      __syncwarp();
+      at_spread(p, in.p, ps, n, lane);
+      if (copy != nullptr) at_spread(copy, copies, cs, n, lane);
+    }
   }
   float top_m = fabsf(m[0]), top_v = v[0], low_m = fabsf(m[0]), low_v = v[0];
 #pragma unroll
@@ -457,11 +506,16 @@ __device__ __forceinline__ void at_chunk(AtPlace<P, G> at, AtStage<P, G>* ring, 
   const G* g_next = at.g;
   const uint8_t* codes = (lane < 16 ? m_all : v_all) + first + (lane & 15) * 16;
   int left = at.rest;         // elements from the block to fetch next on
+  const int ps = WHOLE || at.aligned ? 0 : at_shift(at.p), gs = WHOLE || at.aligned ? 0 : at_shift(at.g);
+  bool begins = at.begins;
   auto fetch = [&](AtStage<P, G>& to) {
     if (WHOLE || (at.aligned && left >= AT_BLOCK)) {
       at_fetch(to.p, p_next, lane);
       at_fetch(to.g, g_next, lane);
-    } else {      // (there for the warp after its next __syncwarp)
+    } else if (left >= AT_BLOCK && !(begins && ps + gs)) {
+      at_fetch_words(to.p, p_next, ps, lane);
+      at_fetch_words(to.g, g_next, gs, lane);
+    } else {      // a tensor's ends (there for the warp after its next __syncwarp)
       P pv[8];
       G gv[8];
 #pragma unroll
@@ -471,8 +525,8 @@ __device__ __forceinline__ void at_chunk(AtPlace<P, G> at, AtStage<P, G>* ring, 
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        to.p[e * 32 + lane] = pv[e];
-        to.g[e * 32 + lane] = gv[e];
+        to.p[ps + e * 32 + lane] = pv[e];
+        to.g[gs + e * 32 + lane] = gv[e];
       }
     }
     at_copy_16((lane < 16 ? to.m : to.v) + (lane & 15) * 16, codes);
@@ -480,6 +534,7 @@ __device__ __forceinline__ void at_chunk(AtPlace<P, G> at, AtStage<P, G>* ring, 
     g_next += step;
     codes += step;
     left -= step;
+    begins = false;
   };
   if (warp < held) fetch(ring[0]);
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -500,7 +555,7 @@ __device__ __forceinline__ void at_chunk(AtPlace<P, G> at, AtStage<P, G>* ring, 
     __syncwarp();
     uint32_t em = exponents[0][j], ev = exponents[1][j];
     const int n = WHOLE || rest >= AT_BLOCK ? AT_BLOCK : rest;
-    at_block(ring[stage], p, copy, n, WHOLE || (at.aligned && n == AT_BLOCK), mc, vc, low, key, em, ev, s, lane);
+    at_block(ring[stage], ps, gs, p, copy, n, WHOLE || (at.aligned && n == AT_BLOCK), mc, vc, low, key, em, ev, s, lane);
     if (lane == 0) {
       exponents[0][j] = static_cast<uint8_t>(em);
       exponents[1][j] = static_cast<uint8_t>(ev);

@@ -193,6 +193,33 @@ def test_codes_of_extreme_and_of_far_apart_gradients(size, cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("p_type,g_type", [(F32, F32), (F32, BF), (BF, BF), (BF, F32)])
+@pytest.mark.parametrize("shifts", [(1, 1, 1), (1, 0, 0), (0, 1, 1), (2, 3, 1), (3, 2, 2), (5, 4, 7)])
+def test_tensors_at_any_address_beside_others(bits, p_type, g_type, shifts, cuda_status):
+    """Weights, gradients and copies that start at addresses of their own, between numbers that are none: the bits of the same step on
+    16 bytes, and the neighbours as they were."""
+    shapes = [(256,), (255,), (20000 + 7,), (1,), (40, 64), (8192,)]
+    params, grads, copies = _set(shapes, p_type, g_type)
+    whole = [[t.cuda() for t in ts] if ts else None for ts in (params, grads, copies)]
+    bufs, cut = [], []
+    for ts, at in zip((params, grads, copies), shifts):
+        bufs.append([torch.full((t.numel() + 16,), float("nan"), dtype=t.dtype, device="cuda") for t in ts] if ts else None)
+        cut.append([b[at:at + t.numel()].copy_(t.cuda().view(-1)).view(t.shape) for b, t in zip(bufs[-1], ts)] if ts else None)
+    sizes = [t.numel() for t in params]
+    a, b = M.TensorMoments(sizes, "cuda", bits), M.TensorMoments(sizes, "cuda", bits)
+    for t in (1, 2):
+        rng = torch.tensor([t * 7 ** 11], device="cuda")
+        for st, (p, g, c) in ((a, whole), (b, cut)):
+            st.step(p, g, _hyper(t, device="cuda"), rng=rng, copies=c)
+    assert torch.equal(a.m, b.m) and torch.equal(a.v, b.v) and (bits == 32 or torch.equal(a.scales, b.scales))
+    for x, y, buf in zip(whole, cut, bufs):
+        for s, t, around in zip(x or (), y or (), buf or ()):
+            assert torch.equal(s, t)
+            assert int(around.isnan().sum()) == 16
+
+
+@pytest.mark.gpu
 def test_more_tensors_than_a_launch_takes(cuda_status):
     shapes = [(1 + 37 * i % 900,) for i in range(301)]
     _same(*_both(shapes, F32, F32, 8, steps=1), F32)
