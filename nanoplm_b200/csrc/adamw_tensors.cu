@@ -21,9 +21,9 @@
 // table of tensors travels in the launch's parameters: nothing is kept between calls, and a captured launch has its own.
 //
 // Measured: 114 M elements, fp32 gradients and a bf16 copy: 8-bit moments, read back afterwards, 419 us (6.0 TB/s, 0.93 of the copy
-// rate, with an instruction issued in 80 % of the cycles), fp32 moments 508 us (6.7 TB/s). 32 M bf16 weights and gradients at addresses off 16 bytes, 8-bit moments:
-// 132 us, 3.4 TB/s, bound by instructions: as many an element as fp32 weights take, beside 14 instead of 22 bytes. (By single elements
-// from and to memory 139.)
+// rate, with an instruction issued in 80 % of the cycles), fp32 moments 508 us (6.7 TB/s). 32 M bf16 weights and gradients at
+// addresses off 16 bytes, 8-bit moments: 132 us, 3.4 TB/s, bound by instructions: as many an element as fp32 weights take, beside
+// 14 instead of 22 bytes. (By single elements from and to memory 139.)
 #include "common.cuh"
 
 namespace nplm {
