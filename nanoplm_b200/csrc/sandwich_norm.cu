@@ -840,6 +840,7 @@ sandwich_bwd_kernel(const __grid_constant__ SandwichArgs a) {
 }
 
 // out[k][c] (= or +=) the sum over the blocks' partial sums, in their order. kind: 0 none, 1 bf16, 2 fp16, 3 fp32, 4 add to fp32.
+// A kind is a block's, so no two outputs may share memory.
 struct ColumnSums {
   void* out[4];
   int kind[4];

@@ -391,6 +391,12 @@ def norm(x, w, eps: float = 1e-5, rms: bool = False):
     return y.to(x.dtype)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    p, q = a.data_ptr(), b.data_ptr()
+    return p < q + b.numel() * b.element_size() and q < p + a.numel() * a.element_size()
+
+
 class _SandwichFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, post, nxt, gate, scale, eps, rms, sigmoid, with_next):
@@ -415,12 +421,21 @@ class _SandwichFn(torch.autograd.Function):
         rows = lambda t: t if t is None or t.stride(1) == 1 else t.contiguous()
         need = ctx.needs_input_grad
         wanted = (need[3] and dh is not None, need[2], need[5], need[4] and ctx.refs[3] is not None)
-        sums, add = [], []
+        sums, add, behind = [], [], []
         for p, want in zip(ctx.refs, wanted):
             running = want and _has_main_grad(p) and p.main_grad.dtype == torch.float32 and p.main_grad.is_contiguous()
+            # (one weight in two places: the kernel adds one of its sums to the running gradient, the other follows)
+            if running and any(a and _overlap(p.main_grad, s) for s, a in zip(sums, add)):
+                behind.append((p.main_grad, len(sums)))
+                running = False
+                sums.append(K._like(p.main_grad))
+            else:
+                sums.append(None if not want else p.main_grad if running else K._like(p))
             add.append(running)
-            sums.append(None if not want else p.main_grad if running else K._like(p))
         dx, df, dg = K.sandwich_bwd(rows(dy), rows(dh), x, f, stats, post, nxt, gate, scale, rms, sigmoid, sums, add)
+        for main, i in behind:
+            main.add_(sums[i])
+            sums[i] = None
         dnext, dpost, dscale, dgate = (None if a else s for s, a in zip(sums, add))
         if dg is not None:
             dgate = dg

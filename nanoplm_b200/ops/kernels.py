@@ -422,11 +422,30 @@ def sandwich_fwd(x, f, post, nxt, gate=None, scale=None, eps: float = 1e-5, rms:
 _SUM_KINDS = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
 
 
+def _sum_kinds(sums, add, C: int) -> list[int]:
+    """Checks where column sums go; what each is there (`ColumnSums` of csrc/sandwich_norm.cu). A block of the kernel reads and writes
+    each of them, so no two may share memory."""
+    kinds, spans = [], []
+    for s, a in zip(sums, add):
+        if s is None:
+            kinds.append(0)
+            continue
+        if s.numel() != C or not s.is_contiguous() or s.dtype not in _SUM_KINDS or (a and s.dtype != torch.float32):
+            raise ValueError(f"sums must be contiguous [{C}] tensors, fp32 where added to")
+        kinds.append(4 if a else _SUM_KINDS[s.dtype])
+        at = s.data_ptr()
+        spans.append((at, at + C * s.element_size()))
+    spans.sort()
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("sums share memory")
+    return kinds
+
+
 def sandwich_bwd(dy, dh, x, f, stats, post, nxt, gate=None, scale=None, rms: bool = False, sigmoid: bool = False,
                  sums=(None, None, None, None), add=(False, False, False, False)):
     """Gradients of `sandwich_fwd` from dy and dh (one of them may be None): (dx, df, dgate of a gate of tokens or None).
     sums: [C] tensors for the gradients of nxt, post, scale and a gate per channel, None where unwanted; written, or
-    with `add` (fp32 only) added to."""
+    with `add` (fp32 only) added to. No two of them may share memory."""
     mode, param32 = check_sandwich(x, f, gate, post, nxt, scale, sigmoid)
     _sandwich_rows(x, f, gate, dy, dh)
     (T, C), kind = x.shape, ROW_TYPES[x.dtype]
@@ -437,15 +456,10 @@ def sandwich_bwd(dy, dh, x, f, stats, post, nxt, gate=None, scale=None, rms: boo
             raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}, got {tuple(d.shape)} {d.dtype}")
     if stats.dtype != torch.float32 or tuple(stats.shape) != (T, 4) or not stats.is_contiguous():
         raise ValueError(f"stats must be the fp32 [{T}, 4] of the forward pass")
+    kinds = _sum_kinds(sums, add, C)
     with _device_of(x, f, gate, post, nxt, scale, dy, dh, stats, *sums):
         dx, df = _like(x), _like(x)
         dg = _like(x) if mode >= GATE_TOKEN else None
-        kinds = []
-        for s, a in zip(sums, add):
-            if s is not None and (s.numel() != C or not s.is_contiguous() or s.dtype not in _SUM_KINDS
-                                  or (a and s.dtype != torch.float32)):
-                raise ValueError(f"sums must be contiguous [{C}] tensors, fp32 where added to")
-            kinds.append(0 if s is None else 4 if a else _SUM_KINDS[s.dtype])
         partial = None
         if any(kinds) and T:
             blocks = typed("sandwich_norm", "nplm_sandwich_bwd_blocks", "li")(T, C)

@@ -109,6 +109,54 @@ def test_refusals():
         K.sandwich_bwd(x, None, x, x, torch.empty(3, 4), None, None)
 
 
+@pytest.mark.parametrize("tied", [("post", "nxt"), ("gate", "scale"), ("post", "nxt", "gate", "scale")])
+def test_one_weight_in_several_places_has_one_running_sum(tied, monkeypatch):
+    """Column sums of one kernel never go to the same memory: a parameter that is, say, post and next gets one of them added to its
+    running gradient by the kernel, and the others behind it."""
+    T, C, given = 6, 8, []
+
+    def fwd(x, f, post, nxt, gate, scale, eps, rms, sigmoid, with_next, stats):
+        y, h = _formula(x, f, post, nxt, gate, sigmoid, scale, rms)
+        return y, h, torch.zeros(T, 4)
+
+    def bwd(dy, dh, x, f, stats, post, nxt, gate, scale, rms, sigmoid, sums, add):
+        given.append([s.data_ptr() for s in sums if s is not None])
+        v = [t.detach().clone().requires_grad_(True) for t in (nxt, post, scale, gate)]
+        with torch.enable_grad():
+            out = _formula(x, f, v[1], v[0], v[3], sigmoid, v[2], rms)
+            grads = torch.autograd.grad(out, v, (dy, dh))
+        for s, a, g in zip(sums, add, grads):
+            s.copy_(s + g if a else g)
+        return torch.zeros_like(x), torch.zeros_like(f), None
+    monkeypatch.setattr(K, "sandwich_fwd", fwd)
+    monkeypatch.setattr(K, "sandwich_bwd", bwd)
+    p = _inputs(T, C, F32, "channel", True, True, "cpu")
+    dy, dh = torch.randn(T, C), torch.randn(T, C)
+    call = lambda q: ops._SandwichFn.apply(q["x"], q["f"], q["post"], q["nxt"], q["gate"], q["scale"], EPS, False, False, True)
+    for name in tied:
+        p[name] = p[tied[0]]
+    apart = {k: p[k].detach().clone().requires_grad_(True) for k in p}
+    want = sum(torch.autograd.grad(call(apart), [apart[k] for k in tied], (dy, dh)))
+    p[tied[0]].main_grad = torch.full((C,), 3.0)
+    torch.autograd.backward(call(p), (dy, dh))
+    assert len(set(given[-1])) == len(given[-1]) == 4 and p[tied[0]].grad is None
+    assert torch.allclose(p[tied[0]].main_grad - 3.0, want, rtol=1e-5, atol=1e-5)
+
+
+def test_sums_that_share_memory_are_refused():
+    x, st, buf = torch.randn(4, 8), torch.empty(4, 4), torch.zeros(20)
+    a, b = buf[:8], buf[8:16]
+    with pytest.raises(ValueError, match="CUDA"):       # apart, and for the next check to refuse
+        K.sandwich_bwd(x, None, x, x, st, None, None, sums=(a, b, None, buf[16:].view(BF)), add=(True, True, False, False))
+    for sums in ((a, a, None, None), (None, a, None, buf[4:12]), (a, None, buf[7:15], None), (a, b, None, buf[:4].view(BF)[:8])):
+        with pytest.raises(ValueError, match="share"):
+            K.sandwich_bwd(x, None, x, x, st, None, None, sums=sums, add=(False,) * 4)
+    for sums, add in (((a[:7], None, None, None), (False,) * 4), ((buf[::2][:8], None, None, None), (False,) * 4),
+                      ((a.to(BF), None, None, None), (True, False, False, False))):
+        with pytest.raises(ValueError):
+            K.sandwich_bwd(x, None, x, x, st, None, None, sums=sums, add=add)
+
+
 # ------------------------------------------------------------------------------------------- GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,C", [(1, 1), (1, 8), (2, 3), (33, 7), (150, 16), (1, 24), (301, 17), (700, 32), (37, 66), (500, 100), (149, 128),
@@ -217,6 +265,25 @@ def test_running_gradients_are_added_to(cuda_status):
     for k in names:
         assert p[k].grad is None
         assert torch.allclose(p[k].main_grad - 3.0, plain[k].float(), rtol=2 ** -7, atol=1e-4), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [("post", "nxt"), ("gate", "scale")])
+def test_running_gradient_of_a_weight_in_two_places(tied, cuda_status):
+    """Every time the sum of the gradients of two weights apart. Both are sums of T terms in fp32 here (the kernel's partial sums, the
+    same in either call), and what is compared are the roundings of three additions to numbers of at most 3 + both gradients."""
+    T, C = 700, 512
+    p = _inputs(T, C, F32, "channel", True, True, "cuda")
+    p[tied[1]] = p[tied[0]]
+    apart = {k: v.detach().clone().requires_grad_(True) for k, v in p.items()}
+    dy, dh = torch.randn(T, C, device="cuda"), torch.randn(T, C, device="cuda")
+    a, b = torch.autograd.grad(_call(apart, False, False), [apart[k] for k in tied], (dy, dh))
+    main = p[tied[0]].main_grad = torch.empty(C, device="cuda")
+    for _ in range(100):
+        main.fill_(3.0)
+        torch.autograd.backward(_call(p, False, False), (dy, dh))
+        assert p[tied[0]].grad is None
+        assert ((main - 3.0 - (a + b)).abs() <= 4 * 2.0 ** -24 * (3.0 + a.abs() + b.abs())).all()
 
 
 @pytest.mark.gpu
