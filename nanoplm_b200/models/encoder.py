@@ -453,13 +453,14 @@ class ProtEncoderMLM(nn.Module):
             for lin in lins:
                 if lin.bias is not None:
                     nn.init.zeros_(lin.bias)
-            for join, out in ((layer.attn_join, layer.attn.Wo), (layer.mlp_join, getattr(layer.mlp, "Wo", None))):
+            mlp_out = layer.mlp.experts_Wo if layer.is_moe else getattr(getattr(layer.mlp, "Wo", None), "weight", None)
+            for join, out in ((layer.attn_join, layer.attn.Wo.weight), (layer.mlp_join, mlp_out)):
                 if join is not None:
                     # a norm behind zeros multiplies the first gradients by 1 / sqrt(eps): the projection starts like the
                     # others, and the branches add up to a stream of twice the input's variance through the norm's weight
                     nn.init.constant_(join.norm_weight, (2 * cfg.num_hidden_layers) ** -0.5)
                     if out is not None:
-                        nn.init.uniform_(out.weight, -bound, bound)
+                        nn.init.uniform_(out, -bound, bound)
                     if join.gate_proj is not None:
                         nn.init.zeros_(join.gate_proj.weight)
         nn.init.uniform_(self.head.dense.weight, -bound, bound)

@@ -78,6 +78,22 @@ def test_layer_by_layer_is_what_the_joined_layers_give():
     assert sorted(seen) == ["attn_norm", "layer", "mlp_norm"] and torch.allclose(got, want, atol=1e-6)
 
 
+@pytest.mark.parametrize("gate", ["none", "channel", "token"])
+def test_first_gradients_of_a_fresh_model_are_alike(gate):
+    """A projection of zeros behind whose block a norm stands gets first gradients 1 / sqrt(eps) = 316 times as large as one whose outputs
+    have a deviation of one. As the models start, no output projection's gradient is eight times another kind's largest."""
+    torch.manual_seed(0)
+    m = ProtEncoderMLM(ModelConfig(**dict(GEOM, hidden_size=128, num_hidden_layers=4), sandwich_norm=True, residual_gate=gate,
+                                   moe={"num_experts": 4, "top_k": 2, "expert_intermediate_size": 64, "every_n_layers": 2}), ProtTokenizer())
+    ids, cu, labels = _batch(lens=(100, 128, 90))
+    m(input_ids=ids, cu_seqlens=cu, labels=labels)["loss"].backward()
+    size = {n: float(p.grad.norm()) for n, p in m.named_parameters()}
+    experts = [v for n, v in size.items() if n.endswith("experts_Wo")]
+    dense = [v for n, v in size.items() if n.endswith("Wo.weight")]
+    assert len(experts) == 2 and len(dense) == 6
+    assert max(experts) <= 8 * max(dense) and max(dense) <= 8 * max(experts), (experts, dense)
+
+
 def test_a_layer_follows_its_formula():
     m = _model(**OPTIONS[1])
     layer, rope = m.model.layers[1], m.model.rope("cpu")["sliding_attention"]
