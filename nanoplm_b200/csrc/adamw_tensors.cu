@@ -110,14 +110,16 @@ __device__ __forceinline__ uint32_t at_codes(const float* x, const uint32_t* r, 
   return four;
 }
 
-// The same for values of at least code 1 in a block with an exponent E that AT_PLAIN admits. Times 2^(96 - the block's lowest
+// The same for values of at least code 1 in a block with an exponent E that at_plain admits. Times 2^(96 - the block's lowest
 // exponent), an exact product, a value's pattern is 96 x 8 + code on bits 20 and up, and 96 x 8 = 0 modulo 256: no offset is
 // left to subtract, nor a sign to cut off, where the pattern is moved up by 4 bits and its top byte taken.
 constexpr int AT_OCTAVE = 96;
 template <bool SIGNED>
-__device__ __forceinline__ bool at_plain(uint32_t e) {        // E from which 2^(96 - lowest) is a number
+__device__ __forceinline__ bool at_plain(uint32_t e) {
+  // 2^(96 - lowest) is a number, and the lowest codes are of the normal range (with E at `below` they are patterns of subnormal numbers,
+  // which a product does not move by octaves)
   constexpr uint32_t below = SIGNED ? 15 : 31;
-  return e - below < AT_OCTAVE + 126u;
+  return e - below - 1u < AT_OCTAVE + 125u;
 }
 template <bool SIGNED>
 __device__ __forceinline__ float at_lift(uint32_t e) {

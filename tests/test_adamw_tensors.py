@@ -193,6 +193,31 @@ def test_codes_of_extreme_and_of_far_apart_gradients(size, cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("exponent", [1, 2, 14, 15, 16, 17, 30, 31, 32, 33, 150, 235, 236, 237, 238, 251, 252, 253, 254])
+@pytest.mark.parametrize("second", [False, True])
+def test_codes_at_the_ends_of_the_exponents(exponent, second, cuda_status):
+    """Blocks whose largest moment has a given exponent field, with elements in every octave down to fp32's smallest numbers, and again
+    with all of them in the block's two lowest octaves: the restatement's bits, where the kernel's two ways of coding meet and
+    where a block reaches below the normal range. With beta 0 a moment is its gradient, or the gradient's square."""
+    gen = torch.Generator().manual_seed(exponent)
+    n, below = 4096, 31 if second else 15
+    lowest = max(exponent - below, 0)
+    fields = torch.cat((torch.randint(0, exponent + 1, (n,), generator=gen), torch.randint(max(lowest - 1, 0), min(lowest + 2, exponent + 1), (n,), generator=gen)))
+    patterns = (fields << 23) + torch.randint(0, 2 ** 23, (2 * n,), generator=gen)
+    patterns[::256] = (exponent << 23) + 12345                  # the largest of the block, which no rounding takes beyond its exponent
+    patterns = torch.minimum(patterns, patterns[::256].repeat_interleave(256))
+    x = patterns.to(torch.int32).view(F32)
+    g = x.double().sqrt().float() if second else x * torch.where(torch.rand(2 * n, generator=gen) < 0.5, -1.0, 1.0)
+    a, b = M.TensorMoments([2 * n], "cpu", 8), M.TensorMoments([2 * n], "cuda", 8)
+    for t in (1, 2, 3):
+        how, rng = dict(lr=0.0, b1=0.0, b2=0.0, gs=1.0, most=0.0), torch.tensor([t * 98765432109])
+        a.step([torch.zeros(2 * n)], [g], _hyper(t, **how), rng=rng)
+        b.step([torch.zeros(2 * n, device="cuda")], [g.cuda()], _hyper(t, device="cuda", **how), rng=rng.cuda())
+        assert set(a.scales[int(second)].tolist()) == set(b.scales[int(second)].tolist()) == {exponent}
+        assert torch.equal(a.v if second else a.m, (b.v if second else b.m).cpu())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("p_type,g_type", [(F32, F32), (F32, BF), (BF, BF), (BF, F32)])
 @pytest.mark.parametrize("shifts", [(1, 1, 1), (1, 0, 0), (0, 1, 1), (2, 3, 1), (3, 2, 2), (5, 4, 7)])
