@@ -299,11 +299,12 @@ __device__ __forceinline__ void at_moments(const float (&g)[8], float (&m)[8], f
     v[e + 1] = __fadd_rn(v0.y, v1.y);
   }
 }
-// pv: the weights, old and then new; half: their copies. s.decay: the tensor's.
+// pv: the weights, old and then new; half: their copies. s.decay: the tensor's. Root and reciprocal are the approximate ones (2^-23 of
+// the value each): the update is good to 2^-20 of itself, and its sum with the weight is rounded to the weight's type.
 template <typename P>
 __device__ __forceinline__ void at_weights(P (&pv)[8], const float (&m)[8], const float (&v)[8], __nv_bfloat16 (&half)[8], const AdamScalars& s) {
   float root[8];
-  if (s.eps >= 1e-15f) {      // (a second moment below fp32's normal range does not matter beside eps)
+  if (s.eps >= s.inv_bc2 * 0x1p-38f) {      // (the root of a second moment below fp32's normal range is under 2^-25 of eps)
 #pragma unroll
     for (int e = 0; e < 8; ++e) asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root[e]) : "f"(v[e]));
   } else {

@@ -218,6 +218,26 @@ def test_codes_at_the_ends_of_the_exponents(exponent, second, cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("step", [1, 100])
+@pytest.mark.parametrize("eps", [1e-18, 1e-15, 1e-13, 1e-11, 1e-10, 1e-8])
+def test_second_moments_below_the_normal_range_beside_epsilon(eps, step, cuda_status):
+    """The update of weights of zero from moments down to fp32's smallest numbers, against the formula in 64 bits from the step's own
+    moments. Rounded: the root by 2^-23, the correction's root, its reciprocal and the product with it 3 x 2^-24, the sum 2^-24, its
+    reciprocal 2^-23, the learning rate over its correction, and two products 3 x 2^-24: below 2^-20 of the update."""
+    n = 4096
+    v = torch.exp2(-149 + 40 * torch.rand(n)).clamp(min=2.0 ** -149)
+    m = torch.randn(n).abs() * 2.0 ** -60 + 2.0 ** -61
+    st = M.TensorMoments([n], "cuda")
+    st.load([m], [v])
+    p, hyper = torch.zeros(n, device="cuda"), _hyper(step, gs=1.0, most=0.0, device="cuda")
+    hyper[3] = eps
+    st.step([p], [torch.zeros_like(p)], hyper)
+    lr, b1, b2, eps32, wd, bc1, bc2, _, _ = hyper.double()
+    want = -lr / bc1 * st.m.double() / ((st.v.double() / bc2).sqrt() + eps32)
+    assert ((p.double() - want).abs() <= 2.0 ** -20 * want.abs()).all(), float(((p.double() - want) / want).abs().max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bits", [8, 32])
 @pytest.mark.parametrize("p_type,g_type", [(F32, F32), (F32, BF), (BF, BF), (BF, F32)])
 @pytest.mark.parametrize("shifts", [(1, 1, 1), (1, 0, 0), (0, 1, 1), (2, 3, 1), (3, 2, 2), (5, 4, 7)])
