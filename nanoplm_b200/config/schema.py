@@ -226,7 +226,7 @@ class PretrainingConfig:
     shard_params: bool = False           # keep 1/N of every layer's weights per rank, gather inside the GEMMs
     nvtx_ranges: bool = False            # NVTX ranges around data / forward / backward / optimizer (for profilers)
     deterministic_attention: bool = False  # attention backward (~1.4x its time) and linear weight gradients: the same bits every run
-    optimizer_state_bits: int = 32       # 8: AdamW moments as stochastically rounded 8-bit codes, 2 bytes a parameter instead of 8
+    optimizer_state_bits: int = 32       # 8: AdamW moments as stochastically rounded 8-bit codes, 2 bytes a parameter, without fused_comm
     hf_checkpoint_files: bool = False    # also write model.safetensors + trainer_state.json (HF-Trainer layout)
 
 

@@ -108,7 +108,7 @@ pretraining:
   # shard_params: false           # shard the layers' weights over the ranks (all-gather fused into the GEMMs)
   # nvtx_ranges: false            # NVTX ranges around forward / backward / optimizer step
   # deterministic_attention: false  # attention backward and linear weight gradients bitwise reproducible (slower)
-  # optimizer_state_bits: 32      # 8: AdamW moments in 8 bits (2 bytes a parameter instead of 8)
+  # optimizer_state_bits: 32      # 8: AdamW moments in 8 bits (2 bytes a parameter instead of 8); fused_comm is then off
   # hf_checkpoint_files: false    # also write model.safetensors + trainer_state.json with every checkpoint
 
 # The native pipeline (own CUDA kernels, sharded data parallelism). `use_compile` is accepted for

@@ -28,6 +28,8 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 
+from nanoplm_b200.utils.logging import logger
+
 ALIGN = 64  # elements; 64 bf16 = 128 bytes
 
 
@@ -75,11 +77,11 @@ class ShardedEngine:
                  process_group=None, compute_dtype: torch.dtype = torch.bfloat16,
                  fused_comm: bool = False, exclude: Iterable[str] = (), decay_all: bool = False, state_bits: int = 32):
         """state_bits 8: the moments as 8-bit codes (`ops.moments`), 2 bytes an element instead of 8; the step is then one kernel
-        over all tensors, and between ranks the library's collectives move gradients and parameters."""
+        over all tensors, and between ranks the library's collectives move gradients and parameters: `fused_comm` is off, with a
+        warning."""
         if state_bits not in (8, 32):
             raise ValueError(f"optimizer states have 8 or 32 bits, got {state_bits}")
         self.state_bits = state_bits
-        fused_comm = fused_comm and state_bits == 32
         self.model = model
         self.hyper = hyper
         self.device = torch.device(device)
@@ -88,6 +90,11 @@ class ShardedEngine:
             dist.get_world_size(process_group) > 1)
         self.world = dist.get_world_size(process_group) if self.distributed else 1
         self.rank = dist.get_rank(process_group) if self.distributed else 0
+        if fused_comm and state_bits == 8:
+            fused_comm = False
+            if self.distributed and self.rank == 0:
+                logger.warning("optimizer_state_bits: 8 has no step over peer memory: fused_comm is off, gradients and parameters move "
+                               "by the library's collectives")
         self.on_cuda = self.device.type == "cuda"
         self.compute_dtype = compute_dtype if self.on_cuda else torch.float32
         # the optimizer kernels write the bf16 compute copy; an fp32 compute copy on a GPU

@@ -241,6 +241,46 @@ def test_8bit_engine_on_two_ranks():
     assert all(same for _, same, _, _ in got) and got[0][2:] == got[1][2:]
 
 
+def _spawned(target, *args, world=2):
+    """What the ranks of a gloo group put into their queue as (rank, ...), by rank."""
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=target, args=(r, world, port, q, *args)) for r in range(world)]
+    for p in procs:
+        p.start()
+    got = sorted((q.get(timeout=120) for _ in procs), key=lambda g: g[0])
+    for p in procs:
+        p.join(timeout=60)
+    return got
+
+
+def _warned_rank(rank, world, port, q):
+    import logging
+    from nanoplm_b200.utils.logging import logger
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    torch.set_num_threads(1)
+    said = []
+    handler = logging.Handler(logging.WARNING)
+    handler.emit = lambda record: said.append(record.getMessage())
+    logger.addHandler(handler)
+    counts = []
+    for kw in (dict(bits=8, fused_comm=True), dict(bits=8), dict(bits=32, fused_comm=True)):
+        said.clear()
+        _engine(_model(), **kw)
+        counts.append(sum("fused_comm" in m and "optimizer_state_bits" in m for m in said))
+    q.put((rank, counts))
+    dist.destroy_process_group()
+
+
+def test_8bit_engine_says_that_fused_comm_is_off():
+    """Once, by the first rank, where both were asked for and there are ranks to move anything between."""
+    assert _spawned(_warned_rank) == [(0, [1, 0, 0]), (1, [0, 0, 0])]
+
+
 # ------------------------------------------------------------------------------------------- GPU
 BIG = dict(hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, max_position_embeddings=256)
 
