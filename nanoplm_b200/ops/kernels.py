@@ -834,10 +834,11 @@ def check_step(params, grads, copies, decay, m, v, scales, hyper, rng, sumsq) ->
                 raise ValueError(f"{name} and the moments are on different devices")
     if copies is not None and n and params[0].dtype != torch.float32:
         raise ValueError("bf16 copies are of fp32 params")
-    if len(set(map(tensor.data_ptr, params))) != n:       # (tensors without elements have none)
-        starts = [p.data_ptr() for p, k in zip(params, sizes) if k]
-        if len(set(starts)) != len(starts):
-            raise ValueError("a tensor is listed twice")
+    for written in (params, copies):
+        if written is not None and len(set(map(tensor.data_ptr, written))) != n:       # (tensors without elements have none)
+            starts = [p.data_ptr() for p, k in zip(written, sizes) if k]
+            if len(set(starts)) != len(starts):
+                raise ValueError("a tensor is listed twice")
     if hyper.dtype != torch.float32 or hyper.numel() != 9 or not hyper.is_contiguous():
         raise ValueError("hyper must be 9 contiguous fp32 numbers")
     if sumsq is not None and (sumsq.dtype != torch.float32 or sumsq.numel() != 1):
@@ -854,7 +855,8 @@ def adamw_tensors_(params, grads, exp_avg, exp_avg_sq, hyper, *, scales=None, rn
                    sumsq=None) -> None:
     """One AdamW step (the update of `adamw_`) over a list of tensors, 128 to a launch.
 
-    params, grads: lists of contiguous tensors, fp32 or bf16 each. copies: bf16 copies of fp32 params, written too.
+    params, grads: lists of contiguous tensors, fp32 or bf16 each. copies: bf16 copies of fp32 params, written too. No two tensors that
+    are written may share memory (one that is listed twice is refused).
     decay: which tensors the weight decay acts on (None: all). exp_avg, exp_avg_sq: fp32 [blocks * 256] in the order of the
     tensors, each starting a block; or their 8-bit codes, uint8, with scales uint8 [2, blocks] (see `moment_values`) and rng,
     an int64 number that must be another one each step: codes are rounded stochastically.

@@ -120,6 +120,11 @@ def test_refusals():
         step(params=[p.to(BF) for p in params])
     with pytest.raises(ValueError):     # the same tensor twice
         M.TensorMoments([8, 8], "cpu").step([params[1]] * 2, [grads[1]] * 2, hyper)
+    two = [torch.zeros(8), torch.zeros(8)]
+    with pytest.raises(ValueError, match="twice"):     # the same copy twice, of which one would be lost
+        M.TensorMoments([8, 8], "cpu").step(two, [grads[1]] * 2, hyper, copies=[copies[1]] * 2)
+    M.TensorMoments([8, 8, 0, 0], "cpu").step(two + [torch.zeros(0)] * 2, [grads[1]] * 2 + [torch.zeros(0)] * 2, hyper,
+                                              copies=[copies[1], copies[1].clone()] + [torch.zeros(0, dtype=BF)] * 2)
     with pytest.raises(ValueError):     # not contiguous
         M.TensorMoments([16], "cpu").step([torch.zeros(4, 4).t()[:, :]], [torch.zeros(4, 4)], hyper)
     with pytest.raises(ValueError):
