@@ -366,6 +366,27 @@ def test_rows_by_words_past_32_bit_offsets(dtype, C, apart, cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [100, 256, 264, 1111])
+def test_gates_far_from_zero(C, cuda_status):
+    """fp32 rows of ones and minus ones, whose norm is 1 / sqrt(1 + eps) and whose block input is zero: y is the sigmoid alone, and the
+    gate's gradient its slope. Rounded, in units of 2^-24: the mean of the squares (a sum of equal terms) log2 C + 8, its reciprocal
+    root 4, the exponential 4, its sum with one 1, the division 1, the products of y 2 and of the gradient 4: below 32 units of either."""
+    T = 64
+    f = torch.where(torch.rand(T, C, device="cuda") < 0.5, -1.0, 1.0)
+    gate = (170 * torch.rand(T, C, device="cuda") - 85).requires_grad_(True)
+    y, _ = ops.sandwich_norm(torch.zeros_like(f), f, gate=gate, sigmoid=True, eps=EPS, rms=True, with_next=False)
+    dg, = torch.autograd.grad(y, gate, torch.ones_like(y))
+    n, v = f.double() / (1 + EPS) ** 0.5, gate.detach().double()
+    for got, want in ((y, n * torch.sigmoid(v)), (dg, n * torch.sigmoid(v) * torch.sigmoid(-v))):
+        assert ((got.double() - want).abs() <= 32 * 2.0 ** -24 * want.abs()).all(), float(((got.double() - want) / want).abs().max())
+    for v, at in ((-float("inf"), 0.0), (float("inf"), 1.0), (-200.0, 0.0), (200.0, 1.0)):
+        gate = torch.full((T, C), v, device="cuda", requires_grad=True)
+        y, _ = ops.sandwich_norm(torch.zeros_like(f), f, gate=gate, sigmoid=True, eps=EPS, rms=True, with_next=False)
+        dg, = torch.autograd.grad(y, gate, torch.ones_like(y))
+        assert (y.abs() <= at).all() and (y.abs() >= at * 0.9999).all() and not dg.any()
+
+
+@pytest.mark.gpu
 def test_rows_without_variance_and_large_means(cuda_status):
     """Constant rows are zeros behind a LayerNorm, and a mean a thousand times the deviation costs no more than the cast did."""
     T, C = 6, 384
