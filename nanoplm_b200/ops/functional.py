@@ -381,14 +381,22 @@ def norm(x, w, eps: float = 1e-5, rms: bool = False):
     """LayerNorm without bias (reference encoder norms) or RMSNorm (T5LayerNorm) over the last dim."""
     if x.is_cuda and x.dtype == BF and x.shape[-1] % 8 == 0 and x.shape[-1] <= 4096:
         return _call(_NormFn, x, w, eps, rms)
-    xf = x.float()
+    return _norm_plain(x.float(), w, eps, rms).to(x.dtype)
+
+
+def _norm_plain(x, w, eps, rms):
+    """The norm in x's own type."""
+    if w is not None:
+        w = w.to(x.dtype)
     if rms:
-        y = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
-        if w is not None:
-            y = y * w.float()
-    else:
-        y = F.layer_norm(xf, (x.shape[-1],), None if w is None else w.float(), None, eps)
-    return y.to(x.dtype)
+        y = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps)
+        return y if w is None else y * w
+    return F.layer_norm(x, (x.shape[-1],), w, None, eps)
+
+
+def _wide(dtype):
+    """What a restatement computes in: 32 bits, or the 64 of its inputs."""
+    return torch.promote_types(dtype, torch.float32)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -456,11 +464,12 @@ def sandwich_norm(x, f, post=None, next=None, *, gate=None, sigmoid: bool = Fals
     if x.is_cuda and x.dtype in K.ROW_TYPES and x.dim() == 2 and x.shape[1] <= K.SANDWICH_MAX_C:      # (checked there)
         return _call(_SandwichFn, x, f, post, next, gate, scale, eps, rms, sigmoid, with_next)
     K.check_sandwich(x, f, gate, post, next, scale, sigmoid)
-    n = norm(f.float(), post, eps, rms)
+    acc = _wide(x.dtype)
+    n = _norm_plain(f.to(acc), post, eps, rms)
     if gate is not None:
-        n = n * (torch.sigmoid(gate.float()) if sigmoid else gate.float())
-    y = n + (x.float() if scale is None else scale.float() * x.float())
-    return y.to(x.dtype), (norm(y, next, eps, rms).to(x.dtype) if with_next else None)
+        n = n * (torch.sigmoid(gate.to(acc)) if sigmoid else gate.to(acc))
+    y = n + (x.to(acc) if scale is None else scale.to(acc) * x.to(acc))
+    return y.to(x.dtype), (_norm_plain(y, next, eps, rms).to(x.dtype) if with_next else None)
 
 
 class _EmbedNormFn(torch.autograd.Function):
@@ -566,10 +575,10 @@ def rotary_frequencies(rotated: int, theta: float, scaling: dict | None = None, 
 
 
 def _rotate_plain(x, positions, frequencies, factor, interleaved):
-    R = 2 * frequencies.numel()
+    R, acc = 2 * frequencies.numel(), _wide(x.dtype)
     a = positions.double()[..., None] * frequencies
-    c, s = (factor * a.cos()).to(torch.float32)[..., None, :], (factor * a.sin()).to(torch.float32)[..., None, :]
-    r, rest = x[..., :R].float(), x[..., R:]
+    c, s = (factor * a.cos()).to(acc)[..., None, :], (factor * a.sin()).to(acc)[..., None, :]
+    r, rest = x[..., :R].to(acc), x[..., R:]
     x1, x2 = (r[..., 0::2], r[..., 1::2]) if interleaved else r.chunk(2, dim=-1)
     y1, y2 = x1 * c - x2 * s, x2 * c + x1 * s
     y = torch.stack((y1, y2), -1).flatten(-2) if interleaved else torch.cat((y1, y2), -1)

@@ -53,6 +53,17 @@ def test_restatement(D, n, interleaved):
     assert torch.equal(ops.rotary(q, positions=pos, frequencies=w, factor=1.25, interleaved=interleaved), a)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_64_bit_heads_are_turned_in_64_bits(interleaved):
+    """To the last bits: cos, sin and the factor with them 3 roundings, the two products and their sum 3."""
+    q, pos, w = torch.randn(7, 3, 10, dtype=torch.float64, requires_grad=True), torch.randint(0, 9000, (7,)), _w(4)
+    how = dict(factor=1.25, interleaved=interleaved)
+    got = ops.rotary(q, positions=pos, frequencies=w, **how)
+    want, size = _exact(q.detach(), pos, w, **how)
+    assert got.dtype == torch.float64 and ((got - want).abs() <= 16 * 2.0 ** -53 * size).all()
+    assert torch.autograd.gradcheck(lambda t: ops.rotary(t, positions=pos, frequencies=w, **how), [q])
+
+
 def test_plain_frequencies_are_those_of_the_tables():
     cos, sin = ops.rope_tables(100, 64, 10000.0, "cpu")
     w, factor = ops.rotary_frequencies(64, 10000.0)

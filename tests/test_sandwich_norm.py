@@ -90,6 +90,18 @@ def test_restatement(gate, sigmoid, rms):
     _check(_inputs(5, 24, F32, gate, True, True, "cpu"), sigmoid, rms)
 
 
+@pytest.mark.parametrize("gate,sigmoid", [("none", False), ("channel", False), ("token", True)])
+@pytest.mark.parametrize("rms", [False, True])
+def test_64_bit_rows_are_computed_in_64_bits(gate, sigmoid, rms):
+    """Outputs to the last bits (rows of 9 numbers: some 40 roundings of 2^-53 of numbers below 100), gradients against differences."""
+    p = _inputs(4, 9, torch.float64, gate, True, True, "cpu")
+    y, h = _call(p, sigmoid, rms)
+    for got, want in zip((y, h), _formula(p["x"], p["f"], p["post"], p["nxt"], p["gate"], sigmoid, p["scale"], rms)):
+        assert got.dtype == torch.float64 and ((got - want).abs() <= 40 * 2.0 ** -53 * 100).all()
+    names = [k for k in p if p[k] is not None]
+    assert torch.autograd.gradcheck(lambda *a: _call(p | dict(zip(names, a)), sigmoid, rms), [p[k] for k in names])
+
+
 def test_refusals():
     p = _inputs(4, 8, F32, "token", True, True, "cpu")
     x = p["x"]
