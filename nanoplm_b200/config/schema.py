@@ -71,7 +71,7 @@ class ModelConfig:
     mhc_streams: int = 1                 # 1 = plain residual, 4 = hyper-connections
     mhc_sinkhorn_iters: int = 5
     # rotary positions beyond the reference's: {"type": linear | ntk | yarn, "factor": s, "original_max_position": n} for a
-    # context s times the trained one; the part of a head's channels that rotates; pairs of neighbours instead of halves
+    # context s times the trained one (yarn with "truncate": true for models tuned with whole pairs at the blend's ends); the part of a head's channels that rotates; pairs of neighbours instead of halves
     rope_scaling: Optional[dict] = None
     rotary_fraction: float = 1.0
     rope_interleaved: bool = False
@@ -130,9 +130,11 @@ class ModelConfig:
                 raise ValueError(f"rope_scaling.factor must be at least 1, got {sc.get('factor')}")
             if kind == "yarn" and not int(sc.get("original_max_position", 0)) > 0:
                 raise ValueError("rope_scaling of type yarn needs original_max_position")
-            unknown = sorted(set(sc) - {"type", "factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor"})
+            unknown = sorted(set(sc) - {"type", "factor", "original_max_position", "beta_fast", "beta_slow", "attention_factor", "truncate"})
             if unknown:
                 raise ValueError(f"Unexpected rope_scaling keys: {', '.join(unknown)}")
+            if "truncate" in sc and (kind != "yarn" or not isinstance(sc["truncate"], bool)):
+                raise ValueError(f"rope_scaling.truncate is true or false, and for type yarn, got {sc['truncate']} with {kind}")
             self.rope_scaling = None if kind == "none" else sc
         if not 0.0 < self.rotary_fraction <= 1.0 or self.rotary_channels < 2:
             raise ValueError(f"rotary_fraction must leave 2 to {self.head_dim} rotating channels a head, got {self.rotary_fraction}")

@@ -29,7 +29,8 @@ model:
   # conv_bias: false
   # mhc_streams: 1                # 4 = manifold-constrained hyper-connections
   # mhc_sinkhorn_iters: 5
-  # rope_scaling: {type: "yarn", factor: 4.0, original_max_position: 1024}   # longer contexts: linear | ntk | yarn
+  # rope_scaling: {type: "yarn", factor: 4.0, original_max_position: 1024}   # longer contexts: linear | ntk | yarn (truncate: true
+  #                               # for models tuned with the published default: blend between whole pairs)
   # rotary_fraction: 1.0          # part of each head's channels that rotates
   # rope_interleaved: false       # rotate pairs of neighbours instead of halves
   # sandwich_norm: false          # a norm after each block as well

@@ -547,9 +547,12 @@ def rotary_frequencies(rotated: int, theta: float, scaling: dict | None = None, 
 
     scaling {"type": ..., "factor": s > 1} stretches the positions that a model was trained on (`original_max_position`)
     s-fold: "linear" divides every frequency by s; "ntk" raises theta so that the slowest pair turns s times slower and
-    the fastest as before; "yarn" (Peng et al., 2023) divides the frequencies of pairs that turn at most `beta_slow` (1) times in
-    the original context, keeps those above `beta_fast` (32) turns, blends between them linearly in the logarithm of the
-    turns, that is in the pair's index, and multiplies cos and sin by 0.1 ln s + 1 (or `attention_factor`)."""
+    the fastest as before; "yarn" divides the frequencies of pairs that turn at most `beta_slow` (1) times in the original
+    context, keeps those above `beta_fast` (32) turns, blends between them, and multiplies cos and sin by 0.1 ln s + 1 (or
+    `attention_factor`). The blend is linear in the pair's index, that is in the logarithm of the turns, as in the code
+    published with YaRN (Peng et al., 2023; the paper's own formula is linear in the turns). With `truncate` it starts and ends at whole pairs,
+    rounded outwards and kept within the head, which is that code's default and what models tuned with it expect; without, at the
+    fractional places themselves, which moves single frequencies by up to some 20 %."""
     if rotated < 2 or rotated % 2:
         raise ValueError(f"an even number of channels rotates, got {rotated}")
     at = torch.arange(0, rotated, 2, dtype=torch.float64, device=device) / rotated
@@ -569,6 +572,11 @@ def rotary_frequencies(rotated: int, theta: float, scaling: dict | None = None, 
             raise ValueError(f"beta_slow and beta_fast must be positive and in this order: {slow}, {fast}")
         turns = float(scaling["original_max_position"]) * w / (2 * math.pi)
         keep = ((turns.log() - math.log(slow)) / (math.log(fast) - math.log(slow))).clamp(0, 1)
+        if scaling.get("truncate", False):
+            first = float(scaling["original_max_position"]) / (2 * math.pi)
+            place = lambda t: rotated * math.log(first / t) / (2 * math.log(float(theta)))        # of the pair that turns t times
+            low, high = max(math.floor(place(fast)), 0), min(math.ceil(place(slow)), rotated - 1)
+            keep = 1 - ((at * (rotated / 2) - low) / max(high - low, 0.001)).clamp(0, 1)
         factor = scaling.get("attention_factor")
         return w / s * (1 - keep) + w * keep, float(0.1 * math.log(s) + 1.0 if factor is None else factor)
     raise ValueError(f"unknown rotary scaling {kind!r}: none, linear, ntk or yarn")

@@ -110,6 +110,12 @@ def test_a_layer_follows_its_formula():
     assert aux is None and torch.allclose(got, y, rtol=1e-5, atol=1e-5)
 
 
+def test_yarn_ends_its_ramp_where_the_configuration_says():
+    whole = ops.rotary_frequencies(32, 160000.0, dict(YARN, truncate=True))[0]
+    plan = _model(rope_scaling=dict(YARN, truncate=True), rope_interleaved=True).model.rope("cpu")["full_attention"]
+    assert torch.equal(plan.frequencies, whole) and not torch.equal(whole, ops.rotary_frequencies(32, 160000.0, YARN)[0])
+
+
 def test_plain_models_keep_their_tables_and_parameters():
     m = _model()
     rope = m.model.rope("cpu")["full_attention"]
@@ -129,7 +135,8 @@ def test_plain_models_keep_their_tables_and_parameters():
                                  dict(rotary_fraction=0.0), dict(rotary_fraction=1.5), dict(rotary_fraction=0.01),
                                  dict(rope_scaling={"type": "other", "factor": 2}), dict(rope_scaling={"type": "linear"}),
                                  dict(rope_scaling={"type": "linear", "factor": 0.5}), dict(rope_scaling={"type": "yarn", "factor": 2}),
-                                 dict(rope_scaling={"type": "ntk", "factor": 2, "base": 3})])
+                                 dict(rope_scaling={"type": "ntk", "factor": 2, "base": 3}), dict(rope_scaling=dict(YARN, truncate="no")),
+                                 dict(rope_scaling={"type": "linear", "factor": 2, "truncate": True})])
 def test_configurations_that_are_refused(bad):
     with pytest.raises(ValueError):
         ModelConfig(**GEOM, **bad)

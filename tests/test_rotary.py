@@ -88,6 +88,28 @@ def test_scaled_frequencies():
     assert ops.rotary_frequencies(64, 10000.0, dict(scaling, attention_factor=1.0))[1] == 1.0
 
 
+@pytest.mark.parametrize("rotated,theta,s,first", [(64, 1e4, 4.0, 1024), (128, 1e4, 8.0, 4096), (32, 1.6e5, 2.0, 64), (2, 1e4, 2.0, 64)])
+def test_yarn_with_whole_pairs_at_the_ends_of_its_ramp(rotated, theta, s, first):
+    """`truncate`: the blend goes linearly from the pair below the one that turns beta_fast times to the pair above the one that turns beta_slow
+    times, both within the head; without it from the fractional places themselves. Pair by pair, and the two differ."""
+    scaling = {"type": "yarn", "factor": s, "original_max_position": first}
+    place = lambda turns: rotated * math.log(first / (turns * 2 * math.pi)) / (2 * math.log(theta))
+    found = {}
+    for truncate in (False, True):
+        got, f = ops.rotary_frequencies(rotated, theta, dict(scaling, truncate=truncate))
+        low, high = place(32.0), place(1.0)
+        if truncate:
+            low, high = max(math.floor(low), 0), min(math.ceil(high), rotated - 1)
+        for i in range(rotated // 2):
+            w = theta ** (-2 * i / rotated)
+            slowed = min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
+            assert float(got[i]) == pytest.approx(w / s * slowed + w * (1 - slowed), rel=1e-12), i
+        assert f == pytest.approx(0.1 * math.log(s) + 1)
+        found[truncate] = got
+    assert torch.equal(found[False], ops.rotary_frequencies(rotated, theta, scaling)[0])
+    assert rotated == 2 or (found[True] / found[False] - 1).abs().max() > 0.01
+
+
 @pytest.mark.parametrize("args", [(3, 1e4), (0, 1e4), (4, 1e4, {"type": "other", "factor": 2}), (4, 1e4, {"type": "linear", "factor": 0.5}),
                                   (4, 1e4, {"type": "yarn", "factor": 2, "original_max_position": 8, "beta_fast": 1})])
 def test_frequencies_that_are_refused(args):
