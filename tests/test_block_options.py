@@ -288,6 +288,81 @@ def test_8bit_engine_says_that_fused_comm_is_off():
     assert _spawned(_warned_rank) == [(0, [1, 0, 0]), (1, [0, 0, 0])]
 
 
+def _snapshot(e):
+    """{parameter: (master weights, first moments, second moments)} of all ranks, fp64 (collective)."""
+    parts = [e._gather_full(t).double().cpu() for t in (e.master, *e._moments_flat())]
+    return {s.name: tuple(t[s.offset:s.offset + s.numel] for t in parts) for s in e.slots}
+
+
+def _gradients(e, step, ranks):
+    """One flat gradient over all slots: layers and elements of different sizes, the sum of the ranks'."""
+    total = 0
+    for r in ranks:
+        g = torch.Generator().manual_seed(1000 * step + r)
+        flat = torch.zeros(e.total)
+        for s in e.slots:
+            size = torch.exp(2 * torch.randn(1, generator=g)) * torch.exp(torch.randn(s.numel, generator=g))
+            flat[s.offset:s.offset + s.numel] = 0.05 * size * torch.randn(s.numel, generator=g)
+        total = total + flat
+    return total
+
+
+def _follows_adamw(e, before, after, grad, t, lr, world):
+    """One 8-bit step against the formula in 64 bits, from the moments that were kept before it. The gradient's scale (a norm of fp32 squares)
+    and the moments are good to 2^-18 of their terms, the weights to a few roundings more. A moment is kept as one of the two codes
+    around it, an eighth of its octave apart, or, below a block's smallest code, as that or as zero: 1.125 x 2^-15 of the octave of the block's
+    largest in first moments, and 2^-31 in second ones, where the largest may have been rounded up into the next octave."""
+    h = e.hyper
+    g_all = grad.double() / world
+    g_all = g_all * min(1.0, h.max_grad_norm / (float(g_all.norm()) + 1e-6))
+    assert [s.name for s in e.slots] == list(before) and any(s.decay for s in e.slots) and not all(s.decay for s in e.slots)
+    for s in e.slots:
+        (p0, m0, v0), (p1, m1, v1), g = before[s.name], after[s.name], g_all[s.offset:s.offset + s.numel]
+        m, v = h.beta1 * m0 + (1 - h.beta1) * g, h.beta2 * v0 + (1 - h.beta2) * g ** 2
+        terms = h.beta1 * m0.abs() + (1 - h.beta1) * g.abs()
+        denom = (v / (1 - h.beta2 ** t)).sqrt() + h.eps
+        p = p0 * (1 - lr * h.weight_decay * s.decay) - lr / (1 - h.beta1 ** t) * m / denom
+        assert ((p1 - p).abs() <= 2.0 ** -22 * p0.abs() + 2.0 ** -17 * lr / (1 - h.beta1 ** t) * terms / denom + 1e-30).all(), (s.name, t)
+        assert ((m1 - m).abs() <= m.abs() / 8 + 2.0 ** -18 * terms + 2.0 ** -14 * m.abs().max()).all(), (s.name, t)
+        assert ((v1 - v).abs() <= v * (1 / 8 + 2.0 ** -17) + 2.0 ** -30 * v.max()).all() and (v1[v > 0] > 0).all(), (s.name, t)
+
+
+def _check_steps(e, steps, rank=0, world=1):
+    lr = 3e-3
+    before = _snapshot(e)
+    for t in range(1, steps + 1):
+        e.main_grad.copy_(_gradients(e, t, [rank]))
+        e.step(lr)
+        after = _snapshot(e)
+        _follows_adamw(e, before, after, _gradients(e, t, range(world)), t, lr, world)
+        before = after
+
+
+def test_8bit_engine_follows_the_formula_step_by_step():
+    _check_steps(_engine(_model()), 30)
+
+
+def _checked_rank(rank, world, port, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    torch.set_num_threads(1)
+    e = _engine(_model())
+    crosses = [s.name for s in e.slots if s.offset < e.shard < s.offset + s.numel]
+    error = ""
+    try:
+        _check_steps(e, 8, rank, world)
+    except AssertionError as exc:
+        error = str(exc) or "no"
+    q.put((rank, len(crosses), error))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_8bit_engine_on_two_ranks_follows_the_formula():
+    """With the ranks' gradients summed, and a tensor that lies on both of them."""
+    assert _spawned(_checked_rank) == [(0, 1, ""), (1, 1, "")]
+
+
 # ------------------------------------------------------------------------------------------- GPU
 BIG = dict(hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, max_position_embeddings=256)
 
@@ -343,6 +418,14 @@ def test_training_with_all_options_on_the_gpu(cuda_status):
         K.set_attention_deterministic(False)
     # (embedding and loss-head gradients are sums in any order, and a rounding near its threshold may go the other way)
     assert (ea.master - eb.master).norm() <= 1e-3 * (ea.master).norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_8bit_engine_follows_the_formula_on_the_gpu(dtype, cuda_status):
+    e = _engine(_model(geom=BIG), "cuda:0", compute_dtype=dtype)
+    _check_steps(e, 12)
+    assert torch.equal(e.flat_params, e._gather_full(e.master).to(dtype))
 
 
 @pytest.mark.gpu
