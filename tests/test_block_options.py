@@ -444,3 +444,25 @@ def test_gradients_of_the_packed_rotation(cuda_status):
     gc, = torch.autograd.grad(yc, xc, d.cpu())
     assert torch.allclose(y.cpu(), yc, atol=1e-5) and torch.allclose(g.cpu(), gc, atol=1e-5)
     assert torch.equal(y[:, 2 * H * D:], x[:, 2 * H * D:]) and torch.equal(g[:, 2 * H * D:], d[:, 2 * H * D:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,D,n,interleaved", [(4, 64, 16, False), (3, 64, 25, True), (5, 37, 7, False), (2, 80, 40, True), (1, 512, 1, False)])
+def test_packed_rotation_is_the_rotation_of_its_parts(dtype, H, D, n, interleaved, cuda_status):
+    """In place, with the bits of `rotary` on q and k apart, both ways; values and their gradients pass as they are."""
+    T = 131
+    w, factor = ops.rotary_frequencies(2 * n, 1e4, None, "cuda")
+    how = dict(positions=torch.randint(0, 3000, (T,), device="cuda", dtype=torch.int32), frequencies=w, factor=1.3, interleaved=interleaved)
+    x = torch.randn(T, 3 * H * D, device="cuda").to(dtype).requires_grad_(True)
+    given = x * 1.0
+    at = given.data_ptr()
+    y = ops.rotary_qkv(given, H, D, **how)
+    assert y.data_ptr() == at
+    d = torch.randn(T, 3 * H * D, device="cuda").to(dtype)
+    g, = torch.autograd.grad(y, x, d)
+    q, k, v = (t.detach().contiguous().requires_grad_(True) for t in x.view(T, 3, H, D).unbind(1))
+    parts = [t.contiguous() for t in d.view(T, 3, H, D).unbind(1)]
+    out = ops.rotary(q, k, **how)
+    back = torch.autograd.grad(out, (q, k), parts[:2])
+    assert torch.equal(y.view(T, 3, H, D), torch.stack((*out, v), 1)) and torch.equal(g.view(T, 3, H, D), torch.stack((*back, parts[2]), 1))

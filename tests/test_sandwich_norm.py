@@ -378,6 +378,38 @@ def test_rows_by_words_past_32_bit_offsets(dtype, C, apart, cuda_status):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,C", [(BF, 17), (F32, 17), (F16, 40), (BF, 100), (F32, 100), (BF, 256), (F32, 264), (BF, 1001), (F16, 1002),
+                                     (F32, 1111), (BF, 2048)])
+@pytest.mark.parametrize("rms", [False, True])
+def test_infinities_and_nan_stay_in_their_rows(dtype, C, rms, cuda_status):
+    """Rows with numbers that are none or infinite come out where the formula has such numbers, and all other rows have the bits of a call
+    without them, forward and backward; an infinite gate behind a sigmoid is zero or one."""
+    T, inf, nan = 333, float("inf"), float("nan")
+    p = _inputs(T, C, dtype, "token", True, True, "cuda")
+    clean = {k: v.detach().clone().requires_grad_(True) for k, v in p.items()}
+    at = {3: ("f", inf), 4: ("f", nan), 50: ("x", inf), 51: ("x", nan), 100: ("gate", nan), 101: ("f", -inf), 331: ("x", -inf), 332: ("f", nan),
+          0: ("f", nan), 150: ("gate", inf), 151: ("gate", -inf)}
+    with torch.no_grad():
+        for row, (name, value) in at.items():
+            p[name][row, (7 * row) % C] = value
+    dy, dh = (torch.randn(T, C, device="cuda").to(dtype) for _ in range(2))
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[list(at)] = False
+
+    def run(q):
+        out = _call(q, True, rms)
+        return out + torch.autograd.grad(out, [q[k] for k in ("x", "f", "gate")], (dy, dh))
+    got = run(p)
+    assert all(torch.equal(a[rest], b[rest]) for a, b in zip(got, run(clean)))
+    d = {k: v.detach().double() for k, v in p.items()}
+    want = _formula(d["x"], d["f"], d["post"], d["nxt"], d["gate"], True, d["scale"], rms)
+    for a, b in zip(got, want):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isinf(), b.isinf())
+    for row in (150, 151):
+        assert all(a[row].isfinite().all() for a in got)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C", [100, 256, 264, 1111])
 def test_gates_far_from_zero(C, cuda_status):
     """fp32 rows of ones and minus ones, whose norm is 1 / sqrt(1 + eps) and whose block input is zero: y is the sigmoid alone, and the
