@@ -13,17 +13,18 @@
 // A second moment below code 1 is kept as code 1 (a zero would let its element step by m / eps), a first moment there as code 1
 // or zero, with the probability that keeps its mean. Codes are shifted patterns, so reading back and coding again gives the
 // same values whatever r. All of m, v and their codes is computed with separately rounded operations in the order of
-// the formulas, and gives the bits of the restatement in ops/moments.py; the quotient of p is not.
+// the formulas, and gives the bits of the restatement in ops/moments.py; the quotient of p is not (see at_weights).
 //
 // Bound by memory: fp32 weights and gradients with a bf16 copy move 18 bytes an element with 8-bit moments (p 4 + 4, g 4, copy 2,
 // codes 4, and 4 bytes a block) and 30 with fp32 ones. A warp takes a block: the block's largest pattern is then one
 // integer reduction a moment, and a lane has twice 4 consecutive elements, so that every access of a warp is contiguous. The
 // table of tensors travels in the launch's parameters: nothing is kept between calls, and a captured launch has its own.
 //
-// Measured: 114 M elements, fp32 gradients and a bf16 copy: 8-bit moments, read back afterwards, 419 us (6.0 TB/s, 0.93 of the copy
-// rate, with an instruction issued in 80 % of the cycles), fp32 moments 508 us (6.7 TB/s). 32 M bf16 weights and gradients at
-// addresses off 16 bytes, 8-bit moments: 132 us, 3.4 TB/s, bound by instructions: as many an element as fp32 weights take, beside
-// 14 instead of 22 bytes. (By single elements from and to memory 139.)
+// Measured: 114 M elements, fp32 gradients and a bf16 copy: 8-bit moments 307 us (6.7 TB/s, the copy rate, with an instruction issued
+// in 83 % of the cycles), with their values read back 420 us, and 436 where one step with one set of random numbers has been
+// repeated until most first moments are below code 1; fp32 moments 510 us (6.7 TB/s). 32 M bf16 weights and gradients at
+// addresses off 16 bytes, 8-bit moments and their values: 132 us, 3.4 TB/s, bound by instructions (one issued in 89 % of the
+// cycles): as many an element as fp32 weights take, beside 14 instead of 22 bytes. (By single elements from and to memory 139.)
 #include "common.cuh"
 
 namespace nplm {
@@ -383,7 +384,7 @@ __device__ __forceinline__ void at_pack(const float (&v)[8], float low, uint32_t
   for (int j = 0; j < 2; ++j) {
     uint32_t t[4];
 #pragma unroll
-    // (with a * 16 + r * 16 in this place nvcc 12.9 gives other top bytes than the sum has; the tests of the codes' bits show it)
+    // (the sum moved up, in this form: it is the one that the tests of the codes' bits have passed)
     for (int i = 0; i < 4; ++i) t[i] = u[4 * j + i] << 4;
     code[j] = at_top_bytes(t[0], t[1], t[2], t[3]);
     if (SIGNED) code[j] |= 0x80808080u & at_top_bytes(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);

@@ -34,8 +34,9 @@ SOURCES = [
     "adamw_tensors.cu",
 ]
 
-# Sources compiled with IEEE divisions, square roots and denormals: angles of far positions, and moments whose
-# bits the CPU restatement of the optimizer has to give again.
+# Sources compiled without fast-math: angles of far positions, and moments whose bits the CPU restatement of the optimizer has
+# to give again. Where such a source takes an approximate instruction all the same (the quotient of AdamW's update, the
+# sigmoid of 16-bit rows, reciprocal roots of norms), it names it, with its error beside it.
 IEEE_SOURCES = {"rotary.cu", "sandwich_norm.cu", "adamw_tensors.cu"}
 
 NVCC_FLAGS = [

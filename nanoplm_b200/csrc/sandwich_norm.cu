@@ -12,7 +12,8 @@
 // of a thread never change: the column sums of the backward pass stay in its registers (in a warp-a-row layout they are
 // 4 C / 32 registers a lane, which ends at 512 channels) and leave once a block, as partial sums that a second small kernel
 // adds in a fixed order: the same bits every run. Statistics, sums and the residual sum are fp32; y and h are rounded
-// once, and h is formed from the unrounded y, which the backward pass forms again from x and f.
+// once, and h is formed from the unrounded y, which the backward pass forms again from x and f. Reciprocal roots are rsqrtf, off by at
+// most 2 units in the last place; a row's own sums are off by more.
 //
 // Measured, forward and backward with a gate of tokens, bf16: 55 424 x 1024 250 us (5.9 TB/s, 0.91 of the copy rate); 13 000 x
 // 4096 361 us (0.59: a block holds one row, and its threads wait together for each sum); 55 000 x 1002 419 us (0.53) and x 1001

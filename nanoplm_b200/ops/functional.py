@@ -455,7 +455,7 @@ class _SandwichFn(torch.autograd.Function):
 def sandwich_norm(x, f, post=None, next=None, *, gate=None, sigmoid: bool = False, scale=None, eps: float = 1e-5,
                   rms: bool = False, with_next: bool = True):
     """The end of a residual block with norms before and after it: y = scale x + g norm(f) post and h = norm(y) next, for the
-    block's input x and output f, both [T, C]; returns (y, h), h None without `with_next`.
+    block's input x and output f, both [T, C]; returns (y, h), h None without `with_next`. One weight may stand in several places.
 
     post, next, scale: weights [C], or None for ones. gate: None for g = 1, weights [C], or values [T, C], of which the
     sigmoid is taken with `sigmoid`. Norms are LayerNorm without bias, or RMSNorm."""
@@ -550,9 +550,9 @@ def rotary_frequencies(rotated: int, theta: float, scaling: dict | None = None, 
     the fastest as before; "yarn" divides the frequencies of pairs that turn at most `beta_slow` (1) times in the original
     context, keeps those above `beta_fast` (32) turns, blends between them, and multiplies cos and sin by 0.1 ln s + 1 (or
     `attention_factor`). The blend is linear in the pair's index, that is in the logarithm of the turns, as in the code
-    published with YaRN (Peng et al., 2023; the paper's own formula is linear in the turns). With `truncate` it starts and ends at whole pairs,
-    rounded outwards and kept within the head, which is that code's default and what models tuned with it expect; without, at the
-    fractional places themselves, which moves single frequencies by up to some 20 %."""
+    published with YaRN (Peng et al., 2023; the paper's own formula is linear in the turns). With `truncate` it starts and
+    ends at whole pairs, rounded outwards and kept within the head, which is that code's default and what models tuned
+    with it expect; without, at the fractional places themselves, which moves single frequencies by up to some 20 %."""
     if rotated < 2 or rotated % 2:
         raise ValueError(f"an even number of channels rotates, got {rotated}")
     at = torch.arange(0, rotated, 2, dtype=torch.float64, device=device) / rotated
@@ -619,8 +619,9 @@ class _RotaryFn(torch.autograd.Function):
 def rotary(q, k=None, *, positions, frequencies, factor: float = 1.0, interleaved: bool = False):
     """Rotary positions of queries and keys [T, heads, width] or [B, S, heads, width] (widths alike, any head counts, any strides):
     (q', k'), or q' alone without k. positions: integers [T], [B, S] or [S]; frequencies (fp64) and factor from
-    `rotary_frequencies`: their 2 n first channels rotate, as pairs (i, i + n) or, interleaved, (2 i, 2 i + 1). Angles are
-    exact to fp32 for every 32-bit position: there is no table that ends."""
+    `rotary_frequencies`: their 2 n first channels rotate, as pairs (i, i + n) or, interleaved, (2 i, 2 i + 1). There is no
+    table that ends: for bf16, fp16 and fp32 on a GPU angles are within 1e-7 radians up to position 2^26 and within 5e-7 at 2^31; other
+    types, wider heads and a CPU take PyTorch's operations, with angles in 64 bits."""
     if q.is_cuda and q.dtype in K.ROW_TYPES and q.shape[-1] <= K.ROTARY_MAX_WIDTH:      # (checked there)
         out = _call(_RotaryFn, q, k, positions, frequencies, factor, interleaved, False)
         return out[0] if k is None else out
